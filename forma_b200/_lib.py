@@ -105,6 +105,10 @@ SIGNATURES = {
     "fb_attention": (C.c_int, [T, T, T, C.c_uint32, T, FbAttentionOptions, T, VP]),
     "fb_attention_low_f32": (C.c_int, [T, T, T, C.c_uint32, T, FbAttentionOptions, T, VP]),
     "fb_attention_low": (C.c_int, [T, T, T, C.c_uint32, T, FbAttentionOptions, T, VP]),
+    "fb_attention_window": (C.c_int, [T, T, T, T, C.c_uint64, C.c_uint64, FbAttentionOptions, T, VP]),
+    "fb_attention_prefix": (C.c_int, [T, T, T, T, T, T, FbAttentionOptions, T, VP]),
+    "fb_token_logprobs": (C.c_int, [T, T, T, T, T, T, T, VP]),
+    "fb_token_logprobs_grad": (C.c_int, [T, T, T, T, T, T, T, VP]),
     "fb_reduce_shape": (C.c_int, [C.c_uint32, U64P, C.c_uint32, U32P, C.c_uint32, C.c_int32, C.c_int32, U64P, U32P]),
     "fb_reduce_f32": (C.c_int, [C.c_uint32, T, U32P, C.c_uint32, C.c_int32, T, VP]),
     "fb_reduce_u32": (C.c_int, [C.c_uint32, T, U32P, C.c_uint32, C.c_int32, T, VP]),

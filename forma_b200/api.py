@@ -15,6 +15,10 @@ this module                 reference (crates/tensor-core/src/...)
                             ``*_low_f32`` methods of ``TensorLowStatsBackend`` for
                             f16/bf16 inputs (low_statistics.rs:25-57)
 ``argmax``                  new: ``Tensor::topk``'s ordering (host_tensor/similarity.rs:82)
+``attention_window``/``attention_prefix``  new: serving forms of ``attention`` (sliding window
+                            with visible first tokens; one prefix shared by a batch)
+``token_logprobs``/``token_logprobs_grad``  new: log-probability, entropy and alternatives of a
+                            row's classes in one pass, and the gradient for the logits
 ``global_sum``              ``reduce_f32(Sum, all axes)`` with rows sharded over ranks
 ==========================  =====================================================
 
@@ -377,6 +381,112 @@ def attention_low(query, key, value, mask: Optional[Mask] = None, options: Atten
     """attention_low_f32 rounded once (nearest even) to the operands' dtype
     (tensor-core/src/low_attention.rs:38-47)."""
     return _attention(lib().fb_attention_low, query, key, value, mask, options, out_dtype=query.dtype)
+
+
+# ------------------------------------------- attention over spans of keys
+
+def attention_window(query, key, value, window: int, sinks: int = 0, lengths: Optional[torch.Tensor] = None,
+                     options: AttentionOptions = AttentionOptions(), out: Optional[torch.Tensor] = None):
+    """Causal attention in which a query at position p sees its last ``window``
+    keys and the first ``sinks`` keys.
+
+    ``lengths`` (int32 holding u32, the batch dims) says how many of each
+    sequence's key rows are filled; the queries are the last of those
+    positions.  Without it every key row is filled, and query i stands at
+    ``i + options.causal``, or at ``Lk - L + i`` when that is None.  The
+    result has the operands' dtype (``out`` may be f32 instead); a query that
+    sees no key gives zeros."""
+    dev = _device(query, key, value, lengths, out)
+    if out is None:
+        dims = attention_plan(list(query.shape), list(key.shape), list(value.shape), None, options)
+        out = torch.empty(dims, dtype=query.dtype, device=dev)
+    dq, dk, dv, do = describe(query), describe(key), describe(value), describe(out)
+    dl = describe(lengths) if lengths is not None else None
+    with _on(dev) as dev_:
+        _check(lib().fb_attention_window(C.byref(dq), C.byref(dk), C.byref(dv), C.byref(dl) if dl is not None else None,
+                                         _extent(window), _extent(sinks), _attn_options(options), C.byref(do),
+                                         _stream(dev_)))
+    return out
+
+
+def attention_prefix(query, prefix_key, prefix_value, key, value, lengths: Optional[torch.Tensor] = None,
+                     options: AttentionOptions = AttentionOptions(), out: Optional[torch.Tensor] = None):
+    """Attention of a batch [B, H, L, D] that continues one shared prefix
+    [Hkv, P, D], read once for the whole batch, over each sequence's own keys
+    [B, Hkv, S, D] (causal, ``lengths`` of them filled, as in
+    :func:`attention_window`)."""
+    dev = _device(query, prefix_key, prefix_value, key, value, lengths, out)
+    if out is None:
+        dims = attention_plan(list(query.shape), list(key.shape), list(value.shape), None, options)
+        out = torch.empty(dims, dtype=query.dtype, device=dev)
+    dq, dpk, dpv, dk, dv, do = (describe(t) for t in (query, prefix_key, prefix_value, key, value, out))
+    dl = describe(lengths) if lengths is not None else None
+    with _on(dev) as dev_:
+        _check(lib().fb_attention_prefix(C.byref(dq), C.byref(dpk), C.byref(dpv), C.byref(dk), C.byref(dv),
+                                         C.byref(dl) if dl is not None else None, _attn_options(options), C.byref(do),
+                                         _stream(dev_)))
+    return out
+
+
+def _extent(n: int) -> int:
+    """A count of keys for the C ABI: refuses what would wrap to a huge u64."""
+    if n < 0:
+        raise TensorError(10, "invalid attention: window and sinks count keys")
+    return min(int(n), 2**64 - 1)
+
+
+# ------------------------------------------------- token log probabilities
+
+NO_TOKEN = -1  # FB_NO_TOKEN (0xffffffff) as an int32 target: the row's token is not scored
+
+
+@dataclass
+class TokenLogprobs:
+    """Per row: log p(target) (0 for NO_TOKEN), the entropy, log sum exp, and
+    the ``top`` likeliest classes with their log probabilities."""
+
+    logprob: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    logsumexp: torch.Tensor
+    top_logprob: Optional[torch.Tensor] = None
+    top_index: Optional[torch.Tensor] = None
+
+
+def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of the target class of each row of ``logits`` [..., V]
+    (f32, f16 or bf16), the rows' entropies, and their ``top`` likeliest
+    classes (argmax's order: IEEE total order, lowest index on ties), in one
+    pass over the logits.  ``targets`` are int32 holding u32."""
+    dev = _device(logits, targets)
+    lead = list(logits.shape[:-1])
+    f32 = dict(dtype=torch.float32, device=dev)
+    r = TokenLogprobs(torch.empty(lead, **f32) if targets is not None else None, torch.empty(lead, **f32),
+                      torch.empty(lead, **f32))
+    if top:
+        r.top_logprob = torch.empty(lead + [top], **f32)
+        r.top_index = torch.empty(lead + [top], dtype=torch.int32, device=dev)
+    d = [describe(t) if t is not None else None
+         for t in (logits, targets, r.logprob, r.entropy, r.logsumexp, r.top_logprob, r.top_index)]
+    with _on(dev) as dev_:
+        _check(lib().fb_token_logprobs(*(C.byref(x) if x is not None else None for x in d), _stream(dev_)))
+    return r
+
+
+def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, logsumexp: torch.Tensor, grad_logprob: torch.Tensor,
+                        entropy: Optional[torch.Tensor] = None, grad_entropy: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Gradient of ``sum(grad_logprob * logprob + grad_entropy * entropy)`` for
+    the logits, from :func:`token_logprobs`' ``logsumexp`` and ``entropy``, in
+    the logits' dtype.  ``out`` may be the logits themselves (in place) or an
+    f32 tensor."""
+    dev = _device(logits, targets, logsumexp, grad_logprob, entropy, grad_entropy, out)
+    if out is None:
+        out = torch.empty(list(logits.shape), dtype=logits.dtype, device=dev)
+    d = [describe(t) if t is not None else None
+         for t in (logits, targets, logsumexp, grad_logprob, entropy, grad_entropy, out)]
+    with _on(dev) as dev_:
+        _check(lib().fb_token_logprobs_grad(*(C.byref(x) if x is not None else None for x in d), _stream(dev_)))
+    return out
 
 
 # ------------------------------------------------------------- reductions

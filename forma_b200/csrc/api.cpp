@@ -447,6 +447,66 @@ int conv_impl(const fb_tensor* input, const fb_tensor* weight, const fb_conv_opt
 
 // ------------------------------------------------------------ attention
 
+// Canonical layouts (compute-cuda/src/attention_dispatch.rs:9-18): rank-2
+// operands gain a zero-stride head axis, batches broadcast with stride 0.
+// Fills the operands, output and geometry of `a`; false when the canonical
+// rank exceeds FB_MAX_RANK.
+bool canonical_attention(const AttentionPlan& plan, const View& qv, const View& kv, const View& vv, const View& out,
+                         AttnArgs* args) {
+    auto canonical = [&](const View& t, const Dims& promoted) {
+        Dims strides = t.strides;
+        if (t.dims.size() == 2) strides.insert(strides.begin(), 0);
+        const size_t lead = plan.batch.size() + 3 - promoted.size();
+        Dims s(plan.batch.size() + 3, 0);
+        for (size_t i = 0; i < promoted.size(); ++i)
+            s[lead + i] = promoted[i] == 1 && i < promoted.size() - 3 ? 0 : strides[i];
+        // Unit head/sequence/depth axes keep their stride: indices stay 0.
+        return s;
+    };
+    Dims qs = canonical(qv, plan.query), ks = canonical(kv, plan.key), vs = canonical(vv, plan.value);
+    const size_t r = plan.batch.size() + 3;
+    AttnArgs& a = *args;
+    a.q = qv.data;
+    a.k = kv.data;
+    a.v = vv.data;
+    a.out = static_cast<float*>(out.data);
+    a.dtype = qv.dtype;
+    a.row_rank = (uint32_t)(r - 1);
+    if (a.row_rank > FB_MAX_RANK) return false;
+    // Output strides in canonical form (a rank-2 output has no head axis).
+    Dims os(r, 0);
+    if (out.dims.size() == 2) {
+        os[r - 2] = out.strides[0];
+        os[r - 1] = out.strides[1];
+    } else {
+        for (size_t i = 0; i < r; ++i) os[i] = out.strides[i];
+    }
+    for (size_t i = 0; i + 1 < r; ++i) {
+        a.row_dims[i] = plan.canonical_output[i];
+        a.q_row_strides[i] = qs[i];
+        a.k_row_strides[i] = i == r - 2 ? 0 : ks[i];
+        a.v_row_strides[i] = i == r - 2 ? 0 : vs[i];
+        a.o_row_strides[i] = os[i];
+    }
+    a.q_offset = qv.offset;
+    a.k_offset = kv.offset;
+    a.v_offset = vv.offset;
+    a.o_offset = out.offset;
+    a.q_stride_d = qs[r - 1];
+    a.k_stride_key = ks[r - 2];
+    a.k_stride_d = ks[r - 1];
+    a.v_stride_key = vs[r - 2];
+    a.v_stride_d = vs[r - 1];
+    a.o_stride_d = os[r - 1];
+    a.rows = out.count / plan.value_depth;
+    a.keys = plan.keys;
+    a.depth = plan.depth;
+    a.value_depth = plan.value_depth;
+    a.group_size = plan.group_size;
+    a.scale = plan.scale;
+    return true;
+}
+
 int attention_impl(const fb_tensor* q, const fb_tensor* k, const fb_tensor* v, uint32_t mask_kind,
                    const fb_tensor* mask, fb_attention_options options, fb_tensor* output, void* stream, bool low,
                    bool round_low = false) {
@@ -496,38 +556,11 @@ int attention_impl(const fb_tensor* q, const fb_tensor* k, const fb_tensor* v, u
     };
     if (plan.keys == 0) return finish(fill_view(res, 0u, stream));
 
-    // Canonical layouts (compute-cuda/src/attention_dispatch.rs:9-18): rank-2
-    // operands gain a zero-stride head axis, batches broadcast with stride 0.
-    auto canonical = [&](const View& t, const Dims& promoted) {
-        Dims strides = t.strides;
-        if (t.dims.size() == 2) strides.insert(strides.begin(), 0);
-        const size_t lead = plan.batch.size() + 3 - promoted.size();
-        Dims s(plan.batch.size() + 3, 0);
-        for (size_t i = 0; i < promoted.size(); ++i)
-            s[lead + i] = promoted[i] == 1 && i < promoted.size() - 3 ? 0 : strides[i];
-        // Unit head/sequence/depth axes keep their stride: indices stay 0.
-        return s;
-    };
-    Dims qs = canonical(qv, plan.query), ks = canonical(kv, plan.key), vs = canonical(vv, plan.value);
-    const size_t r = plan.batch.size() + 3;
     AttnArgs a;
-    a.q = qv.data;
-    a.k = kv.data;
-    a.v = vv.data;
-    a.out = static_cast<float*>(out.data);
+    if (!canonical_attention(plan, qv, kv, vv, out, &a)) return fail(FB_ERR_INVALID_INPUT, "attention rank too large");
     a.out_low = round_low ? out.dtype : 0;
-    a.dtype = qv.dtype;
     a.mask_kind = mask_kind;
-    a.row_rank = (uint32_t)(r - 1);
-    if (a.row_rank > FB_MAX_RANK) return fail(FB_ERR_INVALID_INPUT, "attention rank too large");
-    // Output strides in canonical form (a rank-2 output has no head axis).
-    Dims os(r, 0);
-    if (out.dims.size() == 2) {
-        os[r - 2] = out.strides[0];
-        os[r - 1] = out.strides[1];
-    } else {
-        for (size_t i = 0; i < r; ++i) os[i] = out.strides[i];
-    }
+    const size_t r = plan.batch.size() + 3;
     Dims ms(r, 0);
     if (mask_kind != FB_MASK_NONE) {
         const size_t lead = r - mv.dims.size();
@@ -535,31 +568,8 @@ int attention_impl(const fb_tensor* q, const fb_tensor* k, const fb_tensor* v, u
         a.mask = mv.data;
         a.m_offset = mv.offset;
     }
-    for (size_t i = 0; i + 1 < r; ++i) {
-        a.row_dims[i] = plan.canonical_output[i];
-        a.q_row_strides[i] = qs[i];
-        a.k_row_strides[i] = i == r - 2 ? 0 : ks[i];
-        a.v_row_strides[i] = i == r - 2 ? 0 : vs[i];
-        a.m_row_strides[i] = ms[i];
-        a.o_row_strides[i] = os[i];
-    }
-    a.q_offset = qv.offset;
-    a.k_offset = kv.offset;
-    a.v_offset = vv.offset;
-    a.o_offset = out.offset;
-    a.q_stride_d = qs[r - 1];
-    a.k_stride_key = ks[r - 2];
-    a.k_stride_d = ks[r - 1];
-    a.v_stride_key = vs[r - 2];
-    a.v_stride_d = vs[r - 1];
+    for (size_t i = 0; i + 1 < r; ++i) a.m_row_strides[i] = ms[i];
     a.m_stride_key = ms[r - 1];
-    a.o_stride_d = os[r - 1];
-    a.rows = out.count / plan.value_depth;
-    a.keys = plan.keys;
-    a.depth = plan.depth;
-    a.value_depth = plan.value_depth;
-    a.group_size = plan.group_size;
-    a.scale = plan.scale;
     a.causal = plan.causal;
     a.causal_offset = plan.causal_offset;
     // 16-bit operands: tensor cores when the layout allows (fastest for
@@ -575,6 +585,178 @@ int attention_impl(const fb_tensor* q, const fb_tensor* k, const fb_tensor* v, u
     s = launch_attention_decode(a, stream);
     if (s == FB_ERR_UNSUPPORTED) s = launch_attention_simt(a, stream);
     return finish(launched(s, "attention"));
+}
+
+// Windowed attention and, with a prefix (pk and pv not null), attention over
+// a shared prefix.
+int span_impl(const fb_tensor* q, const fb_tensor* pk, const fb_tensor* pv, const fb_tensor* k, const fb_tensor* v,
+              const fb_tensor* lengths, uint64_t window, uint64_t sinks, fb_attention_options options, fb_tensor* output,
+              void* stream, bool prefix) {
+    auto invalid = [](const char* m) { return fail(FB_ERR_INVALID_ATTENTION, std::string("invalid attention: ") + m); };
+    View qv, pkv, pvv, kv, vv, lv, out;
+    FB_TRY(view_of(q, "query", &qv));
+    if (prefix) {
+        FB_TRY(view_of(pk, "prefix key", &pkv));
+        FB_TRY(view_of(pv, "prefix value", &pvv));
+    }
+    FB_TRY(view_of(k, "key", &kv));
+    FB_TRY(view_of(v, "value", &vv));
+    if (qv.dtype != FB_F32 && !is_low(qv.dtype)) return fail(FB_ERR_DTYPE, "attention needs f32, f16 or bf16 operands");
+    if (kv.dtype != qv.dtype || vv.dtype != qv.dtype || (prefix && (pkv.dtype != qv.dtype || pvv.dtype != qv.dtype)))
+        return fail(is_low(qv.dtype) ? FB_ERR_LOW_DTYPE_MISMATCH : FB_ERR_DTYPE, "attention operands must have one dtype");
+    options.has_causal = options.has_causal != 0;
+    AttentionPlan plan;
+    FB_TRY(attention_plan(qv.dims, kv.dims, vv.dims, nullptr, options, &plan));
+    if (prefix) {
+        if (qv.dims.size() != 4 || kv.dims.size() != 4 || vv.dims.size() != 4 || kv.dims[0] != qv.dims[0] ||
+            vv.dims[0] != qv.dims[0])
+            return invalid("a shared prefix needs query, key and value of rank four with one batch");
+        if (pkv.dims.size() != 3 || pvv.dims.size() != 3) return invalid("prefix key and value need rank three");
+        if (pkv.dims[0] != plan.key_heads || pvv.dims[0] != plan.key_heads || pkv.dims[2] != plan.depth ||
+            pvv.dims[2] != plan.value_depth)
+            return invalid("prefix heads and depths must be the keys' and values'");
+        if (pkv.dims[1] != pvv.dims[1]) return invalid("prefix key and value lengths must match");
+    }
+    if (window == 0) return invalid("the window must hold at least one key");
+    if (lengths) {
+        FB_TRY(view_of(lengths, "lengths", &lv));
+        if (lv.dtype != FB_U32) return fail(FB_ERR_DTYPE, "lengths must be u32");
+        if (lv.dims != plan.batch) return fail(FB_ERR_INVALID_INPUT, "lengths need the batch dims");
+        if (options.has_causal) return invalid("lengths place the queries: no causal offset");
+    }
+    const bool low_out = output && is_low(output->dtype) && output->dtype == qv.dtype;
+    FB_TRY(check_output(output, "output", plan.output, low_out ? qv.dtype : (uint32_t)FB_F32, &out));
+    if (out.count == 0) return FB_OK;
+    if (plan.keys > 0x7fffffffull || plan.queries > 0x7fffffffull || (prefix && pkv.dims[1] > 0x7fffffffull))
+        return fail(FB_ERR_INVALID_INPUT, "sequence length exceeds 2^31 - 1");
+    SpanArgs s;
+    if (!canonical_attention(plan, qv, kv, vv, out, &s.base)) return fail(FB_ERR_INVALID_INPUT, "attention rank too large");
+    s.base.out_low = low_out ? out.dtype : 0;
+    s.offset = options.has_causal ? (int64_t)options.causal : (int64_t)plan.keys - (int64_t)plan.queries;
+    // Beyond any position, a longer window or more sinks change nothing.
+    s.window = std::min<uint64_t>(window, 1ull << 33);
+    s.sinks = std::min<uint64_t>(sinks, 1ull << 32);
+    if (lengths) {
+        const Nest n = make_nest(lv.dims, lv.strides, all_axes(lv.dims.size()));
+        if (n.rank > 1) return fail(FB_ERR_INVALID_INPUT, "lengths need one stride over the batch");
+        s.lengths = static_cast<const uint32_t*>(lv.data) + lv.offset;
+        s.length_stride = n.rank ? n.strides[0] : 0;
+    }
+    if (prefix) {
+        s.pk = pkv.data, s.pv = pvv.data;
+        s.pk_offset = pkv.offset, s.pv_offset = pvv.offset;
+        s.prefix_keys = pkv.dims[1];
+        s.pk_stride_head = pkv.strides[0], s.pk_stride_key = pkv.strides[1], s.pk_stride_d = pkv.strides[2];
+        s.pv_stride_head = pvv.strides[0], s.pv_stride_key = pvv.strides[1], s.pv_stride_d = pvv.strides[2];
+    }
+    return launched(launch_span_simt(s, stream), prefix ? "shared-prefix attention" : "windowed attention");
+}
+
+// Per-row f32 input or output of the token log probabilities.
+Error row_f32(const fb_tensor* t, const char* name, const Dims& dims, bool output, RowOut* out) {
+    View v;
+    if (output) {
+        Error e = check_output(t, name, dims, FB_F32, &v);
+        if (!ok(e)) return e;
+    } else {
+        Error e = view_of(t, name, &v);
+        if (!ok(e)) return e;
+        if (v.dtype != FB_F32) return err(FB_ERR_DTYPE, std::string(name) + " must be f32");
+        if (v.dims != dims) return err(FB_ERR_INVALID_INPUT, std::string(name) + " needs the logits' leading dims");
+    }
+    *out = make_row_out(v);
+    return {};
+}
+
+Error row_targets(const fb_tensor* t, const Dims& dims, const uint32_t** data, uint64_t* offset, Nest* nest) {
+    View v;
+    Error e = view_of(t, "targets", &v);
+    if (!ok(e)) return e;
+    if (v.dtype != FB_U32) return err(FB_ERR_DTYPE, "targets must be u32");
+    if (v.dims != dims) return err(FB_ERR_INVALID_INPUT, "targets need the logits' leading dims");
+    *data = static_cast<const uint32_t*>(v.data);
+    *offset = v.offset;
+    *nest = make_nest(v.dims, v.strides, all_axes(v.dims.size()));
+    return {};
+}
+
+// The logits as rows over their last axis; their leading dims in `lead`.
+Error token_logits(const fb_tensor* t, View* in, Dims* lead, Rows* rows) {
+    Error e = view_of(t, "logits", in);
+    if (!ok(e)) return e;
+    if (in->dtype != FB_F32 && !is_low(in->dtype)) return err(FB_ERR_DTYPE, "logits must be f32, f16 or bf16");
+    if (in->dims.empty()) return err(FB_ERR_INVALID_INPUT, "logits need rank at least one");
+    if (in->dims.back() >= FB_NO_TOKEN) return err(FB_ERR_INVALID_INPUT, "classes exceed u32 indices");
+    lead->assign(in->dims.begin(), in->dims.end() - 1);
+    *rows = make_rows(*in, {(uint32_t)in->dims.size() - 1});
+    if (rows->rows != 0 && rows->cols == 0)
+        return err(FB_ERR_EMPTY_REDUCTION, "log probabilities need at least one class");
+    return {};
+}
+
+int token_logprobs_impl(const fb_tensor* logits, const fb_tensor* targets, fb_tensor* logprob, fb_tensor* entropy,
+                        fb_tensor* lse, fb_tensor* top_logprob, fb_tensor* top_index, void* stream) {
+    View in, tl, ti;
+    Dims lead;
+    TokenArgs a;
+    FB_TRY(token_logits(logits, &in, &lead, &a.logits));
+    if (logprob && !targets) return fail(FB_ERR_INVALID_INPUT, "logprob needs targets");
+    if (!top_logprob != !top_index) return fail(FB_ERR_INVALID_INPUT, "top_logprob and top_index go together");
+    if (targets) FB_TRY(row_targets(targets, lead, &a.targets, &a.target_offset, &a.target_nest));
+    if (logprob) FB_TRY(row_f32(logprob, "logprob", lead, true, &a.logprob));
+    if (entropy) FB_TRY(row_f32(entropy, "entropy", lead, true, &a.entropy));
+    if (lse) FB_TRY(row_f32(lse, "logsumexp", lead, true, &a.lse));
+    if (top_index) {
+        Dims dims = lead;
+        if (top_index->rank != lead.size() + 1) return fail(FB_ERR_INVALID_INPUT, "top_index needs the logits' rank");
+        const uint64_t k = top_index->dims[lead.size()];
+        if (k > FB_MAX_TOP || k > in.dims.back())
+            return fail(FB_ERR_INVALID_INPUT, "at most " + std::to_string(FB_MAX_TOP) + " alternatives, and no more than classes");
+        dims.push_back(k);
+        FB_TRY(check_output(top_index, "top_index", dims, FB_U32, &ti));
+        FB_TRY(check_output(top_logprob, "top_logprob", dims, FB_F32, &tl));
+        if (!is_contiguous(ti) || !is_contiguous(tl))
+            return fail(FB_ERR_INVALID_INPUT, "top_index and top_logprob must be contiguous");
+        a.top = (uint32_t)k;
+        a.top_index = static_cast<uint32_t*>(ti.data) + ti.offset;
+        a.top_logprob = static_cast<float*>(tl.data) + tl.offset;
+    }
+    if (a.logits.rows == 0 || (!logprob && !entropy && !lse && a.top == 0)) return FB_OK;
+    return launched(launch_token_logprobs(a, stream), "token log probabilities");
+}
+
+int token_logprobs_grad_impl(const fb_tensor* logits, const fb_tensor* targets, const fb_tensor* lse, const fb_tensor* gl,
+                             const fb_tensor* entropy, const fb_tensor* gh, fb_tensor* grad, void* stream) {
+    View in, out;
+    Dims lead;
+    TokenGradArgs a;
+    FB_TRY(token_logits(logits, &in, &lead, &a.logits));
+    FB_TRY(row_targets(targets, lead, &a.targets, &a.target_offset, &a.target_nest));
+    FB_TRY(row_f32(lse, "logsumexp", lead, false, &a.lse));
+    FB_TRY(row_f32(gl, "grad_logprob", lead, false, &a.g_logprob));
+    if (gh) {
+        FB_TRY(row_f32(gh, "grad_entropy", lead, false, &a.g_entropy));
+        FB_TRY(row_f32(entropy, "entropy", lead, false, &a.entropy));
+    }
+    const bool low_out = grad && is_low(grad->dtype) && grad->dtype == in.dtype;
+    FB_TRY(check_output(grad, "grad_logits", in.dims, low_out ? in.dtype : (uint32_t)FB_F32, &out));
+    if (out.count == 0) return FB_OK;
+    // An update in place reads each logit before it writes it: only the
+    // identical view may share memory.
+    auto span = [](const View& v) {
+        uint64_t hi = v.offset;
+        for (size_t i = 0; i < v.dims.size(); ++i) hi += (v.dims[i] - 1) * v.strides[i];
+        const uintptr_t base = reinterpret_cast<uintptr_t>(v.data), esz = dtype_size(v.dtype);
+        return std::make_pair(base + v.offset * esz, base + (hi + 1) * esz);
+    };
+    const auto x = span(in), o = span(out);
+    bool same = x.first == o.first && in.dtype == out.dtype;
+    for (size_t i = 0; i < in.dims.size(); ++i) same &= in.dims[i] == 1 || in.strides[i] == out.strides[i];
+    if (!same && x.first < o.second && o.first < x.second)
+        return fail(FB_ERR_INVALID_INPUT, "grad_logits overlaps the logits without being the same view");
+    a.out = make_elem_out(out, {(uint32_t)in.dims.size() - 1});
+    a.out.dtype = out.dtype;
+    return launched(launch_token_logprobs_grad(a, stream), "token log probability gradient");
 }
 
 // f64 sum of every element of an f32 view into the device double `partial`
@@ -913,6 +1095,32 @@ int fb_attention_low(const fb_tensor* query, const fb_tensor* key, const fb_tens
                      const fb_tensor* mask, fb_attention_options options, fb_tensor* output, void* stream) {
     begin_route();
     return attention_impl(query, key, value, mask_kind, mask, options, output, stream, true, true);
+}
+
+int fb_attention_window(const fb_tensor* query, const fb_tensor* key, const fb_tensor* value, const fb_tensor* lengths,
+                        uint64_t window, uint64_t sinks, fb_attention_options options, fb_tensor* output, void* stream) {
+    begin_route();
+    return span_impl(query, nullptr, nullptr, key, value, lengths, window, sinks, options, output, stream, false);
+}
+
+int fb_attention_prefix(const fb_tensor* query, const fb_tensor* prefix_key, const fb_tensor* prefix_value,
+                        const fb_tensor* key, const fb_tensor* value, const fb_tensor* lengths,
+                        fb_attention_options options, fb_tensor* output, void* stream) {
+    begin_route();
+    return span_impl(query, prefix_key, prefix_value, key, value, lengths, UINT64_MAX, 0, options, output, stream, true);
+}
+
+int fb_token_logprobs(const fb_tensor* logits, const fb_tensor* targets, fb_tensor* logprob, fb_tensor* entropy,
+                      fb_tensor* logsumexp, fb_tensor* top_logprob, fb_tensor* top_index, void* stream) {
+    begin_route();
+    return token_logprobs_impl(logits, targets, logprob, entropy, logsumexp, top_logprob, top_index, stream);
+}
+
+int fb_token_logprobs_grad(const fb_tensor* logits, const fb_tensor* targets, const fb_tensor* logsumexp,
+                           const fb_tensor* grad_logprob, const fb_tensor* entropy, const fb_tensor* grad_entropy,
+                           fb_tensor* grad_logits, void* stream) {
+    begin_route();
+    return token_logprobs_grad_impl(logits, targets, logsumexp, grad_logprob, entropy, grad_entropy, grad_logits, stream);
 }
 
 int fb_reduce_shape(uint32_t op, const uint64_t* dims, uint32_t rank, const uint32_t* axes, uint32_t n_axes,

@@ -85,7 +85,8 @@ enum ScratchSlot : int {
     SCRATCH_ATTN_SPLIT = 5,   // split-key attention partials (f64 per row and key range)
     SCRATCH_ATTN_RESULT = 6,  // f32 attention result before low rounding
     SCRATCH_COLLECTIVE = 7,   // the global sum's f64 partial, all-reduced in place
-    SCRATCH_SLOTS = 8,
+    SCRATCH_SPAN = 8,         // windowed / shared-prefix attention: key-range records and their counters
+    SCRATCH_SLOTS = 9,
 };
 void* scratch(void* stream, uint64_t bytes, int slot);
 int sm_count();
@@ -225,5 +226,51 @@ int launch_attention_simt(const AttnArgs& a, void* stream);
 // FB_ERR_UNSUPPORTED for other shapes.
 int launch_attention_decode(const AttnArgs& a, void* stream);
 int launch_attention_tc(const AttnArgs& a, void* stream);
+
+// ---- attention over spans of keys (attention_span_simt.cu, attention_span.cu) ----
+// fb_attention_window and fb_attention_prefix.  `base` holds the query, the
+// sequences' own keys and values and the output (mask and causal fields
+// unused; out_low as there).  The query of index i in batch b stands at
+// position n_b - L + i (n_b = min(lengths[b], keys)) or, without lengths,
+// at offset + i over all keys; own key j is visible to a query at position p
+// iff j < n_b, j <= p and (j > p - window or j < sinks).  prefix_keys > 0:
+// every query sees all the keys of [Hkv, prefix_keys, D] too.
+struct SpanArgs {
+    AttnArgs base;
+    const uint32_t* lengths = nullptr;  // one per batch index (row-major over the batch axes), or null
+    uint64_t length_stride = 0;
+    int64_t offset = 0;
+    uint64_t window = 0, sinks = 0;
+    const void* pk = nullptr;
+    const void* pv = nullptr;
+    uint64_t pk_offset = 0, pv_offset = 0, prefix_keys = 0;
+    uint64_t pk_stride_head = 0, pk_stride_key = 0, pk_stride_d = 0;
+    uint64_t pv_stride_head = 0, pv_stride_key = 0, pv_stride_d = 0;
+};
+// Any strides, depths and types (f32, f16, bf16); one block per query row.
+int launch_span_simt(const SpanArgs& a, void* stream);
+
+// ---- token log probabilities (token_logprobs.cu) ----
+struct TokenArgs {
+    Rows logits;                       // [rows, classes]
+    const uint32_t* targets = nullptr; // one per row (null: no logprob)
+    uint64_t target_offset = 0;
+    Nest target_nest;
+    RowOut logprob, entropy, lse;      // f32, one per row; data null: not wanted
+    float* top_logprob = nullptr;      // [rows, top], contiguous
+    uint32_t* top_index = nullptr;
+    uint32_t top = 0;
+};
+int launch_token_logprobs(const TokenArgs& a, void* stream);
+
+struct TokenGradArgs {
+    Rows logits;
+    const uint32_t* targets = nullptr;
+    uint64_t target_offset = 0;
+    Nest target_nest;
+    RowOut lse, g_logprob, entropy, g_entropy;  // f32 inputs, one per row; g_entropy.data null: no entropy term
+    ElemOut out;                                // [rows, classes], f32 or the logits' 16-bit dtype
+};
+int launch_token_logprobs_grad(const TokenGradArgs& a, void* stream);
 
 }  // namespace fb

@@ -231,6 +231,42 @@ int fb_attention_low(const fb_tensor* query, const fb_tensor* key,
                      const fb_tensor* mask, fb_attention_options options,
                      fb_tensor* output, void* stream);
 
+/* --------------------------------------- attention over spans of keys */
+
+/* Two serving forms of the attention above for causal models.  No trait
+ * method in the reference (its masks are dense tensors); operand types, head
+ * grouping, broadcasting of key/value batches, the default scale and the
+ * zeros of rows without a visible key are fb_attention's.  Q/K/V are F32, F16
+ * or BF16 of one dtype; `output` is f32, or the operands' 16-bit dtype
+ * (rounded once, nearest even).  With 16-bit operands, D = value depth in
+ * {64, 128}, contiguous depth and 16-byte aligned rows the tensor cores serve
+ * the call; other geometries run CUDA-core kernels in f64.
+ *
+ * `lengths` (NULL, or u32 of the batch dims, one stride) says how many of
+ * each sequence's key rows are filled: n_b = min(lengths[b], Lk); the rest of
+ * the cache is not read into the result, whatever it holds.  The L queries
+ * are the last L of those positions: query i stands at p = n_b - L + i.
+ * Without lengths n_b = Lk and p = i + options.causal when
+ * options.has_causal, else Lk - L + i; giving both is
+ * FB_ERR_INVALID_ATTENTION.  Keys that a query's mask hides but that another
+ * query of the call may see must hold finite values.
+ *
+ * fb_attention_window: key j is visible iff j < n_b, j <= p and
+ * (j > p - window or j < sinks): the last `window` positions and the first
+ * `sinks` keys.  window >= 1 (FB_ERR_INVALID_ATTENTION). */
+int fb_attention_window(const fb_tensor* query, const fb_tensor* key, const fb_tensor* value, const fb_tensor* lengths,
+                        uint64_t window, uint64_t sinks, fb_attention_options options, fb_tensor* output, void* stream);
+
+/* fb_attention_prefix: a batch of sequences that continue one shared prefix.
+ * query [B, H, L, D]; prefix_key [Hkv, P, D] and prefix_value [Hkv, P, Dv]
+ * are visible to every query and read once for the whole batch; key
+ * [B, Hkv, S, D] and value [B, Hkv, S, Dv] are each sequence's own keys, key
+ * j visible iff j < n_b and j <= p (positions and n_b as above, counted
+ * within the sequence's own keys).  P or S may be 0. */
+int fb_attention_prefix(const fb_tensor* query, const fb_tensor* prefix_key, const fb_tensor* prefix_value,
+                        const fb_tensor* key, const fb_tensor* value, const fb_tensor* lengths,
+                        fb_attention_options options, fb_tensor* output, void* stream);
+
 /* -------------------------------------------------------------- reduction */
 
 /* reduction_shape / mean_shape (tensor-core/src/reduction.rs:44-72). */
@@ -350,6 +386,45 @@ int fb_moments(const fb_tensor* input, const uint32_t* axes, uint32_t n_axes,
 int fb_layer_norm(const fb_tensor* input, const uint32_t* axes,
                   uint32_t n_axes, float epsilon, fb_tensor* output,
                   void* stream);
+
+/* ------------------------------------------------ token log probabilities */
+
+#define FB_NO_TOKEN 0xffffffffu /* a target that is not scored */
+#define FB_MAX_TOP 64           /* most alternatives per row */
+
+/* One pass over logits [..., V] (F32, F16 or BF16) for a scored token per
+ * row.  No trait method in the reference, where it is log_softmax, a gather,
+ * a reduction and Tensor::topk (tensor-core/src/host_tensor/similarity.rs:82).
+ * With lse = log sum_v e^x_v and p_v = e^(x_v - lse):
+ *   logprob[...]        = x_target - lse; 0 where the target is FB_NO_TOKEN,
+ *                         NaN where it is another value >= V
+ *   entropy[...]        = -sum_v p_v log p_v (0 log 0 = 0: a class at -inf
+ *                         adds nothing)
+ *   logsumexp[...]      = lse
+ *   top_index[..., k], top_logprob[..., k] = the k likeliest classes in
+ *                         fb_argmax's order (IEEE total order, lowest index
+ *                         on ties) and their x - lse
+ * Outputs are f32 (top_index u32), sums are f32 or wider; each output may be
+ * NULL (top_* together; targets may be NULL without logprob).  top_* are
+ * contiguous; k <= min(V, FB_MAX_TOP).  A row that holds NaN or +inf, or only
+ * -inf, gives NaN as log_softmax does.  V = 0 with rows is
+ * FB_ERR_EMPTY_REDUCTION. */
+int fb_token_logprobs(const fb_tensor* logits, const fb_tensor* targets, fb_tensor* logprob, fb_tensor* entropy,
+                      fb_tensor* logsumexp, fb_tensor* top_logprob, fb_tensor* top_index, void* stream);
+
+/* Its gradient for the logits, from the forward call's logsumexp and entropy:
+ *   grad_logits = grad_logprob ([v = target] - p_v)
+ *                 - grad_entropy p_v (log p_v + entropy)
+ * f32 per-row inputs of the leading dims, any strides; grad_entropy NULL: no
+ * entropy term (entropy is not read and may be NULL).  A term whose row
+ * gradient is 0, and the first term of a row whose target is FB_NO_TOKEN (or
+ * another value >= V), is 0 whatever the row holds.  `grad_logits` has the
+ * logits' dims and dtype (or f32), any layout that addresses each element
+ * once; it may share memory with the logits only as the identical view of
+ * the same dtype (an in-place update; FB_ERR_INVALID_INPUT otherwise). */
+int fb_token_logprobs_grad(const fb_tensor* logits, const fb_tensor* targets, const fb_tensor* logsumexp,
+                           const fb_tensor* grad_logprob, const fb_tensor* entropy, const fb_tensor* grad_entropy,
+                           fb_tensor* grad_logits, void* stream);
 
 /* ----------------------------------------------------------- low storage */
 
