@@ -108,6 +108,12 @@ __global__ void __launch_bounds__(BLOCK) token_rows_kernel(TokenArgs a) {
     }
 }
 
+// A logit that this kernel may overwrite: a plain load, not the read-only path.
+template <typename T>
+__device__ __forceinline__ float logit(const T* p) {
+    return Bits<T>::value(*reinterpret_cast<const typename Bits<T>::U*>(p));
+}
+
 // Gradient of one logit.  A term whose coefficient is 0 is 0 whatever x is.
 __device__ __forceinline__ float logit_grad(float x, float lse, float h, float gl, float gh, bool at_target) {
     const float z = x - lse, p = expf(z);
@@ -131,7 +137,7 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
         const float gh = a.g_entropy.data ? row_value(a.g_entropy, row) : 0.0f;
         const float h = gh != 0.0f ? row_value(a.entropy, row) : 0.0f;
         for (uint64_t c = c0 + threadIdx.x; c < min(c0 + 4 * BLOCK, in.cols); c += BLOCK) {
-            const float d = logit_grad(Elem<T>::load(x + nest_offset(in.inner, c)), lse, h, gl, gh, c == t);
+            const float d = logit_grad(logit<T>(x + nest_offset(in.inner, c)), lse, h, gl, gh, c == t);
             O* p = out + nest_offset(a.out.inner, c);
             if constexpr (sizeof(O) == 4) *p = d;
             else *p = a.out.dtype == FB_BF16 ? encode_bf16(d) : encode_f16(d);
@@ -139,16 +145,502 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
     }
 }
 
+// ------------------------------------------------- contiguous rows: one pass
+//
+// A row is read once, 16 bytes per lane and load, for everything but the
+// alternatives.  Sums are kept against a reference m shared by a warp, its
+// running maximum: with d_v = (x_v - m) log2 e,
+//   S0 = sum 2^d_v,  S1 = sum d_v 2^d_v,
+//   lse = m + ln S0,  entropy = ln S0 - ln 2 S1 / S0.
+// x - m is subtracted before it is scaled (two packed operations instead of
+// one FMA): the maximum's own term is then exactly 1, a row of one class has
+// entropy and log probability exactly 0, and no m overflows.  Only a
+// segment's maximum (packed 16-bit maxima, one redux) is compared with m, so
+// rescales by 2^((m - m') log2 e) are rare.  d is clamped at -200 (2^-200
+// flushes to 0), which keeps a masked class's 0 * -inf out of S1; the
+// NaN-propagating clamp keeps a NaN in it.
+//
+// Alternatives.  The k-th largest of the 256 threads' maxima is a lower bound
+// t of the row's k-th largest value, and the maxima of the row's segments
+// (kept in shared memory) say where values >= t lie: about k segments are
+// read again (L2), the values >= t collected with their indices and put in
+// order by counting.  More than CAND of them (a row of few distinct values),
+// and rows with NaN or infinities, take a scan per alternative instead.
+//
+// Bound: HBM (the ex2 unit is 3/4 busy at the full rate with 16-bit logits).
+// Few rows are split over the CTAs of a cluster, each with its own sums and
+// alternatives, joined through distributed shared memory.
+constexpr int WARPS = BLOCK / 32;
+constexpr int CAND = 1024;     // candidates that are put in order by counting
+constexpr int MAX_SEGS = 512;  // segment maxima kept per CTA
+constexpr float L2E = 1.4426950408889634f;
+
+struct TokenPartial {  // one CTA's part of a row
+    float m, s0, s1;
+    uint64_t top[FB_MAX_TOP];  // (key << 32 | ~index), largest first; 0: none
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t packed_max(uint32_t a, uint32_t b, __nv_bfloat16) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t packed_max(uint32_t a, uint32_t b, __half) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// A 16-byte vector as words; how a type's words are widened and compared.
+template <typename T>
+struct Words {
+    static constexpr int E = 8;  // elements per vector
+    static constexpr uint32_t LOWEST = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;  // -inf
+    static __device__ __forceinline__ uint32_t maximum(uint32_t a, uint32_t b) { return packed_max(a, b, T()); }
+    // pattern of the larger half
+    static __device__ __forceinline__ uint32_t top(uint32_t w) { return maximum(w, __byte_perm(w, 0, 0x1032)) & 0xffffu; }
+    static __device__ __forceinline__ float2 widen(uint32_t w) {
+        if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<__half2*>(&w));
+        else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+};
+template <>
+struct Words<float> {
+    static constexpr int E = 4;
+    static constexpr uint32_t LOWEST = 0xff800000u;
+    static __device__ __forceinline__ uint32_t maximum(uint32_t a, uint32_t b) {
+        return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    }
+    static __device__ __forceinline__ uint32_t top(uint32_t w) { return w; }
+};
+
+// A contiguous row seen as aligned 16-byte vectors; vector 0 and the last one
+// may hold elements of its neighbours, which read as -inf.
+template <typename T>
+struct RowVectors {
+    using U = typename Bits<T>::U;
+    static constexpr int E = Words<T>::E;
+    const U* x;          // element 0
+    uint32_t head;       // elements of vector 0 before element 0
+    uint64_t end;        // head + columns
+    __device__ __forceinline__ RowVectors(const T* row, uint64_t cols)
+        : x(reinterpret_cast<const U*>(row)),
+          head((uint32_t)(reinterpret_cast<uintptr_t>(row) & 15u) / (uint32_t)sizeof(U)),
+          end(head + cols) {}
+    __device__ __forceinline__ uint64_t vectors() const { return (end + E - 1) / E; }
+    // NC: through the read-only path (not where the row is being overwritten)
+    template <bool NC>
+    __device__ __forceinline__ uint4 load(uint64_t j) const {
+        const uint64_t v = j * E;
+        if (v >= head && v + E <= end) {
+            const uint4* p = reinterpret_cast<const uint4*>(x + (v - head));
+            return NC ? __ldg(p) : *p;
+        }
+        uint4 r = make_uint4(Words<T>::LOWEST, Words<T>::LOWEST, Words<T>::LOWEST, Words<T>::LOWEST);
+        if (v >= end) return r;
+        uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (v + e >= head && v + e < end) {
+                const uint32_t b = NC ? __ldg(x + (v + e - head)) : x[v + e - head];
+                if constexpr (E == 4) w[e] = b;
+                else w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | (b << 16) : (w[e / 2] & 0xffff0000u) | b;
+            }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+__device__ __forceinline__ uint32_t mapa_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_peer_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint64_t ld_peer_u64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sync_cluster() {
+    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// Base-2 exponent of x against the reference m.
+__device__ __forceinline__ float below(float x, float m) { return max_nan((x - m) * L2E, -200.0f); }
+
+// {m, S0, S1} += another part's: both brought to the larger reference.
+__device__ __forceinline__ void join_sums(float& m, float& s0, float& s1, float m2, float t0, float t1) {
+    if (t0 == 0.0f) return;
+    if (s0 == 0.0f) {
+        m = m2, s0 = t0, s1 = t1;
+        return;
+    }
+    const float top = fmaxf(m, m2), da = below(m, top), db = below(m2, top), a = ex2_approx(da), b = ex2_approx(db);
+    s1 = fmaf(da, s0, s1) * a + fmaf(db, t0, t1) * b;
+    s0 = s0 * a + t0 * b;
+    m = top;
+}
+
+// `parts` CTAs (a cluster when > 1) per row, `part_segs` segments of 32 * VPL
+// vectors each; `mult` segments share a kept maximum.
+template <typename T, int VPL>
+__global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(TokenArgs a, uint32_t parts, uint32_t part_segs, uint32_t mult) {
+    using W = Words<T>;
+    constexpr int NW = VPL * 4;
+    __shared__ __align__(16) uint32_t tkey[BLOCK];
+    __shared__ uint32_t seg_max[MAX_SEGS], sel[MAX_SEGS];
+    __shared__ uint64_t cand[CAND];
+    __shared__ uint64_t scan_keys[WARPS];
+    __shared__ float wsum[3][WARPS];
+    __shared__ uint32_t n_sel, n_cand, tau;
+    __shared__ TokenPartial mine;
+    const Rows& in = a.logits;
+    const uint64_t row = blockIdx.x / parts;
+    const uint32_t part = blockIdx.x % parts;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const T* x = static_cast<const T*>(in.data) + in.offset + row * in.row_stride;
+    const RowVectors<T> rv(x, in.cols);
+    const uint32_t nseg = (uint32_t)((rv.vectors() + 32 * VPL - 1) / (32 * VPL));
+    const uint32_t seg0 = min(part * part_segs, nseg), seg1 = min(seg0 + part_segs, nseg);
+    const uint32_t groups = (seg1 - seg0 + mult - 1) / mult;
+    if (a.top) {
+        for (uint32_t i = threadIdx.x; i < groups; i += BLOCK) seg_max[i] = 0u;
+        if (threadIdx.x == 0) n_sel = n_cand = 0u;
+        __syncthreads();
+    }
+    auto load_seg = [&](uint32_t seg, uint32_t (&w)[NW]) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const uint4 v = rv.template load<true>((uint64_t)seg * (32 * VPL) + i * 32 + lane);
+            w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+    };
+    float m = 0.0f;  // the reference: 0 while nothing but -inf was seen
+    float2 s0[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, s1[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    uint32_t run = 0u, own_max = W::LOWEST;
+    for (uint32_t seg = seg0 + warp; seg < seg1; seg += WARPS) {
+        uint32_t w[NW];
+        load_seg(seg, w);
+        uint32_t mx = w[0];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) mx = W::maximum(mx, w[i]);
+        own_max = W::maximum(own_max, mx);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, Bits<T>::key(W::top(mx)));
+        if (a.top && lane == 0) atomicMax(&seg_max[(seg - seg0) / mult], top);
+        if (top > run) {
+            run = top;
+            const float v = Bits<T>::value(Bits<T>::pattern(top));
+            const float m2 = v == -__int_as_float(0x7f800000) ? 0.0f : v;
+            const float dm = below(m, m2), f = ex2_approx(dm);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float t0 = s0[h].x + s0[h].y, t1 = s1[h].x + s1[h].y;
+                s0[h] = make_float2(t0 == 0.0f ? 0.0f : t0 * f, 0.0f);
+                s1[h] = make_float2(t0 == 0.0f ? 0.0f : fmaf(dm, t0, t1) * f, 0.0f);
+            }
+            m = m2;
+        }
+        const float2 l2 = make_float2(L2E, L2E), nm = make_float2(-m, -m);
+        constexpr int PAIRS = W::E == 8 ? NW : NW / 2;
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            float2 v;
+            if constexpr (W::E == 8) v = W::widen(w[i]);
+            else v = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+            float2 d = __fmul2_rn(__fadd2_rn(v, nm), l2);
+            d.x = max_nan(d.x, -200.0f), d.y = max_nan(d.y, -200.0f);
+            const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+            s0[i & 1] = __fadd2_rn(s0[i & 1], e);
+            s1[i & 1] = __ffma2_rn(e, d, s1[i & 1]);
+        }
+    }
+    {
+        const float t0 = warp_sum_f((s0[0].x + s0[0].y) + (s0[1].x + s0[1].y));
+        const float t1 = warp_sum_f((s1[0].x + s1[0].y) + (s1[1].x + s1[1].y));
+        if (lane == 0) wsum[0][warp] = m, wsum[1][warp] = t0, wsum[2][warp] = t1;
+        if (a.top) tkey[threadIdx.x] = Bits<T>::key(W::top(own_max));
+    }
+    __syncthreads();
+    float M = wsum[0][0], S0 = wsum[1][0], S1 = wsum[2][0];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) join_sums(M, S0, S1, wsum[0][w], wsum[1][w], wsum[2][w]);
+
+    if (a.top) {
+        const uint32_t k = a.top;
+        if (threadIdx.x < FB_MAX_TOP) mine.top[threadIdx.x] = 0ull;
+        {
+            const uint32_t key = tkey[threadIdx.x];
+            uint32_t rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < BLOCK; j += 4) {
+                const uint4 o = *reinterpret_cast<const uint4*>(&tkey[j]);
+                rank += (o.x > key) + (o.y > key) + (o.z > key) + (o.w > key);
+                rank += (o.x == key && j < (int)threadIdx.x) + (o.y == key && j + 1 < (int)threadIdx.x) +
+                        (o.z == key && j + 2 < (int)threadIdx.x) + (o.w == key && j + 3 < (int)threadIdx.x);
+            }
+            if (rank == k - 1) tau = key;
+        }
+        __syncthreads();
+        const uint32_t t = tau;
+        for (uint32_t i = threadIdx.x; i < groups; i += BLOCK)
+            if (seg_max[i] >= t) sel[atomicAdd(&n_sel, 1u)] = i;
+        __syncthreads();
+        bool ordered = S0 == S0;  // no NaN and no +inf among the values
+        if (ordered) {
+            const uint32_t reads = n_sel * mult;
+            for (uint32_t i = warp; i < reads; i += WARPS) {
+                const uint32_t seg = seg0 + sel[i / mult] * mult + i % mult;
+                if (seg >= seg1) continue;
+                uint32_t w[NW];
+                load_seg(seg, w);
+                uint32_t mx = w[0];
+#pragma unroll
+                for (int j = 1; j < NW; ++j) mx = W::maximum(mx, w[j]);
+                if (Bits<T>::key(W::top(mx)) < t) continue;
+                const uint64_t v0 = ((uint64_t)seg * (32 * VPL) + lane) * W::E;
+#pragma unroll
+                for (int e = 0; e < VPL * W::E; ++e) {
+                    uint32_t b;
+                    if constexpr (W::E == 8) b = e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
+                    else b = w[e];
+                    const uint32_t key = Bits<T>::key(b);
+                    const uint64_t v = v0 + (uint64_t)(e / W::E) * 32 * W::E + e % W::E;
+                    if (key >= t && v >= rv.head && v < rv.end) {
+                        const uint32_t n = atomicAdd(&n_cand, 1u);
+                        if (n < CAND) cand[n] = ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)(v - rv.head));
+                    }
+                }
+            }
+            __syncthreads();
+            ordered = n_cand <= CAND;
+        }
+        if (ordered) {
+            const uint32_t n = n_cand;
+            for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
+                const uint64_t me = cand[i];
+                uint32_t rank = 0;
+                for (uint32_t j = 0; j < n; ++j) rank += cand[j] > me;
+                if (rank < k) mine.top[rank] = me;
+            }
+        } else {
+            const uint64_t v0 = max((uint64_t)seg0 * (32 * VPL) * W::E, (uint64_t)rv.head);
+            const uint64_t v1 = min((uint64_t)seg1 * (32 * VPL) * W::E, rv.end);
+            uint64_t bound = ~0ull;
+            for (uint32_t r = 0; r < k && bound; ++r) {
+                uint64_t best = 0;
+                for (uint64_t v = v0 + threadIdx.x; v < v1; v += BLOCK) {
+                    const uint64_t q = ((uint64_t)Bits<T>::key(__ldg(rv.x + (v - rv.head))) << 32) |
+                                       (0xffffffffu - (uint32_t)(v - rv.head));
+                    if (q < bound && q > best) best = q;
+                }
+                bound = block_max_u64<BLOCK>(best, scan_keys);
+                if (threadIdx.x == 0) mine.top[r] = bound;
+            }
+        }
+        __syncthreads();
+    }
+    if (parts > 1) {
+        if (threadIdx.x == 0) mine.m = M, mine.s0 = S0, mine.s1 = S1;
+        sync_cluster();
+        if (part == 0) {
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(&mine);
+            for (uint32_t p = 1; p < parts; ++p) {
+                const uint32_t peer = mapa_rank(at, p);
+                join_sums(M, S0, S1, ld_peer_f32(peer), ld_peer_f32(peer + 4), ld_peer_f32(peer + 8));
+            }
+            if (a.top) {
+                // the parts' alternatives in one list: their order by counting
+                const uint32_t n = parts * a.top;
+                const uint32_t off = (uint32_t)(reinterpret_cast<const char*>(mine.top) - reinterpret_cast<const char*>(&mine));
+                for (uint32_t i = threadIdx.x; i < n; i += BLOCK)
+                    cand[i] = ld_peer_u64(mapa_rank(at + off, i / a.top) + (i % a.top) * 8);
+                __syncthreads();
+                uint64_t me[2];
+                uint32_t rank[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t i = threadIdx.x + h * BLOCK;
+                    rank[h] = a.top;
+                    if (i < n && cand[i]) {
+                        me[h] = cand[i], rank[h] = 0;
+                        for (uint32_t j = 0; j < n; ++j) rank[h] += cand[j] > me[h];
+                    }
+                }
+                sync_cluster();  // every peer's list has been read
+                for (int h = 0; h < 2; ++h)
+                    if (rank[h] < a.top) mine.top[rank[h]] = me[h];
+                __syncthreads();
+            } else {
+                sync_cluster();
+            }
+        } else {
+            sync_cluster();  // this CTA's sums and list stay until they are read
+            return;
+        }
+    }
+    // One row's results, in f64 from here.
+    const double ls = S0 == 0.0f ? (double)row_nan() : log((double)S0), lse = (double)M + ls;
+    if (threadIdx.x == 0) {
+        row_store(a.lse, row, (float)lse);
+        row_store(a.entropy, row, (float)(ls - (double)S1 / (double)S0 * 0.6931471805599453));
+        if (a.logprob.data) {
+            const uint32_t t = a.targets[a.target_offset + nest_offset(a.target_nest, row)];
+            float r = 0.0f;
+            if (t != FB_NO_TOKEN) r = t < in.cols ? (float)((double)Elem<T>::load(x + t) - lse) : row_nan();
+            row_store(a.logprob, row, r);
+        }
+    }
+    if (threadIdx.x < a.top) {
+        const uint64_t q = mine.top[threadIdx.x];
+        a.top_index[row * a.top + threadIdx.x] = 0xffffffffu - (uint32_t)q;
+        a.top_logprob[row * a.top + threadIdx.x] =
+            (float)((double)Bits<T>::value(Bits<T>::pattern((uint32_t)(q >> 32))) - lse);
+    }
+}
+
+template <typename T, int VPL>
+int launch_stream(const TokenArgs& a, cudaStream_t st) {
+    const Rows& in = a.logits;
+    const uint64_t E = Words<T>::E, seg = 32 * VPL;
+    const uint64_t nseg = ((in.cols + 2 * E - 2) / E + seg - 1) / seg;  // at the worst alignment
+    // Parts per row: powers of two up to a cluster of eight, while the grid is
+    // under eight CTAs per SM and a part keeps two segments per warp, or under
+    // one per SM and it keeps half a segment per warp.
+    uint64_t parts = 1;
+    const uint64_t sms = (uint64_t)sm_count();
+    while (parts < 8 && ((in.rows * parts * 2 <= sms * 8 && nseg >= parts * 2 * 2 * WARPS) ||
+                         (in.rows * parts * 2 <= sms && nseg >= parts * WARPS)))
+        parts *= 2;
+    const uint64_t part_segs = (nseg + parts - 1) / parts;
+    const uint64_t mult = (part_segs + MAX_SEGS - 1) / MAX_SEGS;
+    if (in.rows * parts > 0x7fffffffull || nseg > 0xffffffffull) return FB_ERR_UNSUPPORTED;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(in.rows * parts));
+    cfg.blockDim = dim3(BLOCK);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)parts;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    (void)cudaLaunchKernelEx(&cfg, token_stream_kernel<T, VPL>, a, (uint32_t)parts, (uint32_t)part_segs, (uint32_t)mult);
+    count_launch("token_stream_kernel");
+    return launch_status("kernel launch");
+}
+
 template <typename T>
 int launch_t(const TokenArgs& a, cudaStream_t st) {
+    if (a.logits.contiguous_rows) {
+        // Short rows: one vector per lane and segment, so that every warp has
+        // one from 8 * 32 vectors on.
+        const int r = a.logits.cols <= (uint64_t)Words<T>::E * 32 * 4 * WARPS ? launch_stream<T, 1>(a, st) : launch_stream<T, 4>(a, st);
+        if (r != FB_ERR_UNSUPPORTED) return r;
+    }
     const unsigned blocks = (unsigned)std::min<uint64_t>(a.logits.rows, (uint64_t)sm_count() * 32);
     token_rows_kernel<T><<<blocks, BLOCK, 0, st>>>(a);
     count_launch("token_rows_kernel");
     return launch_status("kernel launch");
 }
 
+// Contiguous rows whose output vectors line up with the logits': 16 bytes per
+// lane and load.  With d = (x - lse) log2 e, p = 2^d and
+//   grad = gl [v = t] - p (gl + gh (log p + entropy)) = gl [v = t] + 2^d (A + B d),
+//   A = -(gl + gh entropy), B = -gh ln 2:
+// four packed operations, two clamps and two ex2 for a pair of elements; d is
+// clamped at -200 (2^-200 flushes to 0) so that a masked class's -inf meets no
+// 0 or infinity.
+// Bound: HBM, one read and one write.  Loads are issued before the row's
+// scalars arrive; each block does one chunk of 4 vectors per thread.
+template <typename T>
+__global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(TokenGradArgs a, uint32_t chunks) {
+    using W = Words<T>;
+    using U = typename Bits<T>::U;
+    constexpr int E = W::E, N = 4;
+    const Rows& in = a.logits;
+    const uint64_t row = blockIdx.x / chunks;
+    const uint64_t j0 = (uint64_t)(blockIdx.x % chunks) * (N * BLOCK) + threadIdx.x;
+    const T* x = static_cast<const T*>(in.data) + in.offset + row * in.row_stride;
+    U* out = reinterpret_cast<U*>(a.out.data) + a.out.offset + row * a.out.row_stride;
+    const RowVectors<T> rv(x, in.cols);
+    uint32_t w[N][4];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint4 v = rv.template load<false>(j0 + i * BLOCK);
+        w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
+    }
+    const uint32_t t = a.targets[a.target_offset + nest_offset(a.target_nest, row)];
+    const float gl = t < in.cols ? row_value(a.g_logprob, row) : 0.0f;
+    const float gh = a.g_entropy.data ? row_value(a.g_entropy, row) : 0.0f;
+    const bool zero = gl == 0.0f && gh == 0.0f;
+    const float lse = row_value(a.lse, row);
+    const float h = gh != 0.0f ? row_value(a.entropy, row) : 0.0f;
+    const float A = -fmaf(gh, h, gl), B = -gh * 0.6931471805599453f;
+    const uint64_t at = (uint64_t)t + rv.head;  // the target's place among the vectors' elements
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint64_t v = (j0 + i * BLOCK) * E;
+        if (v >= rv.end) break;
+        float g[E];
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            float2 y;
+            if constexpr (E == 8) y = W::widen(w[i][e / 2]);
+            else y = make_float2(__uint_as_float(w[i][e]), __uint_as_float(w[i][e + 1]));
+            float2 d = __fmul2_rn(__fadd2_rn(y, make_float2(-lse, -lse)), make_float2(L2E, L2E));
+            d.x = max_nan(d.x, -200.0f), d.y = max_nan(d.y, -200.0f);
+            const float2 k = __ffma2_rn(d, make_float2(B, B), make_float2(A, A));
+            g[e] = zero ? 0.0f : ex2_approx(d.x) * k.x;
+            g[e + 1] = zero ? 0.0f : ex2_approx(d.y) * k.y;
+        }
+        if (at - v < (uint64_t)E && gl != 0.0f) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (at == v + e) g[e] += gl;
+        }
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (E == 8) o[e] = encode_low_pair(g[2 * e], g[2 * e + 1], std::is_same<T, __half>::value ? FB_F16 : FB_BF16);
+            else o[e] = __float_as_uint(g[e]);
+        }
+        if (v >= rv.head && v + E <= rv.end) {
+            __stcs(reinterpret_cast<uint4*>(out + (v - rv.head)), make_uint4(o[0], o[1], o[2], o[3]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (v + e >= rv.head && v + e < rv.end) {
+                    if constexpr (E == 8) out[v + e - rv.head] = (U)(e % 2 ? o[e / 2] >> 16 : o[e / 2] & 0xffffu);
+                    else out[v + e - rv.head] = o[e];
+                }
+        }
+    }
+}
+
 template <typename T>
 int launch_grad_t(const TokenGradArgs& a, cudaStream_t st) {
+    const Rows& in = a.logits;
+    constexpr uint64_t esz = sizeof(typename Bits<T>::U);
+    const uint32_t dtype = std::is_same<T, float>::value ? FB_F32 : std::is_same<T, __half>::value ? FB_F16 : FB_BF16;
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(in.data) + in.offset * esz;
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(a.out.data) + a.out.offset * esz;
+    if (in.contiguous_rows && a.out.contiguous_rows && a.out.dtype == dtype && (x0 - o0) % 16 == 0 &&
+        (in.row_stride - a.out.row_stride) * esz % 16 == 0) {
+        const uint64_t vectors = (in.cols + 2 * Words<T>::E - 2) / Words<T>::E, chunks = (vectors + 4 * BLOCK - 1) / (4 * BLOCK);
+        if (in.rows * chunks <= 0x7fffffffull) {
+            token_grad_stream_kernel<T><<<(unsigned)(in.rows * chunks), BLOCK, 0, st>>>(a, (uint32_t)chunks);
+            count_launch("token_grad_stream_kernel");
+            return launch_status("kernel launch");
+        }
+    }
     const uint64_t chunks = (a.logits.cols + 4 * BLOCK - 1) / (4 * BLOCK);
     const unsigned blocks = (unsigned)std::min<uint64_t>(a.logits.rows * chunks, (uint64_t)sm_count() * 64);
     if (a.out.dtype == FB_F32) token_grad_rows_kernel<T, float><<<blocks, BLOCK, 0, st>>>(a);
