@@ -649,7 +649,9 @@ int span_impl(const fb_tensor* q, const fb_tensor* pk, const fb_tensor* pv, cons
         s.pk_stride_head = pkv.strides[0], s.pk_stride_key = pkv.strides[1], s.pk_stride_d = pkv.strides[2];
         s.pv_stride_head = pvv.strides[0], s.pv_stride_key = pvv.strides[1], s.pv_stride_d = pvv.strides[2];
     }
-    return launched(launch_span_simt(s, stream), prefix ? "shared-prefix attention" : "windowed attention");
+    int st = launch_span_tc(s, stream);
+    if (st == FB_ERR_UNSUPPORTED) st = launch_span_simt(s, stream);
+    return launched(st, prefix ? "shared-prefix attention" : "windowed attention");
 }
 
 // Per-row f32 input or output of the token log probabilities.
@@ -995,7 +997,7 @@ const char* fb_last_route(void) { return g_route.c_str(); }
 
 uint32_t fb_device_status(void) {
     cudaDeviceSynchronize();
-    return read_reduce_status() | read_gemm_status() | read_attention_status();
+    return read_reduce_status() | read_gemm_status() | read_attention_status() | read_span_status();
 }
 
 int fb_conv_plan(const uint64_t* input_dims, uint32_t input_rank, const uint64_t* weight_dims, uint32_t weight_rank,

@@ -1,0 +1,1362 @@
+// Windowed attention (last `window` keys and the first `sinks`) and attention
+// over a prefix shared by the batch, for 16-bit operands at depth 64 and 128.
+//
+// Many query rows per key/value head: span_tile_kernel, a tcgen05 flash kernel
+// over the key tiles that a block of rows can see.  At most 16 rows per
+// key/value head (single tokens of a few sequences' heads): span_decode_kernel,
+// warp-level MMAs under a stream of exactly the visible keys.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "attention_common.cuh"
+
+namespace fb {
+namespace {
+
+__device__ uint32_t g_span_status;
+
+// ------------------------------------------------------------- key spans
+
+// A block of queries at positions pa .. pb (pa <= pb) over n filled keys sees
+// no key outside [0, first) and [lo, hi], first <= lo: hi = min(pb, n - 1),
+// lo = max(0, pa - window + 1).  hi < 0: nothing at all; lo > hi: only first.
+struct Reach {
+    int64_t first, lo, hi;
+};
+__device__ __forceinline__ Reach reach(int64_t pa, int64_t pb, int64_t n, int64_t window, int64_t sinks) {
+    Reach r;
+    r.hi = min(pb, n - 1);
+    r.lo = max((int64_t)0, pa - window + 1);
+    r.first = max((int64_t)0, min(min(sinks, r.lo), r.hi + 1));
+    return r;
+}
+
+// What a key range leaves for a query row: {base, l, -, -, O[D]}, O = sum P V
+// and l = sum P unnormalised, base the log2 reference of P's exponentials
+// (l = 0: no key seen).  Joined, with M the largest base of those with l > 0:
+// O = sum O_r 2^(base_r - M) / sum l_r 2^(base_r - M).
+template <int D>
+constexpr int REC = D + 4;
+
+// --------------------------------------------------------- tcgen05 tiles
+//
+// A tile is up to 128 query rows that share a key/value head: GB query heads
+// x LB consecutive queries x NB sequences, gathered by one 4-D TMA box over
+// {depth, heads, queries, batch}, so that grouped heads share the key tiles
+// whatever Q's strides are.  A CTA owns two tiles and walks the key tiles
+// that either sees, in order: those of the first keys, then those of the two
+// windows.  A tile of rows takes part only in the key tiles that it sees.
+//   warp 0      TMA: both Q tiles, then K and V tiles of 128 keys through
+//               rings of 2 (D = 128) or 4 (D = 64) slots
+//   warp 1      TMEM and MMA issue: S_t = Q_t K^T, O_t += P_t V, the two
+//               tiles in turn so that one's products run during the other's
+//               softmax; value rows past the filled keys are zeroed in shared
+//               memory first (a weight of 0 does not hide a NaN there)
+//   warps 2-9   softmax, one query row per thread: lazy running maximum
+//               (raised, and O rescaled, only past 2^8), P over S in TMEM
+// This is attn_fwd_kernel's pipeline; see there for the orderings, the
+// 2^-shift pre-scale of BF16 weights and the bounded waits.
+struct SpanTileParams {
+    uint32_t fmt;                  // 0 f16, 1 bf16
+    uint32_t B, H, L, Lk;          // sequences, query heads, queries, keys per head
+    uint32_t group;                // query heads per key/value head
+    uint32_t GB, LB, NB, rows;     // the tile's box and its row count GB * LB * NB
+    uint32_t l_tiles, tiles;       // tiles along the queries; tiles of one unit
+    uint32_t pairs, units;         // pairs of tiles per unit; units = (batch x) head blocks
+    uint32_t head_blocks;          // H / GB
+    uint32_t shared_keys;          // 1: every row sees all Lk keys of batch 0 (the shared prefix)
+    uint32_t k_batch_bcast, v_batch_bcast;
+    const uint32_t* lengths;
+    uint64_t length_stride;
+    int64_t offset, window, sinks;
+    float scale_log2, shift;
+    uint32_t splits;               // CTAs along the key tiles of a pair
+    float* part;                   // records: ((b * H + h) * L + l) * part_stride + part_first + split
+    uint32_t part_stride, part_first;
+    void* out;                     // part == null: output rows
+    uint32_t out_low, tma_out;
+    uint64_t o_sb, o_sh, o_sl;
+};
+
+template <int D>
+struct TCfg {
+    static constexpr int THREADS = 64 + 2 * 128;
+    static constexpr int BOXES = D / 64;
+    static constexpr int Q_BYTES = TQ * D * 2;
+    static constexpr int K_BYTES = TK * D * 2;
+    static constexpr int STAGE_BYTES = 2 * K_BYTES;
+    static constexpr int STAGES = D == 64 ? 4 : 2;
+    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + 256;
+    static __device__ __forceinline__ uint32_t s_col(int t) { return (uint32_t)(t * TK); }
+    static __device__ __forceinline__ uint32_t o_col(int t) { return (uint32_t)(2 * TK + t * 128); }
+};
+
+// The key tiles of a pair of query tiles: joint index j stands for key tile
+// j < s ? j : a + (j - s); query tile t sees key tiles [0, ns[t]) and
+// [a0[t], e[t]).
+struct TilePlan {
+    uint32_t s, a, n;          // joint list length n
+    uint32_t ns[2], a0[2], e[2];
+    __device__ __forceinline__ uint32_t tile(uint32_t j) const { return j < s ? j : a + (j - s); }
+    __device__ __forceinline__ bool sees(int t, uint32_t tile) const { return tile < ns[t] || (tile >= a0[t] && tile < e[t]); }
+    __device__ __forceinline__ uint32_t count(int t, uint32_t j0, uint32_t j1) const {
+        auto overlap = [](uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
+            const uint32_t lo = max(x0, y0), hi = min(x1, y1);
+            return hi > lo ? hi - lo : 0u;
+        };
+        uint32_t c = overlap(0, ns[t], min(j0, s), min(j1, s)) + overlap(a0[t], e[t], min(j0, s), min(j1, s));
+        if (j1 > s) c += overlap(a0[t], e[t], a + max(j0, s) - s, a + (j1 - s));
+        return c;
+    }
+};
+
+template <int D>
+__global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
+                                                                       const __grid_constant__ CUtensorMap tmK,
+                                                                       const __grid_constant__ CUtensorMap tmV,
+                                                                       const __grid_constant__ CUtensorMap tmO, SpanTileParams p) {
+    using C = TCfg<D>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* sQ = smem;
+    unsigned char* sKV = sQ + 2 * C::Q_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::STAGES * C::STAGE_BYTES);
+    uint64_t* q_full = bars;
+    uint64_t* k_full = bars + 1;
+    uint64_t* k_empty = k_full + C::STAGES;
+    uint64_t* v_full = k_empty + C::STAGES;
+    uint64_t* v_empty = v_full + C::STAGES;
+    uint64_t* s_full = v_empty + C::STAGES;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_done = p_full + 2;
+    uint64_t* drain = o_done + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+
+    // The launch that follows may start while this one ends (where it was made
+    // so); it waits for this grid's results itself.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // Pairs of one unit in consecutive CTAs, last queries first.
+    const uint32_t split = blockIdx.x % p.splits;
+    const uint32_t pair = p.pairs - 1 - (blockIdx.x / p.splits) % p.pairs;
+    const uint32_t unit = blockIdx.x / (p.splits * p.pairs);
+    const uint32_t hb = unit % p.head_blocks;
+    const uint32_t head0 = hb * p.GB, kv_head = head0 / p.group;
+    const uint32_t unit_b = unit / p.head_blocks;  // 0 with shared keys
+    int64_t filled = p.Lk, base = p.offset;
+    if (p.lengths) {
+        filled = min(filled, (int64_t)p.lengths[unit_b * p.length_stride]);
+        base = filled - (int64_t)p.L;
+    }
+    // tile t of the pair: first sequence and first query
+    uint32_t b0[2], l0[2];
+    bool real[2];
+    TilePlan plan;
+    Reach rc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const uint32_t tile = pair * 2 + t;
+        real[t] = tile < p.tiles;
+        b0[t] = p.shared_keys ? tile / p.l_tiles * p.NB : unit_b;
+        l0[t] = (p.shared_keys ? tile % p.l_tiles : tile) * p.LB;
+        plan.ns[t] = plan.a0[t] = plan.e[t] = 0;
+        rc[t] = Reach{0, 0, -1};
+        if (!real[t]) continue;
+        if (p.shared_keys) {
+            rc[t] = Reach{0, 0, (int64_t)p.Lk - 1};
+        } else {
+            rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
+        }
+        if (rc[t].hi < 0) continue;
+        plan.ns[t] = (uint32_t)((rc[t].first + TK - 1) / TK);
+        if (rc[t].lo <= rc[t].hi) {
+            plan.a0[t] = max((uint32_t)(rc[t].lo / TK), plan.ns[t]);
+            plan.e[t] = max((uint32_t)(rc[t].hi / TK) + 1, plan.a0[t]);
+        }
+    }
+    plan.s = max(plan.ns[0], plan.ns[1]);
+    {
+        uint32_t a = 0xffffffffu, e = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            if (plan.e[t] > plan.a0[t]) a = min(a, plan.a0[t]), e = max(e, plan.e[t]);
+        plan.a = e ? max(a, plan.s) : plan.s;
+        plan.n = plan.s + (e > plan.a ? e - plan.a : 0);
+    }
+    // this CTA's share of the joint list
+    const uint32_t per = (plan.n + p.splits - 1) / p.splits;
+    const uint32_t j0 = min(split * per, plan.n), j1 = min(j0 + per, plan.n);
+    const uint32_t n_kv = j1 - j0;
+    const uint32_t n_t[2] = {plan.count(0, j0, j1), plan.count(1, j0, j1)};
+    auto key_tile = [&](uint32_t j) { return plan.tile(j0 + j); };
+    // next local joint index >= j that tile t sees (n_kv if none)
+    auto next_seen = [&](int t, uint32_t j) {
+        while (j < n_kv && !plan.sees(t, key_tile(j))) ++j;
+        return j;
+    };
+    const int32_t k_b = p.shared_keys || p.k_batch_bcast ? 0 : (int32_t)unit_b;
+    const int32_t v_b = p.shared_keys || p.v_batch_bcast ? 0 : (int32_t)unit_b;
+    auto load_k = [&](uint32_t j) {
+        const uint32_t s = j % C::STAGES;
+        mbar_arrive_expect_tx(&k_full[s], C::K_BYTES);
+        for (int b = 0; b < C::BOXES; ++b)
+            tma_load_4d(sKV + s * C::STAGE_BYTES + b * (TK * 128), &tmK, b * 64, (int32_t)(key_tile(j) * TK),
+                        (int32_t)kv_head, k_b, &k_full[s]);
+    };
+    auto load_v = [&](uint32_t j) {
+        const uint32_t s = j % C::STAGES;
+        mbar_arrive_expect_tx(&v_full[s], C::K_BYTES);
+        for (int b = 0; b < C::BOXES; ++b)
+            tma_load_4d(sKV + s * C::STAGE_BYTES + C::K_BYTES + b * (TK * 128), &tmV, b * 64, (int32_t)(key_tile(j) * TK),
+                        (int32_t)kv_head, v_b, &v_full[s]);
+    };
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 128);
+            mbar_init(&o_done[t], 1);
+        }
+        mbar_init(drain, 1);
+        fence_barrier_init();
+        if (n_kv > 0) {
+            const uint32_t tiles = (n_t[0] > 0) + (n_t[1] > 0);
+            mbar_arrive_expect_tx(q_full, tiles * p.rows * (uint32_t)(D * 2));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                for (int b = 0; b < C::BOXES && n_t[t] > 0; ++b)
+                    tma_load_4d(sQ + t * C::Q_BYTES + b * (TQ * 128), &tmQ, b * 64, (int32_t)head0, (int32_t)l0[t],
+                                (int32_t)b0[t], q_full);
+        }
+        for (uint32_t j = 0; j < n_kv && j < (uint32_t)C::STAGES; ++j) {
+            load_k(j);
+            load_v(j);
+        }
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0 && lane == 0) {
+        // ------------------------------------------------ TMA producer
+        const uint32_t pre = n_kv < (uint32_t)C::STAGES ? n_kv : (uint32_t)C::STAGES;
+        uint32_t issued_k = pre, issued_v = pre;
+        bool failed = false;
+        for (uint32_t j = pre; j < n_kv; ++j) {
+            const uint32_t s = j % C::STAGES, ph = ((j / C::STAGES) & 1) ^ 1;
+            if (!mbar_wait(&k_empty[s], ph)) {
+                failed = true;
+                break;
+            }
+            load_k(j);
+            ++issued_k;
+            if (!mbar_wait(&v_empty[s], ph)) {
+                failed = true;
+                break;
+            }
+            load_v(j);
+            ++issued_v;
+        }
+        if (failed) {
+            // drain the copies still in flight (bounded) before exiting
+            atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
+            for (uint32_t j = issued_k >= C::STAGES ? issued_k - C::STAGES : 0; j < issued_k; ++j)
+                (void)mbar_wait(&k_full[j % C::STAGES], (j / C::STAGES) & 1);
+            for (uint32_t j = issued_v >= C::STAGES ? issued_v - C::STAGES : 0; j < issued_v; ++j)
+                (void)mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1);
+        }
+        if (n_kv > 0) (void)mbar_wait(q_full, 0);
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer
+        const uint32_t idesc_s = f16_idesc(p.fmt, TQ, TK);
+        const uint32_t idesc_o = f16_idesc(p.fmt, TQ, D) | (1u << 16);  // B (V) is MN-major
+        auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+        bool ok = n_kv == 0 || wait(q_full, 0);
+        auto issue_s = [&](int t, uint32_t j) -> bool {
+            const uint32_t s = j % C::STAGES;
+            if (!wait(&k_full[s], (j / C::STAGES) & 1)) return false;
+            tc_fence_after();
+            const uint64_t qd = sw128_desc(smem_u32(sQ + t * C::Q_BYTES));
+            const uint64_t kd = sw128_desc(smem_u32(sKV + s * C::STAGE_BYTES));
+            const uint32_t d = tmem + C::s_col(t);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = (uint32_t)((k / 4) * (TQ * 128) + (k % 4) * 32);
+                umma_f16_ss_warp(d, desc_add(qd, off), desc_add(kd, off), idesc_s, k != 0);
+            }
+            umma_commit_warp(&s_full[t]);
+            return true;
+        };
+        // i: how many key tiles query tile t has taken before this one
+        auto issue_pv = [&](int t, uint32_t j, uint32_t i) -> bool {
+            const uint32_t s = j % C::STAGES;
+            if (!wait(&p_full[t], i & 1)) return false;
+            tc_fence_after();
+            const uint64_t vd = sw128_mn_desc(smem_u32(sKV + s * C::STAGE_BYTES + C::K_BYTES), TK * 128);
+            const uint32_t d = tmem + C::o_col(t), a = tmem + C::s_col(t);
+            umma_f16_ts_warp(d, a, vd, idesc_o, i != 0);
+#pragma unroll
+            for (int k = 1; k < TK / 16; ++k) umma_f16_ts_warp(d, a + k * 8, desc_add(vd, k * 16 * 128), idesc_o, 1u);
+            if (i + 1 == n_t[t]) umma_commit_warp(&o_done[t]);
+            return true;
+        };
+        uint32_t at[2], taken[2] = {0, 0};
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            at[t] = n_t[t] ? next_seen(t, 0) : n_kv;
+            if (ok && at[t] < n_kv) ok = issue_s(t, at[t]);
+        }
+        if (ok && n_kv > 0) umma_commit_warp(&k_empty[0]);  // K(0) consumed by every S(0)
+        for (uint32_t j = 0; ok && j < n_kv; ++j) {
+            const uint32_t s = j % C::STAGES;
+            ok = wait(&v_full[s], (j / C::STAGES) & 1);
+            const int64_t key0 = (int64_t)key_tile(j) * TK;
+            if (ok && p.lengths && !p.shared_keys && key0 + TK > filled) {
+                // value rows past the filled keys: zeros
+                const uint32_t from = (uint32_t)(filled - key0);
+                unsigned char* v = sKV + s * C::STAGE_BYTES + C::K_BYTES;
+                for (int b = 0; b < C::BOXES; ++b)
+                    for (uint32_t o = from * 128 + lane * 16; o < TK * 128; o += 512)
+                        *reinterpret_cast<uint4*>(v + b * (TK * 128) + o) = make_uint4(0u, 0u, 0u, 0u);
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (!ok || at[t] != j) continue;
+                ok = issue_pv(t, j, taken[t]);
+                ++taken[t];
+                at[t] = taken[t] < n_t[t] ? next_seen(t, j + 1) : n_kv;
+                if (ok && at[t] < n_kv) ok = issue_s(t, at[t]);
+            }
+            // V(j) is free once every PV(j) has completed, K(j + 1) once
+            // every S(j + 1) has (each was issued by now)
+            if (ok) umma_commit_warp(&v_empty[s]);
+            if (ok && j + 1 < n_kv) umma_commit_warp(&k_empty[(j + 1) % C::STAGES]);
+        }
+        if (!ok && lane == 0) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
+        umma_commit_warp(drain);
+        (void)wait(drain, 0);
+    } else if (warp >= 2) {
+        // ------------------------------------------------ softmax / epilogue
+        const int t = (warp - 2) / 4;
+        const int quarter = warp & 3;
+        const uint32_t row = (uint32_t)(quarter * 32 + lane);
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const uint32_t head = head0 + row % p.GB, l = (t ? l0[1] : l0[0]) + row / p.GB % p.LB,
+                       b = (t ? b0[1] : b0[0]) + row / (p.GB * p.LB);
+        const bool valid = (t ? real[1] : real[0]) && row < p.rows && l < p.L && b < p.B;
+        const uint32_t n = t ? n_t[1] : n_t[0], n_other = t ? n_t[0] : n_t[1];
+        const float NEG = -__int_as_float(0x7f800000);
+        const float sl = p.scale_log2;
+        // keys of this row: [0, sinks) and [low, high]
+        const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1 : base + (int64_t)l;
+        const int32_t high = (int32_t)max((int64_t)-1, min(pos, filled - 1));
+        const int32_t low = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
+        const int32_t sinks = (int32_t)min((int64_t)0x7fffffff, p.sinks);
+        const uint32_t ns = t ? plan.ns[1] : plan.ns[0], a0 = t ? plan.a0[1] : plan.a0[0], e0 = t ? plan.e[1] : plan.e[0];
+        float m_used = NEG;  // running max (log2 units)
+        float lsum = 0.0f;
+        bool ok = true;
+        uint32_t j = 0;
+        for (uint32_t i = 0; i < n && ok; ++i, ++j) {
+            uint32_t kt = key_tile(j);
+            while (kt >= ns && (kt < a0 || kt >= e0)) kt = key_tile(++j);  // n counts what follows: it ends
+            const int32_t key0 = (int32_t)(kt * TK);
+            // Wait outcomes are made warp-uniform: tcgen05.ld/st are .sync.aligned.
+            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], i & 1))) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            float x[TK];
+            {
+                uint32_t r[TK];
+#pragma unroll
+                for (int c = 0; c < TK / 32; ++c)
+                    tmem_ld32(tmem + lane_base + C::s_col(t) + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < TK; ++e) x[e] = __uint_as_float(r[e]);
+            }
+            const bool edge = key0 + TK - 1 > high || (key0 < low && key0 + TK > sinks);
+            if (edge || sl == 0.0f) {
+                const int32_t lim = high + 1 - key0, lo = low - key0, sk = sinks - key0;
+#pragma unroll
+                for (int e = 0; e < TK; ++e) x[e] = e < lim && (e >= lo || e < sk) ? x[e] * sl : NEG;  // logits, masked
+            }
+            const bool raw = !(edge || sl == 0.0f);
+            const bool use_min = raw && sl < 0.0f;
+            // Four chains of three-input extremes: 64 instructions per row.
+            float mx[4] = {x[0], x[1], x[2], x[3]};
+            if (use_min) {
+#pragma unroll
+                for (int e = 4; e < TK - 4; e += 8)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) mx[a] = min3n(mx[a], x[e + 2 * a], x[e + 2 * a + 1]);
+                mx[0] = min3n(mx[0], x[TK - 4], x[TK - 3]);
+                mx[1] = min3n(mx[1], x[TK - 2], x[TK - 1]);
+            } else {
+#pragma unroll
+                for (int e = 4; e < TK - 4; e += 8)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) mx[a] = max3n(mx[a], x[e + 2 * a], x[e + 2 * a + 1]);
+                mx[0] = max3n(mx[0], x[TK - 4], x[TK - 3]);
+                mx[1] = max3n(mx[1], x[TK - 2], x[TK - 1]);
+            }
+            float mt = use_min ? min3n(min3n(mx[0], mx[1], mx[2]), mx[3], mx[3])
+                               : max3n(max3n(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+            if (raw) mt *= sl;  // raw extreme -> logit maximum
+            float alpha = 1.0f;
+            bool rescale = false;
+            if (mt > m_used + 8.0f) {
+                alpha = m_used == NEG ? 0.0f : ex2(m_used - mt);
+                rescale = i > 0 && lsum > 0.0f;
+                m_used = mt;
+            }
+            const float ref = m_used == NEG ? 0.0f : m_used + p.shift;
+            float2 lsa[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            // Packed pairs overwrite the scores they came from, so P needs no
+            // registers of its own; one pair in eight takes the polynomial.
+            uint32_t* xb = reinterpret_cast<uint32_t*>(x);
+            const float2 sl2 = make_float2(raw ? sl : 1.0f, raw ? sl : 1.0f), nb2 = make_float2(-ref, -ref);
+#pragma unroll
+            for (int c = 0; c < TK / 32; ++c) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float2 z = __ffma2_rn(make_float2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), sl2, nb2);
+                    const float2 w = (e & 7) == 7 ? ex2_poly2(z) : make_float2(ex2(z.x), ex2(z.y));
+                    if (!p.fmt) lsa[e & 3] = __fadd2_rn(lsa[e & 3], w);
+                    xb[c * 32 + e] = pack2(w.x, w.y, p.fmt);
+                }
+                tmem_st16(tmem + lane_base + C::s_col(t) + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&xb[c * 32]));
+            }
+            if (__any_sync(0xffffffffu, rescale)) {
+                const float f = rescale ? alpha : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32(tmem + lane_base + C::o_col(t) + c * 32, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                    tmem_st32(tmem + lane_base + C::o_col(t) + c * 32, r);
+                }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[t]);
+            if (p.fmt) {  // BF16 P -> f32 is exact: the high half of the pattern
+#pragma unroll
+                for (int e = 0; e < TK / 2; ++e) {
+                    const uint32_t w = xb[(e / 16) * 32 + (e % 16)];
+                    lsa[e & 3] = __fadd2_rn(lsa[e & 3], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+                }
+            }
+            const float2 l2 = __fadd2_rn(__fadd2_rn(lsa[0], lsa[1]), __fadd2_rn(lsa[2], lsa[3]));
+            lsum = lsum * alpha + (l2.x + l2.y);
+        }
+        if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[t], 0))) ok = false;
+        const uint32_t esz = p.out_low ? 2u : 4u;
+        if (p.tma_out) {
+            // O / l staged in the idle K/V ring once both tiles' MMAs are
+            // done, written by TMA through the output's box map.
+            if (n_other > 0 && ok && !__all_sync(0xffffffffu, mbar_wait(&o_done[1 - t], 0))) ok = false;
+            if (!ok) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
+            tc_fence_after();
+            const bool load = ok && n > 0;
+            const float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
+            unsigned char* stage = sKV + (uint32_t)t * (TQ * D * esz);
+            const uint32_t swz = row & 7u;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t r[32];
+                if (load) {
+                    tmem_ld32(tmem + lane_base + C::o_col(t) + c * 32, r);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = 0u;
+                }
+                if (p.out_low) {  // boxes of 64 16-bit values: chunk c is half of box c / 2
+                    unsigned char* dst = stage + (c / 2) * (TQ * 128) + row * 128;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t q = (uint32_t)((c % 2) * 4 + e);
+                        *reinterpret_cast<uint4*>(dst + ((q ^ swz) * 16)) = make_uint4(
+                            encode_low_pair(__uint_as_float(r[8 * e]) * inv, __uint_as_float(r[8 * e + 1]) * inv, p.out_low),
+                            encode_low_pair(__uint_as_float(r[8 * e + 2]) * inv, __uint_as_float(r[8 * e + 3]) * inv, p.out_low),
+                            encode_low_pair(__uint_as_float(r[8 * e + 4]) * inv, __uint_as_float(r[8 * e + 5]) * inv, p.out_low),
+                            encode_low_pair(__uint_as_float(r[8 * e + 6]) * inv, __uint_as_float(r[8 * e + 7]) * inv, p.out_low));
+                    }
+                } else {  // boxes of 32 f32 values
+                    unsigned char* dst = stage + c * (TQ * 128) + row * 128;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        *reinterpret_cast<float4*>(dst + ((q ^ swz) * 16)) =
+                            make_float4(__uint_as_float(r[4 * q]) * inv, __uint_as_float(r[4 * q + 1]) * inv,
+                                        __uint_as_float(r[4 * q + 2]) * inv, __uint_as_float(r[4 * q + 3]) * inv);
+                }
+            }
+            tc_fence_before();
+            fence_proxy_async_smem();
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // every softmax warp's rows are staged
+            if (warp == 2 && lane == 0) {
+                const int boxes = p.out_low ? D / 64 : D / 32;
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+                    for (int bx = 0; bx < boxes && real[tt]; ++bx)
+                        tma_store_4d(&tmO, bx * (p.out_low ? 64 : 32), (int32_t)head0, (int32_t)l0[tt], (int32_t)b0[tt],
+                                     sKV + tt * (TQ * D * esz) + bx * (TQ * 128));
+                bulk_commit_group();
+                bulk_wait_read_all();
+            }
+        } else {
+            if (!ok) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
+            tc_fence_after();
+            const bool load = ok && n > 0;
+            float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
+            float* rec = nullptr;
+            if (p.part) {
+                inv = 1.0f;
+                rec = p.part + ((((uint64_t)b * p.H + head) * p.L + l) * p.part_stride + p.part_first + split) * REC<D>;
+                if (valid) {
+                    rec[0] = m_used == NEG ? 0.0f : m_used + p.shift;
+                    rec[1] = load ? lsum : 0.0f;
+                }
+                rec += 4;
+            }
+            const uint64_t at = (uint64_t)b * p.o_sb + (uint64_t)head * p.o_sh + (uint64_t)l * p.o_sl;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t r[32];
+                if (load) {
+                    tmem_ld32(tmem + lane_base + C::o_col(t) + c * 32, r);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = 0u;
+                }
+                if (!valid) continue;
+                if (p.part) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<uint4*>(rec + c * 32 + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
+                } else if (p.out_low) {  // rows 16-byte aligned (host)
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + c * 32);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        dst[e / 8] = make_uint4(
+                            encode_low_pair(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv, p.out_low),
+                            encode_low_pair(__uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv, p.out_low),
+                            encode_low_pair(__uint_as_float(r[e + 4]) * inv, __uint_as_float(r[e + 5]) * inv, p.out_low),
+                            encode_low_pair(__uint_as_float(r[e + 6]) * inv, __uint_as_float(r[e + 7]) * inv, p.out_low));
+                } else {
+                    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + c * 32);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        dst[e / 4] = make_float4(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv,
+                                                 __uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv);
+                }
+            }
+            tc_fence_before();
+        }
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------ joining records
+
+template <int D>
+struct RowPiece {  // the D / 32 columns lane * D / 32 .. of one row
+    static constexpr int N = D / 32;
+    float v[N];
+};
+template <int D>
+__device__ __forceinline__ RowPiece<D> load_piece(const float* rec, uint32_t lane) {
+    RowPiece<D> r;
+    if constexpr (D == 128) {
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(rec + 4) + lane);
+        r.v[0] = f.x, r.v[1] = f.y, r.v[2] = f.z, r.v[3] = f.w;
+    } else {
+        const float2 f = __ldcg(reinterpret_cast<const float2*>(rec + 4) + lane);
+        r.v[0] = f.x, r.v[1] = f.y;
+    }
+    return r;
+}
+template <int D>
+__device__ __forceinline__ void store_piece(void* out, uint32_t out_low, uint64_t row_at, uint32_t lane, const float (&o)[D / 32],
+                                            float inv) {
+    const uint64_t at = row_at + lane * (D / 32);
+    if (out_low) {
+        uint16_t* d = static_cast<uint16_t*>(out) + at;
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2)
+            *reinterpret_cast<uint32_t*>(d + i) = encode_low_pair(o[i] * inv, o[i + 1] * inv, out_low);
+    } else {
+        float* d = static_cast<float*>(out) + at;
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) *reinterpret_cast<float2*>(d + i) = make_float2(o[i] * inv, o[i + 1] * inv);
+    }
+}
+
+// A warp joins the records rec(0) .. rec(n - 1) of one row in order, after the
+// state {M, L, o} it has (L = 0, M = -inf: none).  Headers are read by the
+// lanes in parallel, then the rows with eight loads in flight.
+template <int D, typename Rec>
+__device__ __forceinline__ void join_records(uint32_t n, Rec rec, float& M, float& L, float (&o)[D / 32]) {
+    const uint32_t lane = threadIdx.x & 31;
+    const float NEG = -__int_as_float(0x7f800000);
+    float top = M;
+    for (uint32_t i = lane; i < n; i += 32) {
+        const float2 h = __ldcg(reinterpret_cast<const float2*>(rec(i)));
+        if (h.y != 0.0f) top = fmaxf(top, h.x);
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    if (top == NEG) return;
+    const float keep = L == 0.0f ? 0.0f : exp2f(M - top);
+    L *= keep;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] *= keep;
+    M = top;
+    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+        float2 h = make_float2(0.0f, 0.0f);
+        if (i0 + lane < n) h = __ldcg(reinterpret_cast<const float2*>(rec(i0 + lane)));
+        const float w = h.y == 0.0f ? 0.0f : exp2f(h.x - M);
+        const float lw = h.y * w;
+        const uint32_t m = min(n - i0, 32u);
+        for (uint32_t c = 0; c < m; c += 8) {
+            RowPiece<D> r[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e)
+                if (c + e < m) r[e] = load_piece<D>(rec(i0 + c + e), lane);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                if (c + e >= m) break;
+                const float wr = __shfl_sync(0xffffffffu, w, c + e);
+                L += __shfl_sync(0xffffffffu, lw, c + e);
+                if (wr == 0.0f) continue;  // nothing seen, or underflow: O is not multiplied by 0
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[i] = fmaf(r[e].v[i], wr, o[i]);
+            }
+        }
+    }
+}
+__device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 1.0f / l : 0.0f; }
+
+// One warp per row.
+struct SpanMergeParams {
+    const float* part;
+    uint64_t rows;
+    uint32_t count, H, L;
+    void* out;
+    uint32_t out_low;
+    uint64_t o_sb, o_sh, o_sl;
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
+    const uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (w >= p.rows) return;
+    float M = -__int_as_float(0x7f800000), L = 0.0f, o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
+    const float* part = p.part + w * p.count * REC<D>;
+    join_records<D>(p.count, [&](uint32_t i) { return part + i * REC<D>; }, M, L, o);
+    const uint64_t q = w % p.L, h = w / p.L % p.H, b = w / p.L / p.H;
+    store_piece<D>(p.out, p.out_low, b * p.o_sb + h * p.o_sh + q * p.o_sl, threadIdx.x & 31, o, inverse(L));
+}
+
+// ---------------------------------------------------------- few query rows
+//
+// At most 16 query rows share a key/value head (G x L): one 16-row block of
+// warp-level MMAs (m16n8k16) per (sequence, key/value head), as in
+// attn_decode16_kernel (see there for the depth permutation and the combine),
+// over exactly the keys that the rows see: virtual key v of a sequence is key
+// v < s ? v : v + lo - s, with s first keys and the window [lo, hi].
+//
+// Work split: the visible keys of all (sequence, key/value head) units, in
+// 64-key tiles, are dealt out evenly: CTA c takes the tiles [c q, (c + 1) q)
+// of their concatenation, whatever unit borders fall inside, so that ragged
+// lengths and unit counts that do not divide the GPU leave no SM idle.  Each
+// CTA finds its first unit from a block scan over the lengths.  Per unit that
+// a CTA enters, its four warps take a quarter of the keys each through
+// three-stage cp.async rings and combine in shared memory.  A unit inside one
+// CTA is finished there; otherwise its CTAs leave records and the last to
+// arrive (a counter per unit, reset by it) joins them in CTA order, so results
+// do not depend on who is last.  Records of the shared prefix, written by
+// span_tile_kernel just before, are joined at the same place; the launch
+// overlaps that kernel's end (programmatic dependent launch).
+// Bound: HBM, the visible keys and values once.
+constexpr int DTILE = 64;  // keys: 16 per warp and step
+
+struct SpanDecodeParams {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sk, v_sb, v_sh, v_sk;
+    uint32_t B, H, Hkv, G, L, Lk;
+    const uint32_t* lengths;
+    uint64_t length_stride;
+    int64_t offset, window, sinks;
+    float scale_log2, shift;
+    float* part;          // two records x 16 rows per CTA
+    uint32_t* arrived;    // per unit, 0 between launches
+    const float* prefix;  // ((b * H + h) * L + l) * prefix_count + i, or null
+    uint32_t prefix_count;
+    void* out;
+    uint32_t out_low;
+    uint64_t o_sb, o_sh, o_sl;
+};
+
+struct UnitKeys {
+    int64_t base;             // position of query 0
+    uint32_t s, lo, count;    // first keys, window start, visible keys
+    uint32_t tiles;           // at least 1, so that every unit has a CTA
+};
+__device__ __forceinline__ UnitKeys unit_keys(const SpanDecodeParams& p, uint32_t b) {
+    int64_t n = p.Lk;
+    UnitKeys u;
+    u.base = p.offset;
+    if (p.lengths) {
+        n = min(n, (int64_t)p.lengths[b * p.length_stride]);
+        u.base = n - (int64_t)p.L;
+    }
+    const Reach r = reach(u.base, u.base + (int64_t)p.L - 1, n, p.window, p.sinks);
+    u.s = (uint32_t)r.first;
+    u.lo = (uint32_t)min(r.lo, (int64_t)p.Lk);
+    u.count = u.s + (r.hi >= r.lo ? (uint32_t)(r.hi - r.lo + 1) : 0u);
+    u.tiles = max(1u, (u.count + DTILE - 1) / DTILE);
+    return u;
+}
+
+template <int D>
+struct DCfg {
+    static constexpr int CPR = D / 8;            // 16-byte chunks per K / V row
+    static constexpr int STAGE = 2 * 16 * CPR;   // chunks per stage: 16 K rows, 16 V rows
+    static constexpr int RING = DEC_STAGES * STAGE;
+    static constexpr int SMEM = DEC_WARPS * RING * 16;
+    static_assert(RING * 16 >= (16 * (D + 2) + 16 * REC<D>) * 4, "the combine's records fit a warp's ring");
+};
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeParams p) {
+    using C = DCfg<D>;
+    constexpr int QW = D / 8, KS = D / 16, NJ = D / 8, CPR = C::CPR, STAGE = C::STAGE;
+    extern __shared__ uint4 dsm[];
+    __shared__ uint32_t scan[DEC_WARPS], found[2], last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, c = lane & 3;
+    uint4* ring = dsm + (size_t)warp * C::RING;
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+    // the CTA's combined records: the upper half of warp 0's ring
+    float* cmb = reinterpret_cast<float*>(dsm) + ((16 * (D + 2) + 3) / 4) * 4;
+    const uint32_t R = p.G * p.L;
+    const float NEG = -__int_as_float(0x7f800000);
+
+    // This CTA's tiles and its first unit.
+    uint32_t T, t_begin, b, hkv, tin;
+    if (!p.lengths) {
+        const uint32_t tpu = unit_keys(p, 0).tiles;
+        T = p.B * p.Hkv * tpu;
+        const uint32_t q = (T + gridDim.x - 1) / gridDim.x;
+        t_begin = blockIdx.x * q;
+        b = t_begin / (tpu * p.Hkv), hkv = t_begin / tpu % p.Hkv, tin = t_begin % tpu;
+    } else {
+        const uint32_t per = (p.B + 32 * DEC_WARPS - 1) / (32 * DEC_WARPS);
+        const uint32_t b0 = min(threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+        uint32_t mine = 0;
+        for (uint32_t i = b0; i < b1; ++i) mine += unit_keys(p, i).tiles * p.Hkv;
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += x;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        uint32_t before = incl - mine;
+        T = 0;
+#pragma unroll
+        for (int w = 0; w < DEC_WARPS; ++w) {
+            if (w < warp) before += scan[w];
+            T += scan[w];
+        }
+        const uint32_t q = (T + gridDim.x - 1) / gridDim.x;
+        t_begin = blockIdx.x * q;
+        if (t_begin >= before && t_begin < before + mine) {
+            uint32_t at = before, i = b0;
+            for (; i + 1 < b1; ++i) {
+                const uint32_t n = unit_keys(p, i).tiles * p.Hkv;
+                if (t_begin < at + n) break;
+                at += n;
+            }
+            found[0] = i, found[1] = t_begin - at;
+        }
+        __syncthreads();
+        b = found[0];
+        const uint32_t tpu = t_begin < T ? unit_keys(p, b).tiles : 1u;
+        hkv = found[1] / tpu, tin = found[1] % tpu;
+    }
+    const uint32_t per_cta = (T + gridDim.x - 1) / gridDim.x;
+    if (t_begin >= T) return;
+    const uint32_t t_end = min(t_begin + per_cta, T);
+
+    for (uint32_t t = t_begin; t < t_end;) {
+        const UnitKeys u = unit_keys(p, b);
+        const uint32_t seg = min(u.tiles - tin, t_end - t);
+        const uint32_t v_begin = tin * DTILE, v_end = min((tin + seg) * DTILE, u.count);
+        const uint32_t quarter = ((v_end > v_begin ? v_end - v_begin : 0u) + 16 * DEC_WARPS - 1) / (16 * DEC_WARPS) * 16;
+        const uint32_t k_begin = min(v_begin + warp * quarter, v_end), k_end = min(k_begin + quarter, v_end);
+        // Q fragments of rows g and g + 8 (zeros past R); row r is query head r / L, query r % L
+        uint32_t qa[2][QW];
+        int32_t high[2], low[2];  // keys (sinks or [low, high]) of the rows
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+            const uint32_t r = (uint32_t)(g + 8 * rr);
+            const int64_t pos = u.base + (int64_t)(r % p.L);
+            high[rr] = r < R ? (int32_t)max((int64_t)-1, min(pos, (int64_t)p.Lk)) : -1;
+            low[rr] = (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
+            if (r < R) {
+                const uint32_t h = hkv * p.G + r / p.L, l = r % p.L;
+                const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.q_sb + h * p.q_sh + l * p.q_sl + c * (D / 4));
+#pragma unroll
+                for (int i = 0; i < QW / 4; ++i) {
+                    const uint4 w = src[i];
+                    qa[rr][4 * i] = w.x, qa[rr][4 * i + 1] = w.y, qa[rr][4 * i + 2] = w.z, qa[rr][4 * i + 3] = w.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < QW; ++i) qa[rr][i] = 0u;
+            }
+        }
+        const uint32_t skip = u.lo - u.s;
+        const int32_t sinks = (int32_t)min((int64_t)0x7fffffff, p.sinks);
+        const uint16_t* kbase = p.k + (uint64_t)b * p.k_sb + (uint64_t)hkv * p.k_sh;
+        const uint16_t* vbase = p.v + (uint64_t)b * p.v_sb + (uint64_t)hkv * p.v_sh;
+        // One stage: virtual keys v0 .. v0 + 15 of K then V, 16 bytes per copy;
+        // keys past the range are zero-filled (source size 0, address in bounds).
+        auto issue = [&](uint32_t v0, int slot) {
+            const uint32_t dst0 = ring_s + (uint32_t)(slot * STAGE * 16);
+#pragma unroll
+            for (int n = 0; n < STAGE / 32; ++n) {
+                const uint32_t e = (uint32_t)(lane + 32 * n);
+                const uint32_t kv = e / (16 * CPR), row = (e / CPR) % 16, chunk = e % CPR;
+                const bool in = v0 + row < k_end;
+                const uint32_t vk = in ? v0 + row : k_begin, key = vk < u.s ? vk : vk + skip;
+                const uint16_t* src = kv ? vbase + (uint64_t)key * p.v_sk + chunk * 8 : kbase + (uint64_t)key * p.k_sk + chunk * 8;
+                const uint32_t pc = kv ? v_chunk(row, chunk) : k_chunk<D>(row, chunk);
+                cp_async16(dst0 + (kv * 16 * CPR + row * CPR + pc) * 16, src, in ? 16u : 0u);
+            }
+        };
+        float o[NJ][4];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
+        float m[2] = {NEG, NEG}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < DEC_STAGES - 1; ++st) {
+            if (k_begin + 16 * st < k_end) issue(k_begin + 16 * st, st);
+            cp_async_commit();
+        }
+        int slot = 0;
+        for (uint32_t v0 = k_begin; v0 < k_end; v0 += 16) {
+            cp_async_wait<DEC_STAGES - 2>();  // this stage's copies (all but the newest group) have landed
+            __syncwarp();
+            const uint4* kst = ring + slot * STAGE;
+            const uint4* vst = kst + 16 * CPR;
+            float s[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                uint32_t kw[QW];
+                const uint32_t row = (uint32_t)(8 * n + g);
+#pragma unroll
+                for (int i = 0; i < QW / 4; ++i) {
+                    const uint4 w = kst[row * CPR + k_chunk<D>(row, (uint32_t)(c * (QW / 4) + i))];
+                    kw[4 * i] = w.x, kw[4 * i + 1] = w.y, kw[4 * i + 2] = w.z, kw[4 * i + 3] = w.w;
+                }
+                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+                    mma16816<FMT>(s[n], qa[0][2 * ks], qa[1][2 * ks], qa[0][2 * ks + 1], qa[1][2 * ks + 1], kw[2 * ks],
+                                  kw[2 * ks + 1]);
+            }
+            // V words of keys 2c, 2c+1, 2c+8, 2c+9 at columns g*D/8 ..
+            uint32_t vw[4][NJ / 2];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t row = (uint32_t)(2 * c + (n & 1) + 8 * (n >> 1));
+                if constexpr (NJ / 8 == 2) {
+                    const uint32_t odd = (uint32_t)(g & 1);
+                    const uint4 w0 = vst[row * CPR + v_chunk(row, (uint32_t)(2 * g) + odd)];
+                    const uint4 w1 = vst[row * CPR + v_chunk(row, (uint32_t)(2 * g) + (odd ^ 1u))];
+                    const uint4 lo = odd ? w1 : w0, hi = odd ? w0 : w1;
+                    vw[n][0] = lo.x, vw[n][1] = lo.y, vw[n][2] = lo.z, vw[n][3] = lo.w;
+                    vw[n][4] = hi.x, vw[n][5] = hi.y, vw[n][6] = hi.z, vw[n][7] = hi.w;
+                } else {
+                    const uint4 w = vst[row * CPR + v_chunk(row, (uint32_t)g)];
+                    vw[n][0] = w.x, vw[n][1] = w.y, vw[n][2] = w.z, vw[n][3] = w.w;
+                }
+            }
+            __syncwarp();  // every lane has read this slot: it may be refilled
+            if (v0 + 16 * (DEC_STAGES - 1) < k_end) issue(v0 + 16 * (DEC_STAGES - 1), (slot + DEC_STAGES - 1) % DEC_STAGES);
+            cp_async_commit();
+            slot = slot + 1 == DEC_STAGES ? 0 : slot + 1;
+            // scores in log2 units, masked: s[n][e] is row g + 8 * (e >> 1), virtual key v0 + 8n + 2c + (e & 1)
+            float mx[2] = {NEG, NEG};
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int rr = e >> 1;
+                    const uint32_t vk = v0 + 8 * n + 2 * c + (e & 1);
+                    const int32_t key = (int32_t)(vk < u.s ? vk : vk + skip);
+                    const bool seen = vk < k_end && key <= high[rr] && (key >= low[rr] || key < sinks);
+                    const float x = seen ? s[n][e] * p.scale_log2 : NEG;
+                    s[n][e] = x;
+                    mx[rr] = fmaxf(mx[rr], x);
+                }
+            float alpha[2], base[2];
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+                mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xffffffffu, mx[rr], 1));
+                mx[rr] = fmaxf(mx[rr], __shfl_xor_sync(0xffffffffu, mx[rr], 2));
+                const float mn = fmaxf(m[rr], mx[rr]);
+                alpha[rr] = m[rr] == NEG ? 0.0f : ex2(m[rr] - mn);
+                m[rr] = mn;
+                base[rr] = mn == NEG ? 0.0f : mn + p.shift;
+            }
+            // P as the A operand of PV: rows g / g + 8, keys 2c, 2c+1 (tile 0) and 8 + 2c, 9 + 2c (tile 1)
+            uint32_t pa[4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int rr = 0; rr < 2; ++rr)
+                    pa[2 * n + rr] = pack2(ex2(s[n][2 * rr] - base[rr]), ex2(s[n][2 * rr + 1] - base[rr]), FMT);
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr) {
+                const float2 w0 = unpack2<FMT>(pa[rr]), w1 = unpack2<FMT>(pa[2 + rr]);
+                l[rr] = fmaf(l[rr], alpha[rr], (w0.x + w0.y) + (w1.x + w1.y));
+            }
+            if (__any_sync(0xffffffffu, alpha[0] != 1.0f || alpha[1] != 1.0f)) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    o[j][0] *= alpha[0], o[j][1] *= alpha[0];
+                    o[j][2] *= alpha[1], o[j][3] *= alpha[1];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const uint32_t half = (j & 1) ? 0x7632u : 0x5410u;  // high or low 16-bit halves of the word pair
+                const uint32_t b0 = __byte_perm(vw[0][j / 2], vw[1][j / 2], half);
+                const uint32_t b1 = __byte_perm(vw[2][j / 2], vw[3][j / 2], half);
+                mma16816<FMT>(o[j], pa[0], pa[1], pa[2], pa[3], b0, b1);
+            }
+        }
+        cp_async_wait<0>();
+        // The warps combine: each leaves {m, l, O} per row in its own (drained)
+        // ring, then the CTA writes one record per row to `cmb`.
+        float* xs = reinterpret_cast<float*>(ring);  // [16 rows][D + 2]
+        __syncwarp();
+#pragma unroll
+        for (int rr = 0; rr < 2; ++rr) {
+            l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
+            l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 2);
+            float* x = xs + (g + 8 * rr) * (D + 2);
+            if (c == 0) {
+                x[0] = m[rr];
+                x[1] = l[rr];
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                x[2 + 2 * c * NJ + j] = o[j][2 * rr];
+                x[2 + (2 * c + 1) * NJ + j] = o[j][2 * rr + 1];
+            }
+        }
+        __syncthreads();
+        const bool whole = tin == 0 && seg == u.tiles;
+        float* part = p.part + ((uint64_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * 16 * REC<D>;
+        for (uint32_t r = 0; r < R; ++r) {
+            float mw[DEC_WARPS], lw[DEC_WARPS], M = NEG;
+#pragma unroll
+            for (int w = 0; w < DEC_WARPS; ++w) {
+                const float* x = reinterpret_cast<const float*>(dsm + (size_t)w * C::RING) + r * (D + 2);
+                mw[w] = x[0], lw[w] = x[1];
+                if (lw[w] != 0.0f) M = fmaxf(M, mw[w]);
+            }
+            float wt[DEC_WARPS], Lr = 0.0f;
+#pragma unroll
+            for (int w = 0; w < DEC_WARPS; ++w) {
+                wt[w] = lw[w] != 0.0f ? exp2f(mw[w] - M) : 0.0f;
+                Lr = fmaf(lw[w], wt[w], Lr);
+            }
+            float* rec = (whole ? cmb : part) + r * REC<D>;
+            if (threadIdx.x == 0) {
+                rec[0] = M == NEG ? 0.0f : M + p.shift;
+                rec[1] = Lr;
+            }
+            for (uint32_t d = threadIdx.x; d < (uint32_t)D; d += 32 * DEC_WARPS) {
+                float acc = 0.0f;
+#pragma unroll
+                for (int w = 0; w < DEC_WARPS; ++w)
+                    if (wt[w] != 0.0f)
+                        acc = fmaf(reinterpret_cast<const float*>(dsm + (size_t)w * C::RING)[r * (D + 2) + 2 + d], wt[w], acc);
+                rec[4 + d] = acc;
+            }
+        }
+        // Which CTAs share the unit: those of its first and last tiles.
+        const uint32_t u_begin = t - tin, c0 = u_begin / per_cta, c1 = (u_begin + u.tiles - 1) / per_cta;
+        bool finish = whole;
+        if (!whole) {
+            __threadfence();  // this thread's record values before the arrival
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                uint32_t* at = p.arrived + (uint64_t)b * p.Hkv + hkv;
+                const uint32_t n = atomicAdd(at, 1u);
+                last = n == c1 - c0;
+                if (last) *at = 0u;  // re-armed for the next launch
+                __threadfence();
+            }
+            __syncthreads();
+            finish = last;
+        } else {
+            __syncthreads();  // cmb
+        }
+        if (finish) {
+            if (p.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's records are written
+            for (uint32_t r = warp; r < R; r += DEC_WARPS) {
+                float M = NEG, Lr = 0.0f, acc[D / 32];
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
+                if (whole) {
+                    const float* rec = cmb + r * REC<D>;
+                    if (rec[1] != 0.0f) {
+                        M = rec[0], Lr = rec[1];
+#pragma unroll
+                        for (int i = 0; i < D / 32; ++i) acc[i] = rec[4 + lane * (D / 32) + i];
+                    }
+                } else {
+                    // CTA c0 entered the unit as its first segment only if the
+                    // unit begins at the CTA's first tile
+                    const uint32_t second = u_begin == c0 * per_cta ? 0u : 1u;
+                    join_records<D>(c1 - c0 + 1,
+                                    [&](uint32_t i) {
+                                        return p.part + (((uint64_t)(c0 + i) * 2 + (i == 0 ? second : 0u)) * 16 + r) * REC<D>;
+                                    },
+                                    M, Lr, acc);
+                }
+                const uint32_t h = hkv * p.G + r / p.L, q = r % p.L;
+                if (p.prefix) {
+                    const float* pre = p.prefix + (((uint64_t)b * p.H + h) * p.L + q) * p.prefix_count * REC<D>;
+                    join_records<D>(p.prefix_count, [&](uint32_t i) { return pre + i * REC<D>; }, M, Lr, acc);
+                }
+                store_piece<D>(p.out, p.out_low, (uint64_t)b * p.o_sb + (uint64_t)h * p.o_sh + (uint64_t)q * p.o_sl, lane, acc,
+                               inverse(Lr));
+            }
+        }
+        __syncthreads();  // the rings and cmb are free again
+        t += seg;
+        tin = 0;
+        if (++hkv == p.Hkv) hkv = 0, ++b;
+    }
+    if (p.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ------------------------------------------------------------------ host
+
+// A rank-4 map {D, n1, n2, n3} with element strides s[0..2] of the outer axes
+// (unit axes: any) and 128-byte boxes {128 / esz, box[0..2]}; false when the
+// strides or the base do not suit TMA.
+bool span_map(CUtensorMap* map, const void* ptr, uint32_t dtype, uint64_t D, const uint64_t (&n)[3], const uint64_t (&s)[3],
+              const uint32_t (&box)[3], bool promote) {
+    auto enc = encode_tiled_attn();
+    if (!enc || reinterpret_cast<uintptr_t>(ptr) % 16) return false;
+    const uint64_t esz = dtype == FB_F32 ? 4 : 2;
+    cuuint64_t dims[4] = {D, n[0], n[1], n[2]}, strides[3];
+    uint64_t filler = (D * esz + 15) / 16 * 16;
+    for (int i = 0; i < 3; ++i) {
+        uint64_t sb = s[i] * esz;
+        if (n[i] == 0 || n[i] > (1ull << 31)) return false;
+        if (n[i] == 1 && (sb == 0 || sb % 16 || sb >= (1ull << 40))) sb = filler;
+        if (sb == 0 || sb % 16 || sb >= (1ull << 40)) return false;
+        strides[i] = sb;
+        filler = (sb * n[i] + 15) / 16 * 16;
+        if (filler >= (1ull << 40)) filler = 16;
+    }
+    const cuuint32_t b4[4] = {(cuuint32_t)(128 / esz), box[0], box[1], box[2]}, estr[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = dtype == FB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : dtype == FB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                        : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return enc(map, type, 4, const_cast<void*>(ptr), dims, strides, b4, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, promote ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Operands of a call the tensor cores take: layouts with merged batch axes.
+struct SpanOperands {
+    RowsLayout q, k, v, o;
+    uint64_t B, H, Hkv, L, Lk, G;
+    uint32_t fmt;
+    const void *qp, *kp, *vp;
+    void* op;
+};
+
+float weight_shift(uint32_t fmt, uint64_t keys) {  // see attn_fwd_kernel: BF16 weights pre-scaled by 2^-shift
+    return fmt ? 9.0f + std::ceil(std::log2((float)std::max<uint64_t>(keys, 1))) : 0.0f;
+}
+
+uint64_t largest_divisor(uint64_t n, uint64_t most) {
+    uint64_t d = std::min(n, most);
+    while (n % d) --d;
+    return d;
+}
+
+// The tcgen05 kernel over the shared prefix (shared = true) or over the
+// sequences' own keys.  part: records are written there (stride and first
+// index given; `splits` ranges), else output rows.
+template <int D>
+int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* part, uint32_t part_stride, uint32_t part_first,
+                 uint32_t splits, float shift, cudaStream_t st) {
+    using C = TCfg<D>;
+    SpanTileParams p{};
+    p.fmt = a.fmt;
+    p.B = (uint32_t)a.B, p.H = (uint32_t)a.H, p.L = (uint32_t)a.L;
+    p.Lk = (uint32_t)(shared ? s.prefix_keys : a.Lk);
+    p.group = (uint32_t)a.G;
+    p.GB = (uint32_t)largest_divisor(a.G, TQ);
+    p.LB = (uint32_t)std::min<uint64_t>(a.L, TQ / p.GB);
+    p.NB = shared ? (uint32_t)std::min<uint64_t>(a.B, std::max<uint64_t>(1, a.L == p.LB ? TQ / (p.GB * p.LB) : 1)) : 1u;
+    p.rows = p.GB * p.LB * p.NB;
+    p.l_tiles = (p.L + p.LB - 1) / p.LB;
+    p.tiles = shared ? p.l_tiles * ((p.B + p.NB - 1) / p.NB) : p.l_tiles;
+    p.pairs = (p.tiles + 1) / 2;
+    p.head_blocks = p.H / p.GB;
+    p.units = shared ? p.head_blocks : p.head_blocks * p.B;
+    p.shared_keys = shared ? 1 : 0;
+    p.k_batch_bcast = a.k.batch_bcast ? 1 : 0, p.v_batch_bcast = a.v.batch_bcast ? 1 : 0;
+    p.lengths = shared ? nullptr : s.lengths;
+    p.length_stride = s.length_stride;
+    p.offset = s.offset, p.window = (int64_t)s.window, p.sinks = (int64_t)s.sinks;
+    p.scale_log2 = s.base.scale * 1.4426950408889634f;
+    p.shift = shift;
+    p.splits = splits;
+    p.part = part, p.part_stride = part_stride, p.part_first = part_first;
+    p.out = a.op, p.out_low = s.base.out_low;
+    p.o_sb = a.o.s_batch, p.o_sh = a.o.s_head, p.o_sl = a.o.s_row;
+    CUtensorMap tq, tk, tv, to{};
+    const uint32_t dt = a.fmt ? FB_BF16 : FB_F16;
+    const uint32_t qbox[3] = {p.GB, p.LB, p.NB}, kbox[3] = {TK, 1, 1};
+    if (!span_map(&tq, a.qp, dt, D, {a.H, a.L, a.B}, {a.q.s_head, a.q.s_row, a.q.s_batch}, qbox, true)) return FB_ERR_UNSUPPORTED;
+    if (shared) {
+        const uint16_t* pk = static_cast<const uint16_t*>(s.pk) + s.pk_offset;
+        const uint16_t* pv = static_cast<const uint16_t*>(s.pv) + s.pv_offset;
+        if (!span_map(&tk, pk, dt, D, {s.prefix_keys, a.Hkv, 1}, {s.pk_stride_key, s.pk_stride_head, 0}, kbox, true) ||
+            !span_map(&tv, pv, dt, D, {s.prefix_keys, a.Hkv, 1}, {s.pv_stride_key, s.pv_stride_head, 0}, kbox, true))
+            return FB_ERR_UNSUPPORTED;
+    } else {
+        if (!span_map(&tk, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox, true) ||
+            !span_map(&tv, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox, true))
+            return FB_ERR_UNSUPPORTED;
+    }
+    if (!part)
+        p.tma_out = span_map(&to, a.op, s.base.out_low ? s.base.out_low : (uint32_t)FB_F32, D, {a.H, a.L, a.B},
+                             {a.o.s_head, a.o.s_row, a.o.s_batch}, qbox, false)
+                        ? 1
+                        : 0;
+    const uint64_t grid = (uint64_t)p.units * p.pairs * splits;
+    if (grid > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
+    if (cudaFuncSetAttribute(span_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+        return launch_status("shared-memory attribute");
+    span_tile_kernel<D><<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, to, p);
+    count_launch(kernel_name("span_tile_kernel", {D, shared ? 1 : 0}).c_str());
+    return launch_status("kernel launch");
+}
+
+// CTAs of one key range and the key tiles that such a CTA walks at most.
+template <int D>
+void tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared, uint64_t* ctas, uint64_t* key_tiles) {
+    const uint64_t GB = largest_divisor(a.G, TQ), LB = std::min<uint64_t>(a.L, TQ / GB);
+    const uint64_t l_tiles = (a.L + LB - 1) / LB;
+    if (shared) {
+        const uint64_t NB = std::min<uint64_t>(a.B, std::max<uint64_t>(1, a.L == LB ? TQ / (GB * LB) : 1));
+        *ctas = a.H / GB * ((l_tiles * ((a.B + NB - 1) / NB) + 1) / 2);
+        *key_tiles = (s.prefix_keys + TK - 1) / TK;
+    } else {
+        *ctas = a.B * (a.H / GB) * ((l_tiles + 1) / 2);
+        const uint64_t all = (a.Lk + TK - 1) / TK;
+        const uint64_t seen = (std::min(s.sinks, a.Lk) + TK - 1) / TK + (std::min(s.window, a.Lk) + 2 * LB + TK - 1) / TK + 1;
+        *key_tiles = std::min(all, seen);
+    }
+}
+
+// Key ranges that fill the GPU when the pairs alone do not: about one CTA
+// per SM, at least two key tiles each.
+uint64_t tile_splits(uint64_t ctas, uint64_t key_tiles) {
+    const uint64_t sms = (uint64_t)sm_count();
+    if (ctas >= sms || key_tiles < 4) return 1;
+    const uint64_t splits = std::min<uint64_t>(sms / ctas, key_tiles / 2);
+    if (splits <= 1) return 1;
+    const uint64_t per = (key_tiles + splits - 1) / splits;
+    return (key_tiles + per - 1) / per;
+}
+
+template <int D>
+int launch_merge(const SpanArgs& s, const SpanOperands& a, const float* part, uint32_t count, cudaStream_t st) {
+    SpanMergeParams m{};
+    m.part = part;
+    m.rows = a.B * a.H * a.L;
+    m.count = count;
+    m.H = (uint32_t)a.H, m.L = (uint32_t)a.L;
+    m.out = a.op, m.out_low = s.base.out_low;
+    m.o_sb = a.o.s_batch, m.o_sh = a.o.s_head, m.o_sl = a.o.s_row;
+    if ((m.rows + 7) / 8 > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
+    span_merge_kernel<D><<<(unsigned)((m.rows + 7) / 8), 256, 0, st>>>(m);
+    count_launch(kernel_name("span_merge_kernel", {D}).c_str());
+    return launch_status("kernel launch");
+}
+
+template <int D>
+int launch_decode(const SpanArgs& s, const SpanOperands& a, const float* prefix, uint32_t prefix_count, float shift,
+                  cudaStream_t st) {
+    const uint64_t units = a.B * a.Hkv;
+    // The most 64-key tiles that a unit can have, over all lengths.
+    const uint64_t seen = std::min<uint64_t>(a.Lk, std::min(s.sinks, a.Lk) + std::min(s.window, a.Lk) + a.L);
+    const uint64_t tiles = units * std::max<uint64_t>(1, (seen + DTILE - 1) / DTILE);
+    if (tiles > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
+    // Two CTAs per SM, at least two tiles each once every SM has one.
+    const uint64_t sms = (uint64_t)sm_count();
+    const uint64_t grid = tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
+    SpanDecodeParams d{};
+    d.part = static_cast<float*>(scratch(st, grid * 2 * 16 * REC<D> * sizeof(float), SCRATCH_SPAN_PART));
+    d.arrived = static_cast<uint32_t*>(scratch(st, units * sizeof(uint32_t), SCRATCH_SPAN_COUNT));
+    if (!d.part || !d.arrived) return FB_ERR_DRIVER;
+    d.q = static_cast<const uint16_t*>(a.qp), d.k = static_cast<const uint16_t*>(a.kp), d.v = static_cast<const uint16_t*>(a.vp);
+    d.q_sb = a.q.s_batch, d.q_sh = a.q.s_head, d.q_sl = a.q.s_row;
+    d.k_sb = a.k.batch_bcast ? 0 : a.k.s_batch, d.k_sh = a.k.s_head, d.k_sk = a.k.s_row;
+    d.v_sb = a.v.batch_bcast ? 0 : a.v.s_batch, d.v_sh = a.v.s_head, d.v_sk = a.v.s_row;
+    d.B = (uint32_t)a.B, d.H = (uint32_t)a.H, d.Hkv = (uint32_t)a.Hkv, d.G = (uint32_t)a.G;
+    d.L = (uint32_t)a.L, d.Lk = (uint32_t)a.Lk;
+    d.lengths = s.lengths, d.length_stride = s.length_stride;
+    d.offset = s.offset, d.window = (int64_t)s.window, d.sinks = (int64_t)s.sinks;
+    d.scale_log2 = s.base.scale * 1.4426950408889634f;
+    d.shift = shift;
+    d.prefix = prefix, d.prefix_count = prefix_count;
+    d.out = a.op, d.out_low = s.base.out_low;
+    d.o_sb = a.o.s_batch, d.o_sh = a.o.s_head, d.o_sl = a.o.s_row;
+    auto kernel = a.fmt ? span_decode_kernel<D, 1> : span_decode_kernel<D, 0>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DCfg<D>::SMEM) != cudaSuccess)
+        return launch_status("shared-memory attribute");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(32 * DEC_WARPS);
+    cfg.dynamicSmemBytes = DCfg<D>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = prefix ? 1 : 0;
+    (void)cudaLaunchKernelEx(&cfg, kernel, d);
+    count_launch(kernel_name("span_decode_kernel", {D, (int)a.fmt}).c_str());
+    return launch_status("kernel launch");
+}
+
+template <int D>
+int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
+    const bool prefix = s.prefix_keys > 0, own = a.Lk > 0;
+    const float shift = weight_shift(a.fmt, a.Lk + s.prefix_keys);
+    uint64_t pc = 0, pt = 0, oc = 0, ot = 0;
+    if (prefix) tile_grid<D>(s, a, true, &pc, &pt);
+    if (own) tile_grid<D>(s, a, false, &oc, &ot);
+    const uint64_t ps = prefix ? tile_splits(pc, pt) : 0;
+    if (a.G * a.L <= 16) {  // few rows: the own keys streamed, the prefix's records joined there
+        float* part = nullptr;
+        if (prefix) {
+            part = static_cast<float*>(scratch(st, a.B * a.H * a.L * ps * REC<D> * sizeof(float), SCRATCH_SPAN));
+            if (!part) return FB_ERR_DRIVER;
+            if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)ps, 0, (uint32_t)ps, shift, st); r != FB_OK) return r;
+        }
+        return launch_decode<D>(s, a, part, (uint32_t)ps, shift, st);
+    }
+    const uint64_t os = own ? tile_splits(oc, ot) : 0;
+    if (ps + os <= 1) return launch_tiles<D>(s, a, prefix, nullptr, 0, 0, 1, shift, st);
+    const uint64_t count = ps + os;
+    float* part = static_cast<float*>(scratch(st, a.B * a.H * a.L * count * REC<D> * sizeof(float), SCRATCH_SPAN));
+    if (!part) return FB_ERR_DRIVER;
+    if (prefix)
+        if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)count, 0, (uint32_t)ps, shift, st); r != FB_OK) return r;
+    if (own)
+        if (int r = launch_tiles<D>(s, a, false, part, (uint32_t)count, (uint32_t)ps, (uint32_t)os, shift, st); r != FB_OK) return r;
+    return launch_merge<D>(s, a, part, (uint32_t)count, st);
+}
+
+}  // namespace
+
+uint32_t read_span_status() {
+    uint32_t v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_span_status, sizeof(v)) != cudaSuccess) return 0xffffffffu;
+    cudaMemcpyToSymbol(g_span_status, &zero, sizeof(zero));
+    return v;
+}
+
+int launch_span_tc(const SpanArgs& s, void* stream) {
+    const AttnArgs& a = s.base;
+    if (a.dtype != FB_BF16 && a.dtype != FB_F16) return FB_ERR_UNSUPPORTED;
+    if (a.depth != a.value_depth || (a.depth != 64 && a.depth != 128)) return FB_ERR_UNSUPPORTED;
+    if (a.row_rank < 2 || a.rows == 0 || (a.keys == 0 && s.prefix_keys == 0)) return FB_ERR_UNSUPPORTED;
+    if (a.q_stride_d != 1 || a.o_stride_d != 1) return FB_ERR_UNSUPPORTED;
+    if (a.keys > 0 && (a.k_stride_d != 1 || a.v_stride_d != 1)) return FB_ERR_UNSUPPORTED;
+    if (s.prefix_keys > 0 && (s.pk_stride_d != 1 || s.pv_stride_d != 1)) return FB_ERR_UNSUPPORTED;
+    const int r = (int)a.row_rank;
+    SpanOperands x;
+    x.L = a.row_dims[r - 1], x.H = a.row_dims[r - 2], x.Lk = a.keys, x.G = a.group_size;
+    x.Hkv = x.H / x.G;
+    x.fmt = a.dtype == FB_BF16 ? 1 : 0;
+    if (x.L > (1u << 30) || x.Lk > (1u << 30) || s.prefix_keys > (1u << 30)) return FB_ERR_UNSUPPORTED;
+    x.q.rows = x.L, x.q.heads = x.H, x.q.s_row = a.q_row_strides[r - 1], x.q.s_head = a.q_row_strides[r - 2];
+    x.k.rows = x.Lk, x.k.heads = x.Hkv, x.k.s_row = a.k_stride_key, x.k.s_head = a.k_row_strides[r - 2];
+    x.v.rows = x.Lk, x.v.heads = x.Hkv, x.v.s_row = a.v_stride_key, x.v.s_head = a.v_row_strides[r - 2];
+    x.o.rows = x.L, x.o.heads = x.H, x.o.s_row = a.o_row_strides[r - 1], x.o.s_head = a.o_row_strides[r - 2];
+    if (!merge_batch(a, a.q_row_strides, r - 2, &x.q) || !merge_batch(a, a.k_row_strides, r - 2, &x.k) ||
+        !merge_batch(a, a.v_row_strides, r - 2, &x.v) || !merge_batch(a, a.o_row_strides, r - 2, &x.o))
+        return FB_ERR_UNSUPPORTED;
+    if (x.q.batch_bcast || x.o.batch_bcast) return FB_ERR_UNSUPPORTED;
+    x.B = x.q.batch;
+    if (x.B * x.H * x.L != a.rows || x.o.batch != x.B || a.rows > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
+    if ((!x.k.batch_bcast && x.k.batch != x.B) || (!x.v.batch_bcast && x.v.batch != x.B)) return FB_ERR_UNSUPPORTED;
+    // rows of 16-byte vectors: bases, and strides of axes with more than one index
+    auto aligned = [](const void* p, uint64_t esz, const RowsLayout& l) {
+        const uint64_t v = 16 / esz;
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (l.rows <= 1 || l.s_row % v == 0) &&
+               (l.heads <= 1 || l.s_head % v == 0) && (l.batch <= 1 || l.s_batch % v == 0);
+    };
+    x.qp = static_cast<const uint16_t*>(a.q) + a.q_offset;
+    x.kp = static_cast<const uint16_t*>(a.k) + a.k_offset;
+    x.vp = static_cast<const uint16_t*>(a.v) + a.v_offset;
+    x.op = a.out_low ? static_cast<void*>(reinterpret_cast<uint16_t*>(a.out) + a.o_offset) : static_cast<void*>(a.out + a.o_offset);
+    if (!aligned(x.qp, 2, x.q) || !aligned(x.op, a.out_low ? 2 : 4, x.o)) return FB_ERR_UNSUPPORTED;
+    if (x.Lk > 0 && (!aligned(x.kp, 2, x.k) || !aligned(x.vp, 2, x.v))) return FB_ERR_UNSUPPORTED;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return a.depth == 64 ? launch_span<64>(s, x, st) : launch_span<128>(s, x, st);
+}
+
+}  // namespace fb

@@ -85,8 +85,10 @@ enum ScratchSlot : int {
     SCRATCH_ATTN_SPLIT = 5,   // split-key attention partials (f64 per row and key range)
     SCRATCH_ATTN_RESULT = 6,  // f32 attention result before low rounding
     SCRATCH_COLLECTIVE = 7,   // the global sum's f64 partial, all-reduced in place
-    SCRATCH_SPAN = 8,         // windowed / shared-prefix attention: key-range records and their counters
-    SCRATCH_SLOTS = 9,
+    SCRATCH_SPAN = 8,         // windowed / shared-prefix attention: records of key ranges
+    SCRATCH_SPAN_PART = 9,    // records of units that several CTAs share
+    SCRATCH_SPAN_COUNT = 10,  // their arrival counters, 0 between launches
+    SCRATCH_SLOTS = 11,
 };
 void* scratch(void* stream, uint64_t bytes, int slot);
 int sm_count();
@@ -110,6 +112,7 @@ int launch_status(const char* what);
 uint32_t read_reduce_status();
 uint32_t read_gemm_status();
 uint32_t read_attention_status();
+uint32_t read_span_status();
 
 // ---- reductions / statistics (reduce.cu) ----
 int launch_reduce_rows(uint32_t op, const Rows& in, const RowOut& out, void* stream);
@@ -249,6 +252,8 @@ struct SpanArgs {
 };
 // Any strides, depths and types (f32, f16, bf16); one block per query row.
 int launch_span_simt(const SpanArgs& a, void* stream);
+// 16-bit operands on the tensor cores; FB_ERR_UNSUPPORTED for other layouts.
+int launch_span_tc(const SpanArgs& a, void* stream);
 
 // ---- token log probabilities (token_logprobs.cu) ----
 struct TokenArgs {
