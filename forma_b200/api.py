@@ -107,6 +107,23 @@ def lib() -> C.CDLL:
     return _lib.load()
 
 
+_bind = None
+
+
+def bind():
+    """The torch binding of the serving operators (``_torch_bind.so``)."""
+    global _bind
+    if _bind is None:
+        lib()  # the library it links to
+        try:
+            from . import _torch_bind
+        except ImportError as e:
+            raise RuntimeError(f"the torch binding does not load ({e}): build it with `python -m forma_b200.build`") from e
+        _torch_bind.set_error(TensorError)
+        _bind = _torch_bind
+    return _bind
+
+
 def _check(status: int) -> None:
     if status != 0:
         raise TensorError(status, lib().fb_last_error().decode(errors="replace"))
@@ -396,17 +413,7 @@ def attention_window(query, key, value, window: int, sinks: int = 0, lengths: Op
     ``i + options.causal``, or at ``Lk - L + i`` when that is None.  The
     result has the operands' dtype (``out`` may be f32 instead); a query that
     sees no key gives zeros."""
-    dev = _device(query, key, value, lengths, out)
-    if out is None:
-        dims = attention_plan(list(query.shape), list(key.shape), list(value.shape), None, options)
-        out = torch.empty(dims, dtype=query.dtype, device=dev)
-    dq, dk, dv, do = describe(query), describe(key), describe(value), describe(out)
-    dl = describe(lengths) if lengths is not None else None
-    with _on(dev) as dev_:
-        _check(lib().fb_attention_window(C.byref(dq), C.byref(dk), C.byref(dv), C.byref(dl) if dl is not None else None,
-                                         _extent(window), _extent(sinks), _attn_options(options), C.byref(do),
-                                         _stream(dev_)))
-    return out
+    return bind().attention_window(query, key, value, window, sinks, lengths, options.scale, options.causal, out)
 
 
 def attention_prefix(query, prefix_key, prefix_value, key, value, lengths: Optional[torch.Tensor] = None,
@@ -415,24 +422,7 @@ def attention_prefix(query, prefix_key, prefix_value, key, value, lengths: Optio
     [Hkv, P, D], read once for the whole batch, over each sequence's own keys
     [B, Hkv, S, D] (causal, ``lengths`` of them filled, as in
     :func:`attention_window`)."""
-    dev = _device(query, prefix_key, prefix_value, key, value, lengths, out)
-    if out is None:
-        dims = attention_plan(list(query.shape), list(key.shape), list(value.shape), None, options)
-        out = torch.empty(dims, dtype=query.dtype, device=dev)
-    dq, dpk, dpv, dk, dv, do = (describe(t) for t in (query, prefix_key, prefix_value, key, value, out))
-    dl = describe(lengths) if lengths is not None else None
-    with _on(dev) as dev_:
-        _check(lib().fb_attention_prefix(C.byref(dq), C.byref(dpk), C.byref(dpv), C.byref(dk), C.byref(dv),
-                                         C.byref(dl) if dl is not None else None, _attn_options(options), C.byref(do),
-                                         _stream(dev_)))
-    return out
-
-
-def _extent(n: int) -> int:
-    """A count of keys for the C ABI: refuses what would wrap to a huge u64."""
-    if n < 0:
-        raise TensorError(10, "invalid attention: window and sinks count keys")
-    return min(int(n), 2**64 - 1)
+    return bind().attention_prefix(query, prefix_key, prefix_value, key, value, lengths, options.scale, options.causal, out)
 
 
 # ------------------------------------------------- token log probabilities
@@ -457,19 +447,7 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     (f32, f16 or bf16), the rows' entropies, and their ``top`` likeliest
     classes (argmax's order: IEEE total order, lowest index on ties), in one
     pass over the logits.  ``targets`` are int32 holding u32."""
-    dev = _device(logits, targets)
-    lead = list(logits.shape[:-1])
-    f32 = dict(dtype=torch.float32, device=dev)
-    r = TokenLogprobs(torch.empty(lead, **f32) if targets is not None else None, torch.empty(lead, **f32),
-                      torch.empty(lead, **f32))
-    if top:
-        r.top_logprob = torch.empty(lead + [top], **f32)
-        r.top_index = torch.empty(lead + [top], dtype=torch.int32, device=dev)
-    d = [describe(t) if t is not None else None
-         for t in (logits, targets, r.logprob, r.entropy, r.logsumexp, r.top_logprob, r.top_index)]
-    with _on(dev) as dev_:
-        _check(lib().fb_token_logprobs(*(C.byref(x) if x is not None else None for x in d), _stream(dev_)))
-    return r
+    return TokenLogprobs(*bind().token_logprobs(logits, targets, top))
 
 
 def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, logsumexp: torch.Tensor, grad_logprob: torch.Tensor,
@@ -479,14 +457,7 @@ def token_logprobs_grad(logits: torch.Tensor, targets: torch.Tensor, logsumexp: 
     the logits, from :func:`token_logprobs`' ``logsumexp`` and ``entropy``, in
     the logits' dtype.  ``out`` may be the logits themselves (in place) or an
     f32 tensor."""
-    dev = _device(logits, targets, logsumexp, grad_logprob, entropy, grad_entropy, out)
-    if out is None:
-        out = torch.empty(list(logits.shape), dtype=logits.dtype, device=dev)
-    d = [describe(t) if t is not None else None
-         for t in (logits, targets, logsumexp, grad_logprob, entropy, grad_entropy, out)]
-    with _on(dev) as dev_:
-        _check(lib().fb_token_logprobs_grad(*(C.byref(x) if x is not None else None for x in d), _stream(dev_)))
-    return out
+    return bind().token_logprobs_grad(logits, targets, logsumexp, grad_logprob, entropy, grad_entropy, out)
 
 
 # ------------------------------------------------------------- reductions

@@ -4,7 +4,8 @@ Every CUDA translation unit is compiled by nvcc for ``compute_100a/sm_100a``
 with precise f32 arithmetic (no fast-math, no flush-to-zero, IEEE divide and
 square root), the host C++ by nvcc's host compiler, and the CUDA runtime is
 linked statically so the library only needs the driver at run time.
-Objects are rebuilt only when a source or header is newer.
+Objects are rebuilt only when a source or header is newer.  The torch binding
+``_torch_bind.so`` (host C++) is built beside it.
 
 Usage: ``python -m forma_b200.build [--force] [-j N]``
 """
@@ -23,6 +24,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB = PKG / "libforma_b200.so"
+BIND = PKG / "_torch_bind.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -86,12 +88,37 @@ def build(force: bool = False, jobs: int | None = None) -> Path:
     return LIB
 
 
+def build_bind(force: bool = False) -> Path:
+    """The torch binding of the serving operators, linked to the library beside it."""
+    import sysconfig
+
+    import torch
+
+    src = PKG / "bind" / "torch_bind.cpp"
+    if force or _stale(BIND, [src, ROOT / "include" / "forma_b200.h"]):
+        root = Path(torch.__file__).resolve().parent
+        cuda = Path(NVCC).resolve().parent.parent
+        tmp = BIND.with_suffix(".so.tmp")
+        subprocess.run(
+            [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", str(src), "-o", str(tmp),
+             "-isystem", str(root / "include"), "-isystem", str(root / "include/torch/csrc/api/include"),
+             "-isystem", sysconfig.get_paths()["include"], "-isystem", str(cuda / "include"),
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             "-L", str(root / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+             "-L", str(PKG), "-l:" + LIB.name, "-Wl,-rpath,$ORIGIN"],
+            check=True,
+        )
+        os.replace(tmp, BIND)
+    return BIND
+
+
 def main(argv: list[str] | None = None) -> int:
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--force", action="store_true")
     ap.add_argument("-j", type=int, default=None)
     a = ap.parse_args(argv)
     print(build(a.force, a.j))
+    print(build_bind(a.force))
     return 0
 
 

@@ -194,6 +194,41 @@ __device__ __forceinline__ uint32_t packed_max(uint32_t a, uint32_t b, __half) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Per-row values with one stride (elements; 0 for a single value): the
+// streaming kernels index them without the nests' divisions.
+struct RowVec {
+    void* p = nullptr;
+    uint64_t stride = 0;
+    template <typename V>
+    __device__ __forceinline__ V& at(uint64_t row) const {
+        return static_cast<V*>(p)[row * stride];
+    }
+};
+bool row_vec(void* data, uint64_t offset, const Nest& n, RowVec* v) {
+    if (n.rank > 1) return false;
+    v->p = data ? static_cast<uint32_t*>(data) + offset : nullptr;
+    v->stride = n.rank ? n.strides[0] : 0;
+    return true;
+}
+bool row_vec(const RowOut& o, RowVec* v) { return row_vec(o.data, o.offset, o.nest, v); }
+
+struct StreamArgs {
+    const void* x;  // row 0
+    uint64_t rows, cols, row_stride;
+    RowVec targets, logprob, entropy, lse;
+    float* top_logprob;
+    uint32_t* top_index;
+    uint32_t top;
+    uint32_t parts, part_segs, mult;
+};
+struct GradArgs {
+    const void* x;
+    void* out;
+    uint64_t cols, x_stride, out_stride;
+    uint32_t chunks;
+    RowVec targets, lse, g_logprob, entropy, g_entropy;
+};
+
 // A 16-byte vector as words; how a type's words are widened and compared.
 template <typename T>
 struct Words {
@@ -291,7 +326,7 @@ __device__ __forceinline__ void join_sums(float& m, float& s0, float& s1, float 
 // `parts` CTAs (a cluster when > 1) per row, `part_segs` segments of 32 * VPL
 // vectors each; `mult` segments share a kept maximum.
 template <typename T, int VPL>
-__global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(TokenArgs a, uint32_t parts, uint32_t part_segs, uint32_t mult) {
+__global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
     using W = Words<T>;
     constexpr int NW = VPL * 4;
     __shared__ __align__(16) uint32_t tkey[BLOCK];
@@ -301,14 +336,14 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(TokenArgs a, uin
     __shared__ float wsum[3][WARPS];
     __shared__ uint32_t n_sel, n_cand, tau;
     __shared__ TokenPartial mine;
-    const Rows& in = a.logits;
+    const uint32_t parts = a.parts, mult = a.mult;
     const uint64_t row = blockIdx.x / parts;
     const uint32_t part = blockIdx.x % parts;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const T* x = static_cast<const T*>(in.data) + in.offset + row * in.row_stride;
-    const RowVectors<T> rv(x, in.cols);
+    const T* x = static_cast<const T*>(a.x) + row * a.row_stride;
+    const RowVectors<T> rv(x, a.cols);
     const uint32_t nseg = (uint32_t)((rv.vectors() + 32 * VPL - 1) / (32 * VPL));
-    const uint32_t seg0 = min(part * part_segs, nseg), seg1 = min(seg0 + part_segs, nseg);
+    const uint32_t seg0 = min(part * a.part_segs, nseg), seg1 = min(seg0 + a.part_segs, nseg);
     const uint32_t groups = (seg1 - seg0 + mult - 1) / mult;
     if (a.top) {
         for (uint32_t i = threadIdx.x; i < groups; i += BLOCK) seg_max[i] = 0u;
@@ -488,13 +523,13 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(TokenArgs a, uin
     // One row's results, in f64 from here.
     const double ls = S0 == 0.0f ? (double)row_nan() : log((double)S0), lse = (double)M + ls;
     if (threadIdx.x == 0) {
-        row_store(a.lse, row, (float)lse);
-        row_store(a.entropy, row, (float)(ls - (double)S1 / (double)S0 * 0.6931471805599453));
-        if (a.logprob.data) {
-            const uint32_t t = a.targets[a.target_offset + nest_offset(a.target_nest, row)];
+        if (a.lse.p) a.lse.at<float>(row) = (float)lse;
+        if (a.entropy.p) a.entropy.at<float>(row) = (float)(ls - (double)S1 / (double)S0 * 0.6931471805599453);
+        if (a.logprob.p) {
+            const uint32_t t = a.targets.at<uint32_t>(row);
             float r = 0.0f;
-            if (t != FB_NO_TOKEN) r = t < in.cols ? (float)((double)Elem<T>::load(x + t) - lse) : row_nan();
-            row_store(a.logprob, row, r);
+            if (t != FB_NO_TOKEN) r = t < a.cols ? (float)((double)Elem<T>::load(x + t) - lse) : row_nan();
+            a.logprob.at<float>(row) = r;
         }
     }
     if (threadIdx.x < a.top) {
@@ -532,7 +567,15 @@ int launch_stream(const TokenArgs& a, cudaStream_t st) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
-    (void)cudaLaunchKernelEx(&cfg, token_stream_kernel<T, VPL>, a, (uint32_t)parts, (uint32_t)part_segs, (uint32_t)mult);
+    StreamArgs k{};
+    k.x = static_cast<const T*>(in.data) + in.offset;
+    k.rows = in.rows, k.cols = in.cols, k.row_stride = in.row_stride;
+    if (!row_vec(const_cast<uint32_t*>(a.targets), a.target_offset, a.target_nest, &k.targets) || !row_vec(a.logprob, &k.logprob) ||
+        !row_vec(a.entropy, &k.entropy) || !row_vec(a.lse, &k.lse))
+        return FB_ERR_UNSUPPORTED;
+    k.top_logprob = a.top_logprob, k.top_index = a.top_index, k.top = a.top;
+    k.parts = (uint32_t)parts, k.part_segs = (uint32_t)part_segs, k.mult = (uint32_t)mult;
+    (void)cudaLaunchKernelEx(&cfg, token_stream_kernel<T, VPL>, k);
     count_launch("token_stream_kernel");
     return launch_status("kernel launch");
 }
@@ -561,28 +604,27 @@ int launch_t(const TokenArgs& a, cudaStream_t st) {
 // Bound: HBM, one read and one write.  Loads are issued before the row's
 // scalars arrive; each block does one chunk of 4 vectors per thread.
 template <typename T>
-__global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(TokenGradArgs a, uint32_t chunks) {
+__global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(GradArgs a) {
     using W = Words<T>;
     using U = typename Bits<T>::U;
     constexpr int E = W::E, N = 4;
-    const Rows& in = a.logits;
-    const uint64_t row = blockIdx.x / chunks;
-    const uint64_t j0 = (uint64_t)(blockIdx.x % chunks) * (N * BLOCK) + threadIdx.x;
-    const T* x = static_cast<const T*>(in.data) + in.offset + row * in.row_stride;
-    U* out = reinterpret_cast<U*>(a.out.data) + a.out.offset + row * a.out.row_stride;
-    const RowVectors<T> rv(x, in.cols);
+    const uint64_t row = blockIdx.x / a.chunks;
+    const uint64_t j0 = (uint64_t)(blockIdx.x % a.chunks) * (N * BLOCK) + threadIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    U* out = static_cast<U*>(a.out) + row * a.out_stride;
+    const RowVectors<T> rv(x, a.cols);
     uint32_t w[N][4];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const uint4 v = rv.template load<false>(j0 + i * BLOCK);
         w[i][0] = v.x, w[i][1] = v.y, w[i][2] = v.z, w[i][3] = v.w;
     }
-    const uint32_t t = a.targets[a.target_offset + nest_offset(a.target_nest, row)];
-    const float gl = t < in.cols ? row_value(a.g_logprob, row) : 0.0f;
-    const float gh = a.g_entropy.data ? row_value(a.g_entropy, row) : 0.0f;
+    const uint32_t t = a.targets.at<const uint32_t>(row);
+    const float lse = a.lse.at<const float>(row);
+    const float gl = t < a.cols ? a.g_logprob.at<const float>(row) : 0.0f;
+    const float gh = a.g_entropy.p ? a.g_entropy.at<const float>(row) : 0.0f;
+    const float h = gh != 0.0f ? a.entropy.at<const float>(row) : 0.0f;
     const bool zero = gl == 0.0f && gh == 0.0f;
-    const float lse = row_value(a.lse, row);
-    const float h = gh != 0.0f ? row_value(a.entropy, row) : 0.0f;
     const float A = -fmaf(gh, h, gl), B = -gh * 0.6931471805599453f;
     const uint64_t at = (uint64_t)t + rv.head;  // the target's place among the vectors' elements
 #pragma unroll
@@ -635,8 +677,15 @@ int launch_grad_t(const TokenGradArgs& a, cudaStream_t st) {
     if (in.contiguous_rows && a.out.contiguous_rows && a.out.dtype == dtype && (x0 - o0) % 16 == 0 &&
         (in.row_stride - a.out.row_stride) * esz % 16 == 0) {
         const uint64_t vectors = (in.cols + 2 * Words<T>::E - 2) / Words<T>::E, chunks = (vectors + 4 * BLOCK - 1) / (4 * BLOCK);
-        if (in.rows * chunks <= 0x7fffffffull) {
-            token_grad_stream_kernel<T><<<(unsigned)(in.rows * chunks), BLOCK, 0, st>>>(a, (uint32_t)chunks);
+        GradArgs k{};
+        const bool strided = row_vec(const_cast<uint32_t*>(a.targets), a.target_offset, a.target_nest, &k.targets) &&
+                             row_vec(a.lse, &k.lse) && row_vec(a.g_logprob, &k.g_logprob) && row_vec(a.entropy, &k.entropy) &&
+                             row_vec(a.g_entropy, &k.g_entropy);
+        if (strided && in.rows * chunks <= 0x7fffffffull) {
+            k.x = reinterpret_cast<const void*>(x0), k.out = reinterpret_cast<void*>(o0);
+            k.cols = in.cols, k.x_stride = in.row_stride, k.out_stride = a.out.row_stride;
+            k.chunks = (uint32_t)chunks;
+            token_grad_stream_kernel<T><<<(unsigned)(in.rows * chunks), BLOCK, 0, st>>>(k);
             count_launch("token_grad_stream_kernel");
             return launch_status("kernel launch");
         }
