@@ -157,11 +157,11 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
 // entropy and log probability exactly 0, and no m overflows.  Only a
 // segment's maximum (packed 16-bit maxima, one redux) is compared with m, so
 // rescales by 2^((m - m') log2 e) are rare.  d is clamped at -200 (2^-200
-// flushes to 0), which keeps a masked class's 0 * -inf out of S1; the
-// NaN-propagating clamp keeps a NaN in it.
+// flushes to 0) where that matters, which keeps a masked class's 0 * -inf out
+// of S1; the NaN-propagating clamp keeps a NaN in it.
 //
-// Alternatives.  The k-th largest of the 256 threads' maxima is a lower bound
-// t of the row's k-th largest value, and the maxima of the row's segments
+// Alternatives.  The k-th largest of the 256 threads' maxima (to 16 bits, by a
+// binary search in one warp) is a lower bound t of the row's k-th largest value, and the maxima of the row's segments
 // (kept in shared memory) say where values >= t lie: about k segments are
 // read again (L2), the values >= t collected with their indices and put in
 // order by counting.  More than CAND of them (a row of few distinct values),
@@ -350,7 +350,20 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         if (threadIdx.x == 0) n_sel = n_cand = 0u;
         __syncthreads();
     }
+    // segments [in0, in1) lie inside the row: no vector of theirs is partial
+    const uint32_t per_seg = 32 * VPL * W::E;
+    const uint32_t in0 = rv.head ? 1u : 0u, in1 = (uint32_t)(rv.end / per_seg);
+    const uint4* xv = reinterpret_cast<const uint4*>(rv.x - rv.head) + lane;  // vector `lane` of segment 0
     auto load_seg = [&](uint32_t seg, uint32_t (&w)[NW]) {
+        if (seg >= in0 && seg < in1) {
+            const uint4* p = xv + (uint64_t)seg * (32 * VPL);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const uint4 v = __ldg(p + i * 32);
+                w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const uint4 v = rv.template load<true>((uint64_t)seg * (32 * VPL) + i * 32 + lane);
@@ -358,11 +371,13 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         }
     };
     float m = 0.0f;  // the reference: 0 while nothing but -inf was seen
-    float2 s0[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)}, s1[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
     uint32_t run = 0u, own_max = W::LOWEST;
+    uint32_t w[NW];
+    if (seg0 + warp < seg1) load_seg(seg0 + warp, w);
     for (uint32_t seg = seg0 + warp; seg < seg1; seg += WARPS) {
-        uint32_t w[NW];
-        load_seg(seg, w);
+        uint32_t next[NW];  // the next segment's loads are in flight while this one is summed
+        if (seg + WARPS < seg1) load_seg(seg + WARPS, next);
         uint32_t mx = w[0];
 #pragma unroll
         for (int i = 1; i < NW; ++i) mx = W::maximum(mx, w[i]);
@@ -374,53 +389,85 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
             const float v = Bits<T>::value(Bits<T>::pattern(top));
             const float m2 = v == -__int_as_float(0x7f800000) ? 0.0f : v;
             const float dm = below(m, m2), f = ex2_approx(dm);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float t0 = s0[h].x + s0[h].y, t1 = s1[h].x + s1[h].y;
-                s0[h] = make_float2(t0 == 0.0f ? 0.0f : t0 * f, 0.0f);
-                s1[h] = make_float2(t0 == 0.0f ? 0.0f : fmaf(dm, t0, t1) * f, 0.0f);
-            }
+            const float t0 = s0.x + s0.y, t1 = s1.x + s1.y;
+            s0 = make_float2(t0 == 0.0f ? 0.0f : t0 * f, 0.0f);
+            s1 = make_float2(t0 == 0.0f ? 0.0f : fmaf(dm, t0, t1) * f, 0.0f);
             m = m2;
         }
-        const float2 l2 = make_float2(L2E, L2E), nm = make_float2(-m, -m);
-        constexpr int PAIRS = W::E == 8 ? NW : NW / 2;
+        // Without the clamp a class at -inf (or further below than the floats
+        // reach) makes the segment's S1 NaN: only then is it taken again with it.
+        float2 a0, a1;
+        auto sum = [&](auto clamp) {
+            const float2 l2 = make_float2(L2E, L2E), nm = make_float2(-m, -m);
+            constexpr int PAIRS = W::E == 8 ? NW : NW / 2;
+            a0 = a1 = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-            float2 v;
-            if constexpr (W::E == 8) v = W::widen(w[i]);
-            else v = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-            float2 d = __fmul2_rn(__fadd2_rn(v, nm), l2);
-            d.x = max_nan(d.x, -200.0f), d.y = max_nan(d.y, -200.0f);
-            const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
-            s0[i & 1] = __fadd2_rn(s0[i & 1], e);
-            s1[i & 1] = __ffma2_rn(e, d, s1[i & 1]);
-        }
+            for (int i = 0; i < PAIRS; ++i) {
+                float2 v;
+                if constexpr (W::E == 8) v = W::widen(w[i]);
+                else v = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+                float2 d = __fmul2_rn(__fadd2_rn(v, nm), l2);
+                if (clamp) d.x = max_nan(d.x, -200.0f), d.y = max_nan(d.y, -200.0f);
+                const float2 e = make_float2(ex2_approx(d.x), ex2_approx(d.y));
+                a0 = __fadd2_rn(a0, e);
+                a1 = __ffma2_rn(e, d, a1);
+            }
+        };
+        sum(std::false_type());
+        const float t1 = a1.x + a1.y;
+        if (__any_sync(0xffffffffu, t1 != t1)) sum(std::true_type());
+        s0 = __fadd2_rn(s0, a0);
+        s1 = __fadd2_rn(s1, a1);
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = next[i];
     }
     {
-        const float t0 = warp_sum_f((s0[0].x + s0[0].y) + (s0[1].x + s0[1].y));
-        const float t1 = warp_sum_f((s1[0].x + s1[0].y) + (s1[1].x + s1[1].y));
+        const float t0 = warp_sum_f(s0.x + s0.y), t1 = warp_sum_f(s1.x + s1.y);
         if (lane == 0) wsum[0][warp] = m, wsum[1][warp] = t0, wsum[2][warp] = t1;
         if (a.top) tkey[threadIdx.x] = Bits<T>::key(W::top(own_max));
     }
     __syncthreads();
-    float M = wsum[0][0], S0 = wsum[1][0], S1 = wsum[2][0];
+    // The warps' sums, joined by each warp's first lanes.
+    float M, S0, S1;
+    {
+        const int i = lane & (WARPS - 1);
+        const float mi = wsum[0][i], t0 = wsum[1][i], t1 = wsum[2][i];
+        M = t0 == 0.0f ? -__int_as_float(0x7f800000) : mi;
 #pragma unroll
-    for (int w = 1; w < WARPS; ++w) join_sums(M, S0, S1, wsum[0][w], wsum[1][w], wsum[2][w]);
+        for (int o = 1; o < WARPS; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        const float d = t0 == 0.0f ? 0.0f : below(mi, M), f = ex2_approx(d);
+        S0 = t0 * f;
+        S1 = t0 == 0.0f ? 0.0f : fmaf(d, t0, t1) * f;
+#pragma unroll
+        for (int o = 1; o < WARPS; o <<= 1) {
+            S0 += __shfl_xor_sync(0xffffffffu, S0, o);
+            S1 += __shfl_xor_sync(0xffffffffu, S1, o);
+        }
+    }
 
     if (a.top) {
         const uint32_t k = a.top;
         if (threadIdx.x < FB_MAX_TOP) mine.top[threadIdx.x] = 0ull;
-        {
-            const uint32_t key = tkey[threadIdx.x];
-            uint32_t rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < BLOCK; j += 4) {
-                const uint4 o = *reinterpret_cast<const uint4*>(&tkey[j]);
-                rank += (o.x > key) + (o.y > key) + (o.z > key) + (o.w > key);
-                rank += (o.x == key && j < (int)threadIdx.x) + (o.y == key && j + 1 < (int)threadIdx.x) +
-                        (o.z == key && j + 2 < (int)threadIdx.x) + (o.w == key && j + 3 < (int)threadIdx.x);
+        if (warp == 0) {
+            // the k-th largest of the threads' maxima, its upper 16 bits: the
+            // largest value that at least k of them reach, bit by bit
+            uint32_t mine[8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4 v = *reinterpret_cast<const uint4*>(&tkey[lane * 8 + i * 4]);
+                mine[4 * i] = v.x, mine[4 * i + 1] = v.y, mine[4 * i + 2] = v.z, mine[4 * i + 3] = v.w;
             }
-            if (rank == k - 1) tau = key;
+            constexpr int SHIFT = W::E == 8 ? 0 : 16;
+            uint32_t best = 0;
+#pragma unroll 1
+            for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+                const uint32_t want = (best | bit) << SHIFT;
+                uint32_t n = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) n += mine[i] >= want;
+                if (__reduce_add_sync(0xffffffffu, n) >= k) best |= bit;
+            }
+            if (lane == 0) tau = best << SHIFT;
         }
         __syncthreads();
         const uint32_t t = tau;
@@ -520,6 +567,7 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
             return;
         }
     }
+    if (threadIdx.x >= FB_MAX_TOP) return;
     // One row's results, in f64 from here.
     const double ls = S0 == 0.0f ? (double)row_nan() : log((double)S0), lse = (double)M + ls;
     if (threadIdx.x == 0) {
@@ -545,12 +593,12 @@ int launch_stream(const TokenArgs& a, cudaStream_t st) {
     const Rows& in = a.logits;
     const uint64_t E = Words<T>::E, seg = 32 * VPL;
     const uint64_t nseg = ((in.cols + 2 * E - 2) / E + seg - 1) / seg;  // at the worst alignment
-    // Parts per row: powers of two up to a cluster of eight, while the grid is
+    // Parts per row: powers of two up to a cluster of four, while the grid is
     // under eight CTAs per SM and a part keeps two segments per warp, or under
     // one per SM and it keeps half a segment per warp.
     uint64_t parts = 1;
     const uint64_t sms = (uint64_t)sm_count();
-    while (parts < 8 && ((in.rows * parts * 2 <= sms * 8 && nseg >= parts * 2 * 2 * WARPS) ||
+    while (parts < 4 && ((in.rows * parts * 2 <= sms * 8 && nseg >= parts * 2 * 2 * WARPS) ||
                          (in.rows * parts * 2 <= sms && nseg >= parts * WARPS)))
         parts *= 2;
     const uint64_t part_segs = (nseg + parts - 1) / parts;
