@@ -358,26 +358,28 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         const int quarter = warp & 3;
         const uint32_t row = (uint32_t)(quarter * 32 + lane);
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t head = head0 + row % p.GB, l = (t ? l0[1] : l0[0]) + row / p.GB % p.LB,
-                       b = (t ? b0[1] : b0[0]) + row / (p.GB * p.LB);
-        const bool valid = (t ? real[1] : real[0]) && row < p.rows && l < p.L && b < p.B;
         const uint32_t n = t ? n_t[1] : n_t[0], n_other = t ? n_t[0] : n_t[1];
         const float NEG = -__int_as_float(0x7f800000);
         const float sl = p.scale_log2;
+        // What a hidden key's raw score becomes: its logit is -inf whatever the scale's sign.
+        const float hidden = sl < 0.0f ? __int_as_float(0x7f800000) : NEG;
         // keys of this row: [0, sinks) and [low, high]
-        const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1 : base + (int64_t)l;
-        const int32_t high = (int32_t)max((int64_t)-1, min(pos, filled - 1));
-        const int32_t low = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
+        int32_t high, low;
+        {
+            const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1 : base + (int64_t)((t ? l0[1] : l0[0]) + row / p.GB % p.LB);
+            high = (int32_t)max((int64_t)-1, min(pos, filled - 1));
+            low = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
+        }
         const int32_t sinks = (int32_t)min((int64_t)0x7fffffff, p.sinks);
-        const uint32_t ns = t ? plan.ns[1] : plan.ns[0], a0 = t ? plan.a0[1] : plan.a0[0], e0 = t ? plan.e[1] : plan.e[0];
+        // this tile's key tiles: [0, ns) and then from a0 on, n in all from kt
+        const uint32_t ns = t ? plan.ns[1] : plan.ns[0], a0 = t ? plan.a0[1] : plan.a0[0];
+        uint32_t kt = n ? key_tile(t ? next_seen(1, 0) : next_seen(0, 0)) : 0;
         float m_used = NEG;  // running max (log2 units)
         float lsum = 0.0f;
         bool ok = true;
-        uint32_t j = 0;
-        for (uint32_t i = 0; i < n && ok; ++i, ++j) {
-            uint32_t kt = key_tile(j);
-            while (kt >= ns && (kt < a0 || kt >= e0)) kt = key_tile(++j);  // n counts what follows: it ends
+        for (uint32_t i = 0; i < n && ok; ++i) {
             const int32_t key0 = (int32_t)(kt * TK);
+            kt = kt + 1 < ns ? kt + 1 : max(kt + 1, a0);
             // Wait outcomes are made warp-uniform: tcgen05.ld/st are .sync.aligned.
             if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], i & 1))) {
                 ok = false;
@@ -394,14 +396,35 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
 #pragma unroll
                 for (int e = 0; e < TK; ++e) x[e] = __uint_as_float(r[e]);
             }
-            const bool edge = key0 + TK - 1 > high || (key0 < low && key0 + TK > sinks);
-            if (edge || sl == 0.0f) {
-                const int32_t lim = high + 1 - key0, lo = low - key0, sk = sinks - key0;
+            // Hidden keys are masked in the raw scores, only in the tiles that
+            // hold some: past the row's position or the filled keys, or between
+            // the first keys and the window.
+            if (key0 + TK - 1 > high || (key0 < low && key0 + TK > sinks)) {
+                int32_t lim = high + 1 - key0, lo = low - key0;
+                const int32_t sk = sinks - key0;
+                if (lo > 0 && sk > 0) {
+                    if (lo >= TK) {
+                        lim = min(lim, sk), lo = 0;  // first keys only
+                    } else {  // first keys and the window in one tile
 #pragma unroll
-                for (int e = 0; e < TK; ++e) x[e] = e < lim && (e >= lo || e < sk) ? x[e] * sl : NEG;  // logits, masked
+                        for (int e = 0; e < TK; ++e) x[e] = e < sk || e >= lo ? x[e] : hidden;
+                        lo = 0;
+                    }
+                }
+                if (lo > 0) {
+#pragma unroll
+                    for (int e = 0; e < TK; ++e) x[e] = e >= lo ? x[e] : hidden;
+                }
+                if (lim < TK) {
+#pragma unroll
+                    for (int e = 0; e < TK; ++e) x[e] = e < lim ? x[e] : hidden;
+                }
             }
-            const bool raw = !(edge || sl == 0.0f);
-            const bool use_min = raw && sl < 0.0f;
+            if (sl == 0.0f) {  // logits 0, hidden keys stay -inf
+#pragma unroll
+                for (int e = 0; e < TK; ++e) x[e] = x[e] == NEG ? NEG : 0.0f * x[e];
+            }
+            const bool use_min = sl < 0.0f;
             // Four chains of three-input extremes: 64 instructions per row.
             float mx[4] = {x[0], x[1], x[2], x[3]};
             if (use_min) {
@@ -421,7 +444,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             }
             float mt = use_min ? min3n(min3n(mx[0], mx[1], mx[2]), mx[3], mx[3])
                                : max3n(max3n(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-            if (raw) mt *= sl;  // raw extreme -> logit maximum
+            if (sl != 0.0f) mt *= sl;  // raw extreme -> logit maximum
             float alpha = 1.0f;
             bool rescale = false;
             if (mt > m_used + 8.0f) {
@@ -434,7 +457,8 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             // Packed pairs overwrite the scores they came from, so P needs no
             // registers of its own; one pair in eight takes the polynomial.
             uint32_t* xb = reinterpret_cast<uint32_t*>(x);
-            const float2 sl2 = make_float2(raw ? sl : 1.0f, raw ? sl : 1.0f), nb2 = make_float2(-ref, -ref);
+            const float mul = sl == 0.0f ? 1.0f : sl;
+            const float2 sl2 = make_float2(mul, mul), nb2 = make_float2(-ref, -ref);
 #pragma unroll
             for (int c = 0; c < TK / 32; ++c) {
 #pragma unroll
@@ -531,6 +555,12 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             tc_fence_after();
             const bool load = ok && n > 0;
             float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
+            // (worked out here again: kept through the loop they would spill)
+            uint32_t r0 = row;
+            asm volatile("" : "+r"(r0));
+            const uint32_t head = head0 + r0 % p.GB, l = (t ? l0[1] : l0[0]) + r0 / p.GB % p.LB,
+                           b = (t ? b0[1] : b0[0]) + r0 / (p.GB * p.LB);
+            const bool valid = (t ? real[1] : real[0]) && r0 < p.rows && l < p.L && b < p.B;
             float* rec = nullptr;
             if (p.part) {
                 inv = 1.0f;
