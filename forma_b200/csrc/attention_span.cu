@@ -46,9 +46,12 @@ constexpr int REC = D + 4;
 // A tile is up to 128 query rows that share a key/value head: GB query heads
 // x LB consecutive queries x NB sequences, gathered by one 4-D TMA box over
 // {depth, heads, queries, batch}, so that grouped heads share the key tiles
-// whatever Q's strides are.  A CTA owns two tiles and walks the key tiles
-// that either sees, in order: those of the first keys, then those of the two
-// windows.  A tile of rows takes part only in the key tiles that it sees.
+// whatever Q's strides are.  A work item is two tiles and the key tiles that
+// either sees, in order: those of the first keys, then those of the two
+// windows; a tile of rows takes part only in the key tiles that it sees.
+// CTAs are persistent, one per SM: the next item's loads start while this
+// one's last products and epilogue run (an item's own start and end cost
+// 12 us when each was a CTA, eight key tiles' time).
 //   warp 0      TMA: both Q tiles, then K and V tiles of 128 keys through
 //               rings of 2 (D = 128) or 4 (D = 64) slots
 //   warp 1      TMEM and MMA issue: S_t = Q_t K^T, O_t += P_t V, the two
@@ -56,7 +59,9 @@ constexpr int REC = D + 4;
 //               softmax; value rows past the filled keys are zeroed in shared
 //               memory first (a weight of 0 does not hide a NaN there)
 //   warps 2-9   softmax, one query row per thread: lazy running maximum
-//               (raised, and O rescaled, only past 2^8), P over S in TMEM
+//               (raised, and O rescaled, only past 2^8), P over S in TMEM; at
+//               an item's end O / l, or a record, straight from registers, a
+//               row's 32 bytes per store
 // This is attn_fwd_kernel's pipeline; see there for the orderings, the
 // 2^-shift pre-scale of BF16 weights and the bounded waits.
 struct SpanTileParams {
@@ -65,7 +70,7 @@ struct SpanTileParams {
     uint32_t group;                // query heads per key/value head
     uint32_t GB, LB, NB, rows;     // the tile's box and its row count GB * LB * NB
     uint32_t l_tiles, tiles;       // tiles along the queries; tiles of one unit
-    uint32_t pairs, units;         // pairs of tiles per unit; units = (batch x) head blocks
+    uint32_t groups, items;        // pairs of tiles per unit; units x groups x splits
     uint32_t head_blocks;          // H / GB
     uint32_t shared_keys;          // 1: every row sees all Lk keys of batch 0 (the shared prefix)
     uint32_t k_batch_bcast, v_batch_bcast;
@@ -73,11 +78,13 @@ struct SpanTileParams {
     uint64_t length_stride;
     int64_t offset, window, sinks;
     float scale_log2, shift;
-    uint32_t splits;               // CTAs along the key tiles of a pair
+    float hidden;                  // what a hidden key's raw score becomes: its logit is -inf whatever the scale's sign
+    int32_t sinks32;               // sinks, at most 2^31 - 1
+    uint32_t splits;               // key ranges of a pair
     float* part;                   // records: ((b * H + h) * L + l) * part_stride + part_first + split
     uint32_t part_stride, part_first;
     void* out;                     // part == null: output rows
-    uint32_t out_low, tma_out;
+    uint32_t out_low, wide;        // wide: rows of whole, aligned 32-byte runs
     uint64_t o_sb, o_sh, o_sl;
 };
 
@@ -89,7 +96,7 @@ struct TCfg {
     static constexpr int K_BYTES = TK * D * 2;
     static constexpr int STAGE_BYTES = 2 * K_BYTES;
     static constexpr int STAGES = D == 64 ? 4 : 2;
-    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + 256;
+    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + 384;
     static __device__ __forceinline__ uint32_t s_col(int t) { return (uint32_t)(t * TK); }
     static __device__ __forceinline__ uint32_t o_col(int t) { return (uint32_t)(2 * TK + t * 128); }
 };
@@ -113,109 +120,109 @@ struct TilePlan {
     }
 };
 
-template <int D>
-__global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
-                                                                       const __grid_constant__ CUtensorMap tmK,
-                                                                       const __grid_constant__ CUtensorMap tmV,
-                                                                       const __grid_constant__ CUtensorMap tmO, SpanTileParams p) {
-    using C = TCfg<D>;
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    unsigned char* sQ = smem;
-    unsigned char* sKV = sQ + 2 * C::Q_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::STAGES * C::STAGE_BYTES);
-    uint64_t* q_full = bars;
-    uint64_t* k_full = bars + 1;
-    uint64_t* k_empty = k_full + C::STAGES;
-    uint64_t* v_full = k_empty + C::STAGES;
-    uint64_t* v_empty = v_full + C::STAGES;
-    uint64_t* s_full = v_empty + C::STAGES;
-    uint64_t* p_full = s_full + 2;
-    uint64_t* o_done = p_full + 2;
-    uint64_t* drain = o_done + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-
-    // The launch that follows may start while this one ends (where it was made
-    // so); it waits for this grid's results itself.
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // Pairs of one unit in consecutive CTAs, last queries first.
-    const uint32_t split = blockIdx.x % p.splits;
-    const uint32_t pair = p.pairs - 1 - (blockIdx.x / p.splits) % p.pairs;
-    const uint32_t unit = blockIdx.x / (p.splits * p.pairs);
-    const uint32_t hb = unit % p.head_blocks;
-    const uint32_t head0 = hb * p.GB, kv_head = head0 / p.group;
-    const uint32_t unit_b = unit / p.head_blocks;  // 0 with shared keys
-    int64_t filled = p.Lk, base = p.offset;
-    if (p.lengths) {
-        filled = min(filled, (int64_t)p.lengths[unit_b * p.length_stride]);
-        base = filled - (int64_t)p.L;
-    }
-    // tile t of the pair: first sequence and first query
-    uint32_t b0[2], l0[2];
+// One work item: up to two tiles of a unit and one key range.  The producer
+// works it out and leaves it in shared memory, PLANS items ahead at most.
+constexpr int PLANS = 4;
+struct TileItem {
+    uint32_t split, head0, kv_head, unit_b;
+    uint32_t b0[2], l0[2], n_t[2];  // first sequence, first query, key tiles of each tile
     bool real[2];
+    uint32_t j0, n_kv;              // this range of the joint list
+    int64_t filled, base;
     TilePlan plan;
-    Reach rc[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const uint32_t tile = pair * 2 + t;
-        real[t] = tile < p.tiles;
-        b0[t] = p.shared_keys ? tile / p.l_tiles * p.NB : unit_b;
-        l0[t] = (p.shared_keys ? tile % p.l_tiles : tile) * p.LB;
-        plan.ns[t] = plan.a0[t] = plan.e[t] = 0;
-        rc[t] = Reach{0, 0, -1};
-        if (!real[t]) continue;
-        if (p.shared_keys) {
-            rc[t] = Reach{0, 0, (int64_t)p.Lk - 1};
-        } else {
-            rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
-        }
-        if (rc[t].hi < 0) continue;
-        plan.ns[t] = (uint32_t)((rc[t].first + TK - 1) / TK);
-        if (rc[t].lo <= rc[t].hi) {
-            plan.a0[t] = max((uint32_t)(rc[t].lo / TK), plan.ns[t]);
-            plan.e[t] = max((uint32_t)(rc[t].hi / TK) + 1, plan.a0[t]);
-        }
+    __device__ __forceinline__ uint32_t key_tile(uint32_t j) const { return plan.tile(j0 + j); }
+    // next joint index >= j of this range that tile t sees (n_kv if none)
+    __device__ __forceinline__ uint32_t next_seen(int t, uint32_t j) const {
+        while (j < n_kv && !plan.sees(t, key_tile(j))) ++j;
+        return j;
     }
-    plan.s = max(plan.ns[0], plan.ns[1]);
-    {
+    __device__ __forceinline__ void set(const SpanTileParams& p, uint32_t item) {
+        // Last queries (the most keys under a long window) of every unit first.
+        const uint32_t units = p.items / (p.groups * p.splits);
+        split = item % p.splits;
+        const uint32_t group = p.groups - 1 - item / p.splits / units;
+        const uint32_t unit = item / p.splits % units;
+        head0 = unit % p.head_blocks * p.GB, kv_head = head0 / p.group;
+        unit_b = unit / p.head_blocks;  // 0 with shared keys
+        filled = p.Lk, base = p.offset;
+        if (p.lengths) {
+            filled = min(filled, (int64_t)p.lengths[unit_b * p.length_stride]);
+            base = filled - (int64_t)p.L;
+        }
+        Reach rc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t tile = group * 2 + t;
+            real[t] = tile < p.tiles;
+            b0[t] = p.shared_keys ? tile / p.l_tiles * p.NB : unit_b;
+            l0[t] = (p.shared_keys ? tile % p.l_tiles : tile) * p.LB;
+            plan.ns[t] = plan.a0[t] = plan.e[t] = 0;
+            rc[t] = Reach{0, 0, -1};
+            if (!real[t]) continue;
+            if (p.shared_keys) rc[t] = Reach{0, 0, (int64_t)p.Lk - 1};
+            else rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
+            if (rc[t].hi < 0) continue;
+            plan.ns[t] = (uint32_t)((rc[t].first + TK - 1) / TK);
+            if (rc[t].lo <= rc[t].hi) {
+                plan.a0[t] = max((uint32_t)(rc[t].lo / TK), plan.ns[t]);
+                plan.e[t] = max((uint32_t)(rc[t].hi / TK) + 1, plan.a0[t]);
+            }
+        }
+        plan.s = max(plan.ns[0], plan.ns[1]);
         uint32_t a = 0xffffffffu, e = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
             if (plan.e[t] > plan.a0[t]) a = min(a, plan.a0[t]), e = max(e, plan.e[t]);
         plan.a = e ? max(a, plan.s) : plan.s;
         plan.n = plan.s + (e > plan.a ? e - plan.a : 0);
+        const uint32_t per = (plan.n + p.splits - 1) / p.splits;
+        j0 = min(split * per, plan.n);
+        const uint32_t j1 = min(j0 + per, plan.n);
+        n_kv = j1 - j0;
+        n_t[0] = plan.count(0, j0, j1), n_t[1] = plan.count(1, j0, j1);
     }
-    // this CTA's share of the joint list
-    const uint32_t per = (plan.n + p.splits - 1) / p.splits;
-    const uint32_t j0 = min(split * per, plan.n), j1 = min(j0 + per, plan.n);
-    const uint32_t n_kv = j1 - j0;
-    const uint32_t n_t[2] = {plan.count(0, j0, j1), plan.count(1, j0, j1)};
-    auto key_tile = [&](uint32_t j) { return plan.tile(j0 + j); };
-    // next local joint index >= j that tile t sees (n_kv if none)
-    auto next_seen = [&](int t, uint32_t j) {
-        while (j < n_kv && !plan.sees(t, key_tile(j))) ++j;
-        return j;
-    };
-    const int32_t k_b = p.shared_keys || p.k_batch_bcast ? 0 : (int32_t)unit_b;
-    const int32_t v_b = p.shared_keys || p.v_batch_bcast ? 0 : (int32_t)unit_b;
-    auto load_k = [&](uint32_t j) {
-        const uint32_t s = j % C::STAGES;
-        mbar_arrive_expect_tx(&k_full[s], C::K_BYTES);
-        for (int b = 0; b < C::BOXES; ++b)
-            tma_load_4d(sKV + s * C::STAGE_BYTES + b * (TK * 128), &tmK, b * 64, (int32_t)(key_tile(j) * TK),
-                        (int32_t)kv_head, k_b, &k_full[s]);
-    };
-    auto load_v = [&](uint32_t j) {
-        const uint32_t s = j % C::STAGES;
-        mbar_arrive_expect_tx(&v_full[s], C::K_BYTES);
-        for (int b = 0; b < C::BOXES; ++b)
-            tma_load_4d(sKV + s * C::STAGE_BYTES + C::K_BYTES + b * (TK * 128), &tmV, b * 64, (int32_t)(key_tile(j) * TK),
-                        (int32_t)kv_head, v_b, &v_full[s]);
-    };
+};
 
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+template <int D>
+__global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
+                                                                       const __grid_constant__ CUtensorMap tmK,
+                                                                       const __grid_constant__ CUtensorMap tmV, SpanTileParams p) {
+    using C = TCfg<D>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    unsigned char* sQ = smem;
+    unsigned char* sKV = sQ + 2 * C::Q_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::STAGES * C::STAGE_BYTES);
+    uint64_t* k_full = bars;
+    uint64_t* k_empty = k_full + C::STAGES;
+    uint64_t* v_full = k_empty + C::STAGES;
+    uint64_t* v_empty = v_full + C::STAGES;
+    uint64_t* q_full = v_empty + C::STAGES;   // [2]
+    uint64_t* q_empty = q_full + 2;
+    uint64_t* s_full = q_empty + 2;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_done = p_full + 2;
+    uint64_t* o_free = o_done + 2;            // O read out of TMEM
+    uint64_t* plan_full = o_free + 2;         // [PLANS]
+    uint64_t* plan_empty = plan_full + PLANS;
+    uint64_t* drain = plan_empty + PLANS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+    __shared__ TileItem plans[PLANS];
+    // Item i of this CTA: rounds over the grid run back and forth, so that no
+    // CTA gets the longest item of every round.
+    auto item_at = [&](uint32_t i) { return i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); };
+
+    // The launch that follows may start while this one ends (where it was made
+    // so); it waits for this grid's results itself.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1);
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
@@ -223,25 +230,19 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             mbar_init(&v_empty[s], 1);
         }
         for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 1);
+            mbar_init(&q_empty[t], 1);
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 128);
             mbar_init(&o_done[t], 1);
+            mbar_init(&o_free[t], 128);
+        }
+        for (int i = 0; i < PLANS; ++i) {
+            mbar_init(&plan_full[i], 1);
+            mbar_init(&plan_empty[i], 9);  // the issuing warp and the softmax warps
         }
         mbar_init(drain, 1);
         fence_barrier_init();
-        if (n_kv > 0) {
-            const uint32_t tiles = (n_t[0] > 0) + (n_t[1] > 0);
-            mbar_arrive_expect_tx(q_full, tiles * p.rows * (uint32_t)(D * 2));
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                for (int b = 0; b < C::BOXES && n_t[t] > 0; ++b)
-                    tma_load_4d(sQ + t * C::Q_BYTES + b * (TQ * 128), &tmQ, b * 64, (int32_t)head0, (int32_t)l0[t],
-                                (int32_t)b0[t], q_full);
-        }
-        for (uint32_t j = 0; j < n_kv && j < (uint32_t)C::STAGES; ++j) {
-            load_k(j);
-            load_v(j);
-        }
     }
     if (warp == 1) {
         tmem_alloc(tmem_slot, 512);
@@ -254,100 +255,152 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
 
     if (warp == 0 && lane == 0) {
         // ------------------------------------------------ TMA producer
-        const uint32_t pre = n_kv < (uint32_t)C::STAGES ? n_kv : (uint32_t)C::STAGES;
-        uint32_t issued_k = pre, issued_v = pre;
+        // Loads of an item's tiles start as soon as the items before it have
+        // left the buffers: Q_t once its last S_t is computed, K and V through
+        // rings that run on across items (g: ring index of the next K / V).
+        uint32_t g = 0, q_loads[2] = {0, 0};
+        uint32_t issued_k = 0, issued_v = 0;
         bool failed = false;
-        for (uint32_t j = pre; j < n_kv; ++j) {
-            const uint32_t s = j % C::STAGES, ph = ((j / C::STAGES) & 1) ^ 1;
-            if (!mbar_wait(&k_empty[s], ph)) {
+        for (uint32_t i = 0, item; (item = item_at(i)) < p.items && !failed; ++i) {
+            if (!mbar_wait(&plan_empty[i % PLANS], ((i / PLANS) & 1) ^ 1)) {
                 failed = true;
                 break;
             }
-            load_k(j);
-            ++issued_k;
-            if (!mbar_wait(&v_empty[s], ph)) {
-                failed = true;
-                break;
+            TileItem it;
+            it.set(p, item);
+            plans[i % PLANS] = it;
+            mbar_arrive(&plan_full[i % PLANS]);
+            const int32_t k_b = p.shared_keys || p.k_batch_bcast ? 0 : (int32_t)it.unit_b;
+            const int32_t v_b = p.shared_keys || p.v_batch_bcast ? 0 : (int32_t)it.unit_b;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (it.n_t[t] == 0 || failed) continue;
+                if (!mbar_wait(&q_empty[t], (q_loads[t] & 1) ^ 1)) {
+                    failed = true;
+                    break;
+                }
+                mbar_arrive_expect_tx(&q_full[t], p.rows * (uint32_t)(D * 2));
+                for (int b = 0; b < C::BOXES; ++b)
+                    tma_load_4d(sQ + t * C::Q_BYTES + b * (TQ * 128), &tmQ, b * 64, (int32_t)it.head0, (int32_t)it.l0[t],
+                                (int32_t)it.b0[t], &q_full[t]);
+                ++q_loads[t];
             }
-            load_v(j);
-            ++issued_v;
+            for (uint32_t j = 0; j < it.n_kv && !failed; ++j, ++g) {
+                const uint32_t s = g % C::STAGES, ph = ((g / C::STAGES) & 1) ^ 1;
+                const int32_t key = (int32_t)(it.key_tile(j) * TK);
+                unsigned char* kd = sKV + s * C::STAGE_BYTES;
+                if (!mbar_wait(&k_empty[s], ph)) {
+                    failed = true;
+                    break;
+                }
+                mbar_arrive_expect_tx(&k_full[s], C::K_BYTES);
+                for (int b = 0; b < C::BOXES; ++b)
+                    tma_load_4d(kd + b * (TK * 128), &tmK, b * 64, key, (int32_t)it.kv_head, k_b, &k_full[s]);
+                ++issued_k;
+                if (!mbar_wait(&v_empty[s], ph)) {
+                    failed = true;
+                    break;
+                }
+                mbar_arrive_expect_tx(&v_full[s], C::K_BYTES);
+                for (int b = 0; b < C::BOXES; ++b)
+                    tma_load_4d(kd + C::K_BYTES + b * (TK * 128), &tmV, b * 64, key, (int32_t)it.kv_head, v_b, &v_full[s]);
+                ++issued_v;
+            }
         }
-        if (failed) {
-            // drain the copies still in flight (bounded) before exiting
-            atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
-            for (uint32_t j = issued_k >= C::STAGES ? issued_k - C::STAGES : 0; j < issued_k; ++j)
-                (void)mbar_wait(&k_full[j % C::STAGES], (j / C::STAGES) & 1);
-            for (uint32_t j = issued_v >= C::STAGES ? issued_v - C::STAGES : 0; j < issued_v; ++j)
-                (void)mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1);
-        }
-        if (n_kv > 0) (void)mbar_wait(q_full, 0);
+        // the copies still in flight land (bounded) before the block ends
+        if (failed) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
+        for (uint32_t j = issued_k >= C::STAGES ? issued_k - C::STAGES : 0; failed && j < issued_k; ++j)
+            (void)mbar_wait(&k_full[j % C::STAGES], (j / C::STAGES) & 1);
+        for (uint32_t j = issued_v >= C::STAGES ? issued_v - C::STAGES : 0; failed && j < issued_v; ++j)
+            (void)mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1);
+        for (int t = 0; t < 2 && failed; ++t)
+            if (q_loads[t]) (void)mbar_wait(&q_full[t], (q_loads[t] - 1) & 1);
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         const uint32_t idesc_s = f16_idesc(p.fmt, TQ, TK);
         const uint32_t idesc_o = f16_idesc(p.fmt, TQ, D) | (1u << 16);  // B (V) is MN-major
         auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
-        bool ok = n_kv == 0 || wait(q_full, 0);
-        auto issue_s = [&](int t, uint32_t j) -> bool {
-            const uint32_t s = j % C::STAGES;
-            if (!wait(&k_full[s], (j / C::STAGES) & 1)) return false;
-            tc_fence_after();
-            const uint64_t qd = sw128_desc(smem_u32(sQ + t * C::Q_BYTES));
-            const uint64_t kd = sw128_desc(smem_u32(sKV + s * C::STAGE_BYTES));
-            const uint32_t d = tmem + C::s_col(t);
+        bool ok = true;
+        // g: ring index of the item's first K / V; taken: S_t / PV_t pairs so
+        // far; outs: items in which tile t had any
+        uint32_t g = 0, taken[2] = {0, 0}, outs[2] = {0, 0};
+        for (uint32_t n = 0; item_at(n) < p.items; ++n) {
+            if (!(ok = ok && wait(&plan_full[n % PLANS], (n / PLANS) & 1))) break;
+            const TileItem it = plans[n % PLANS];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&plan_empty[n % PLANS]);
+            // left: S_t still to come in this item
+            auto issue_s = [&](int t, uint32_t j, uint32_t left) -> bool {
+                const uint32_t s = (g + j) % C::STAGES;
+                if (!wait(&k_full[s], ((g + j) / C::STAGES) & 1)) return false;
+                tc_fence_after();
+                const uint64_t qd = sw128_desc(smem_u32(sQ + t * C::Q_BYTES));
+                const uint64_t kd = sw128_desc(smem_u32(sKV + s * C::STAGE_BYTES));
+                const uint32_t d = tmem + C::s_col(t);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-                const uint32_t off = (uint32_t)((k / 4) * (TQ * 128) + (k % 4) * 32);
-                umma_f16_ss_warp(d, desc_add(qd, off), desc_add(kd, off), idesc_s, k != 0);
-            }
-            umma_commit_warp(&s_full[t]);
-            return true;
-        };
-        // i: how many key tiles query tile t has taken before this one
-        auto issue_pv = [&](int t, uint32_t j, uint32_t i) -> bool {
-            const uint32_t s = j % C::STAGES;
-            if (!wait(&p_full[t], i & 1)) return false;
-            tc_fence_after();
-            const uint64_t vd = sw128_mn_desc(smem_u32(sKV + s * C::STAGE_BYTES + C::K_BYTES), TK * 128);
-            const uint32_t d = tmem + C::o_col(t), a = tmem + C::s_col(t);
-            umma_f16_ts_warp(d, a, vd, idesc_o, i != 0);
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (uint32_t)((k / 4) * (TQ * 128) + (k % 4) * 32);
+                    umma_f16_ss_warp(d, desc_add(qd, off), desc_add(kd, off), idesc_s, k != 0);
+                }
+                umma_commit_warp(&s_full[t]);
+                if (left == 0) umma_commit_warp(&q_empty[t]);
+                return true;
+            };
+            auto issue_pv = [&](int t, uint32_t j, uint32_t i) -> bool {
+                const uint32_t s = (g + j) % C::STAGES;
+                if (!wait(&p_full[t], taken[t] & 1)) return false;
+                // the first product of an item overwrites O_t: the item
+                // before it must have been read out
+                if (i == 0 && !wait(&o_free[t], (outs[t] & 1) ^ 1)) return false;
+                tc_fence_after();
+                const uint64_t vd = sw128_mn_desc(smem_u32(sKV + s * C::STAGE_BYTES + C::K_BYTES), TK * 128);
+                const uint32_t d = tmem + C::o_col(t), a = tmem + C::s_col(t);
+                umma_f16_ts_warp(d, a, vd, idesc_o, i != 0);
 #pragma unroll
-            for (int k = 1; k < TK / 16; ++k) umma_f16_ts_warp(d, a + k * 8, desc_add(vd, k * 16 * 128), idesc_o, 1u);
-            if (i + 1 == n_t[t]) umma_commit_warp(&o_done[t]);
-            return true;
-        };
-        uint32_t at[2], taken[2] = {0, 0};
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            at[t] = n_t[t] ? next_seen(t, 0) : n_kv;
-            if (ok && at[t] < n_kv) ok = issue_s(t, at[t]);
-        }
-        if (ok && n_kv > 0) umma_commit_warp(&k_empty[0]);  // K(0) consumed by every S(0)
-        for (uint32_t j = 0; ok && j < n_kv; ++j) {
-            const uint32_t s = j % C::STAGES;
-            ok = wait(&v_full[s], (j / C::STAGES) & 1);
-            const int64_t key0 = (int64_t)key_tile(j) * TK;
-            if (ok && p.lengths && !p.shared_keys && key0 + TK > filled) {
-                // value rows past the filled keys: zeros
-                const uint32_t from = (uint32_t)(filled - key0);
-                unsigned char* v = sKV + s * C::STAGE_BYTES + C::K_BYTES;
-                for (int b = 0; b < C::BOXES; ++b)
-                    for (uint32_t o = from * 128 + lane * 16; o < TK * 128; o += 512)
-                        *reinterpret_cast<uint4*>(v + b * (TK * 128) + o) = make_uint4(0u, 0u, 0u, 0u);
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
+                for (int k = 1; k < TK / 16; ++k) umma_f16_ts_warp(d, a + k * 8, desc_add(vd, k * 16 * 128), idesc_o, 1u);
+                if (i + 1 == it.n_t[t]) {
+                    umma_commit_warp(&o_done[t]);
+                    ++outs[t];
+                }
+                ++taken[t];
+                return true;
+            };
+            uint32_t at[2], done[2] = {0, 0};
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (!ok || at[t] != j) continue;
-                ok = issue_pv(t, j, taken[t]);
-                ++taken[t];
-                at[t] = taken[t] < n_t[t] ? next_seen(t, j + 1) : n_kv;
-                if (ok && at[t] < n_kv) ok = issue_s(t, at[t]);
+                at[t] = it.n_t[t] ? it.next_seen(t, 0) : it.n_kv;
+                if (!ok || at[t] >= it.n_kv) continue;
+                ok = wait(&q_full[t], outs[t] & 1) && issue_s(t, at[t], it.n_t[t] - 1);
             }
-            // V(j) is free once every PV(j) has completed, K(j + 1) once
-            // every S(j + 1) has (each was issued by now)
-            if (ok) umma_commit_warp(&v_empty[s]);
-            if (ok && j + 1 < n_kv) umma_commit_warp(&k_empty[(j + 1) % C::STAGES]);
+            if (ok && it.n_kv > 0) umma_commit_warp(&k_empty[g % C::STAGES]);  // the first K consumed by every S of it
+            for (uint32_t j = 0; ok && j < it.n_kv; ++j) {
+                const uint32_t s = (g + j) % C::STAGES;
+                ok = wait(&v_full[s], ((g + j) / C::STAGES) & 1);
+                const int64_t key0 = (int64_t)it.key_tile(j) * TK;
+                if (ok && p.lengths && !p.shared_keys && key0 + TK > it.filled) {
+                    // value rows past the filled keys: zeros
+                    const uint32_t from = (uint32_t)(it.filled - key0);
+                    unsigned char* v = sKV + s * C::STAGE_BYTES + C::K_BYTES;
+                    for (int b = 0; b < C::BOXES; ++b)
+                        for (uint32_t o = from * 128 + lane * 16; o < TK * 128; o += 512)
+                            *reinterpret_cast<uint4*>(v + b * (TK * 128) + o) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (!ok || at[t] != j) continue;
+                    ok = issue_pv(t, j, done[t]);
+                    ++done[t];
+                    at[t] = done[t] < it.n_t[t] ? it.next_seen(t, j + 1) : it.n_kv;
+                    if (ok && at[t] < it.n_kv) ok = issue_s(t, at[t], it.n_t[t] - done[t] - 1);
+                }
+                // V(j) is free once every PV(j) has completed, K(j + 1) once
+                // every S(j + 1) has (each was issued by now)
+                if (ok) umma_commit_warp(&v_empty[s]);
+                if (ok && j + 1 < it.n_kv) umma_commit_warp(&k_empty[(g + j + 1) % C::STAGES]);
+            }
+            g += it.n_kv;
         }
         if (!ok && lane == 0) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
         umma_commit_warp(drain);
@@ -357,261 +410,217 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         const int t = (warp - 2) / 4;
         const int quarter = warp & 3;
         const uint32_t row = (uint32_t)(quarter * 32 + lane);
-        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const uint32_t n = t ? n_t[1] : n_t[0], n_other = t ? n_t[0] : n_t[1];
+        const uint32_t tm_s = tmem + ((uint32_t)(quarter * 32) << 16) + C::s_col(t);
+        const uint32_t tm_o = tmem + ((uint32_t)(quarter * 32) << 16) + C::o_col(t);
         const float NEG = -__int_as_float(0x7f800000);
         const float sl = p.scale_log2;
-        // What a hidden key's raw score becomes: its logit is -inf whatever the scale's sign.
-        const float hidden = sl < 0.0f ? __int_as_float(0x7f800000) : NEG;
-        // keys of this row: [0, sinks) and [low, high]
-        int32_t high, low;
-        {
-            const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1 : base + (int64_t)((t ? l0[1] : l0[0]) + row / p.GB % p.LB);
-            high = (int32_t)max((int64_t)-1, min(pos, filled - 1));
-            low = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
-        }
-        const int32_t sinks = (int32_t)min((int64_t)0x7fffffff, p.sinks);
-        // this tile's key tiles: [0, ns) and then from a0 on, n in all from kt
-        const uint32_t ns = t ? plan.ns[1] : plan.ns[0], a0 = t ? plan.a0[1] : plan.a0[0];
-        uint32_t kt = n ? key_tile(t ? next_seen(1, 0) : next_seen(0, 0)) : 0;
-        float m_used = NEG;  // running max (log2 units)
-        float lsum = 0.0f;
+        uint32_t steps = 0, outs = 0;  // S_t taken, items with any, over all items
         bool ok = true;
-        for (uint32_t i = 0; i < n && ok; ++i) {
-            const int32_t key0 = (int32_t)(kt * TK);
-            kt = kt + 1 < ns ? kt + 1 : max(kt + 1, a0);
-            // Wait outcomes are made warp-uniform: tcgen05.ld/st are .sync.aligned.
-            if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], i & 1))) {
-                ok = false;
+        for (uint32_t turn = 0; item_at(turn) < p.items; ++turn) {
+            if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(&plan_full[turn % PLANS], (turn / PLANS) & 1)))) {
+                atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
                 break;
             }
-            tc_fence_after();
-            float x[TK];
+            // this tile's key tiles: [0, ns) and then from a0 on, n in all from kt
+            const TileItem& it = plans[turn % PLANS];
+            const uint32_t n = it.n_t[t];
+            uint32_t kt;
+            int32_t high, low;
             {
-                uint32_t r[TK];
-#pragma unroll
-                for (int c = 0; c < TK / 32; ++c)
-                    tmem_ld32(tmem + lane_base + C::s_col(t) + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < TK; ++e) x[e] = __uint_as_float(r[e]);
+                // keys of this row: [0, sinks) and [low, high]
+                const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1
+                                                  : it.base + (int64_t)(it.l0[t] + row / p.GB % p.LB);
+                high = (int32_t)max((int64_t)-1, min(pos, it.filled - 1));
+                low = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
+                kt = n ? it.key_tile(it.next_seen(t, 0)) : 0;
             }
-            // Hidden keys are masked in the raw scores, only in the tiles that
-            // hold some: past the row's position or the filled keys, or between
-            // the first keys and the window.
-            if (key0 + TK - 1 > high || (key0 < low && key0 + TK > sinks)) {
-                int32_t lim = high + 1 - key0, lo = low - key0;
-                const int32_t sk = sinks - key0;
-                if (lo > 0 && sk > 0) {
-                    if (lo >= TK) {
-                        lim = min(lim, sk), lo = 0;  // first keys only
-                    } else {  // first keys and the window in one tile
+            float m_used = NEG;  // running max (log2 units)
+            float lsum = 0.0f;
+            for (uint32_t i = 0; i < n && ok; ++i, ++steps) {
+                const int32_t key0 = (int32_t)(kt * TK);
+                kt = kt + 1 < it.plan.ns[t] ? kt + 1 : max(kt + 1, it.plan.a0[t]);
+                // Wait outcomes are made warp-uniform: tcgen05.ld/st are .sync.aligned.
+                if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], steps & 1))) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                float x[TK];
+                {
+                    uint32_t r[TK];
 #pragma unroll
-                        for (int e = 0; e < TK; ++e) x[e] = e < sk || e >= lo ? x[e] : hidden;
-                        lo = 0;
+                    for (int c = 0; c < TK / 32; ++c)
+                        tmem_ld32(tm_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < TK; ++e) x[e] = __uint_as_float(r[e]);
+                }
+                // Hidden keys are masked in the raw scores, only in the tiles that
+                // hold some: past the row's position or the filled keys, or between
+                // the first keys and the window.  A warp's rows are neighbours, so
+                // most 32-key chunks are seen, or hidden, by all of them.
+                if (__any_sync(0xffffffffu, key0 + TK - 1 > high || (key0 < low && key0 + TK > p.sinks32))) {
+                    int32_t lim = high + 1 - key0, lo = low - key0;
+                    const int32_t sk = p.sinks32 - key0;
+                    if (lo > 0 && sk > 0) {
+                        if (lo >= TK) {
+                            lim = min(lim, sk), lo = 0;  // first keys only
+                        } else {  // first keys and the window in one tile
+#pragma unroll
+                            for (int e = 0; e < TK; ++e) x[e] = e < sk || e >= lo ? x[e] : p.hidden;
+                            lo = 0;
+                        }
+                    }
+                    const int32_t lim0 = __reduce_min_sync(0xffffffffu, lim), lo1 = __reduce_max_sync(0xffffffffu, lo);
+#pragma unroll
+                    for (int c = 0; c < TK; c += 32) {
+                        if (lim0 < c + 32 || lo1 > c) {
+#pragma unroll
+                            for (int e = c; e < c + 32; ++e) x[e] = e >= lo && e < lim ? x[e] : p.hidden;
+                        }
                     }
                 }
-                if (lo > 0) {
+                if (sl == 0.0f) {  // logits 0, hidden keys stay -inf
 #pragma unroll
-                    for (int e = 0; e < TK; ++e) x[e] = e >= lo ? x[e] : hidden;
+                    for (int e = 0; e < TK; ++e) x[e] = x[e] == NEG ? NEG : 0.0f * x[e];
                 }
-                if (lim < TK) {
+                const bool use_min = sl < 0.0f;
+                // Four chains of three-input extremes: 64 instructions per row.
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+                if (use_min) {
 #pragma unroll
-                    for (int e = 0; e < TK; ++e) x[e] = e < lim ? x[e] : hidden;
-                }
-            }
-            if (sl == 0.0f) {  // logits 0, hidden keys stay -inf
+                    for (int e = 4; e < TK - 4; e += 8)
 #pragma unroll
-                for (int e = 0; e < TK; ++e) x[e] = x[e] == NEG ? NEG : 0.0f * x[e];
-            }
-            const bool use_min = sl < 0.0f;
-            // Four chains of three-input extremes: 64 instructions per row.
-            float mx[4] = {x[0], x[1], x[2], x[3]};
-            if (use_min) {
-#pragma unroll
-                for (int e = 4; e < TK - 4; e += 8)
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) mx[a] = min3n(mx[a], x[e + 2 * a], x[e + 2 * a + 1]);
-                mx[0] = min3n(mx[0], x[TK - 4], x[TK - 3]);
-                mx[1] = min3n(mx[1], x[TK - 2], x[TK - 1]);
-            } else {
-#pragma unroll
-                for (int e = 4; e < TK - 4; e += 8)
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) mx[a] = max3n(mx[a], x[e + 2 * a], x[e + 2 * a + 1]);
-                mx[0] = max3n(mx[0], x[TK - 4], x[TK - 3]);
-                mx[1] = max3n(mx[1], x[TK - 2], x[TK - 1]);
-            }
-            float mt = use_min ? min3n(min3n(mx[0], mx[1], mx[2]), mx[3], mx[3])
-                               : max3n(max3n(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-            if (sl != 0.0f) mt *= sl;  // raw extreme -> logit maximum
-            float alpha = 1.0f;
-            bool rescale = false;
-            if (mt > m_used + 8.0f) {
-                alpha = m_used == NEG ? 0.0f : ex2(m_used - mt);
-                rescale = i > 0 && lsum > 0.0f;
-                m_used = mt;
-            }
-            const float ref = m_used == NEG ? 0.0f : m_used + p.shift;
-            float2 lsa[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-            // Packed pairs overwrite the scores they came from, so P needs no
-            // registers of its own; one pair in eight takes the polynomial.
-            uint32_t* xb = reinterpret_cast<uint32_t*>(x);
-            const float mul = sl == 0.0f ? 1.0f : sl;
-            const float2 sl2 = make_float2(mul, mul), nb2 = make_float2(-ref, -ref);
-#pragma unroll
-            for (int c = 0; c < TK / 32; ++c) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float2 z = __ffma2_rn(make_float2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), sl2, nb2);
-                    const float2 w = (e & 7) == 7 ? ex2_poly2(z) : make_float2(ex2(z.x), ex2(z.y));
-                    if (!p.fmt) lsa[e & 3] = __fadd2_rn(lsa[e & 3], w);
-                    xb[c * 32 + e] = pack2(w.x, w.y, p.fmt);
-                }
-                tmem_st16(tmem + lane_base + C::s_col(t) + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&xb[c * 32]));
-            }
-            if (__any_sync(0xffffffffu, rescale)) {
-                const float f = rescale ? alpha : 1.0f;
-#pragma unroll 1
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t r[32];
-                    tmem_ld32(tmem + lane_base + C::o_col(t) + c * 32, r);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
-                    tmem_st32(tmem + lane_base + C::o_col(t) + c * 32, r);
-                }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[t]);
-            if (p.fmt) {  // BF16 P -> f32 is exact: the high half of the pattern
-#pragma unroll
-                for (int e = 0; e < TK / 2; ++e) {
-                    const uint32_t w = xb[(e / 16) * 32 + (e % 16)];
-                    lsa[e & 3] = __fadd2_rn(lsa[e & 3], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
-                }
-            }
-            const float2 l2 = __fadd2_rn(__fadd2_rn(lsa[0], lsa[1]), __fadd2_rn(lsa[2], lsa[3]));
-            lsum = lsum * alpha + (l2.x + l2.y);
-        }
-        if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[t], 0))) ok = false;
-        const uint32_t esz = p.out_low ? 2u : 4u;
-        if (p.tma_out) {
-            // O / l staged in the idle K/V ring once both tiles' MMAs are
-            // done, written by TMA through the output's box map.
-            if (n_other > 0 && ok && !__all_sync(0xffffffffu, mbar_wait(&o_done[1 - t], 0))) ok = false;
-            if (!ok) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
-            tc_fence_after();
-            const bool load = ok && n > 0;
-            const float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
-            unsigned char* stage = sKV + (uint32_t)t * (TQ * D * esz);
-            const uint32_t swz = row & 7u;
-#pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                if (load) {
-                    tmem_ld32(tmem + lane_base + C::o_col(t) + c * 32, r);
-                    tmem_wait_ld();
+                        for (int a = 0; a < 4; ++a) mx[a] = min3n(mx[a], x[e + 2 * a], x[e + 2 * a + 1]);
+                    mx[0] = min3n(mx[0], x[TK - 4], x[TK - 3]);
+                    mx[1] = min3n(mx[1], x[TK - 2], x[TK - 1]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = 0u;
-                }
-                if (p.out_low) {  // boxes of 64 16-bit values: chunk c is half of box c / 2
-                    unsigned char* dst = stage + (c / 2) * (TQ * 128) + row * 128;
+                    for (int e = 4; e < TK - 4; e += 8)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t q = (uint32_t)((c % 2) * 4 + e);
-                        *reinterpret_cast<uint4*>(dst + ((q ^ swz) * 16)) = make_uint4(
-                            encode_low_pair(__uint_as_float(r[8 * e]) * inv, __uint_as_float(r[8 * e + 1]) * inv, p.out_low),
-                            encode_low_pair(__uint_as_float(r[8 * e + 2]) * inv, __uint_as_float(r[8 * e + 3]) * inv, p.out_low),
-                            encode_low_pair(__uint_as_float(r[8 * e + 4]) * inv, __uint_as_float(r[8 * e + 5]) * inv, p.out_low),
-                            encode_low_pair(__uint_as_float(r[8 * e + 6]) * inv, __uint_as_float(r[8 * e + 7]) * inv, p.out_low));
+                        for (int a = 0; a < 4; ++a) mx[a] = max3n(mx[a], x[e + 2 * a], x[e + 2 * a + 1]);
+                    mx[0] = max3n(mx[0], x[TK - 4], x[TK - 3]);
+                    mx[1] = max3n(mx[1], x[TK - 2], x[TK - 1]);
+                }
+                float mt = use_min ? min3n(min3n(mx[0], mx[1], mx[2]), mx[3], mx[3])
+                                   : max3n(max3n(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+                if (sl != 0.0f) mt *= sl;  // raw extreme -> logit maximum
+                float alpha = 1.0f;
+                bool rescale = false;
+                if (mt > m_used + 8.0f) {
+                    alpha = m_used == NEG ? 0.0f : ex2(m_used - mt);
+                    rescale = i > 0 && lsum > 0.0f;
+                    m_used = mt;
+                }
+                const float ref = m_used == NEG ? 0.0f : m_used + p.shift;
+                float2 lsa[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                // Packed pairs overwrite the scores they came from, so P needs no
+                // registers of its own; one pair in eight takes the polynomial.
+                uint32_t* xb = reinterpret_cast<uint32_t*>(x);
+                const float mul = sl == 0.0f ? 1.0f : sl;
+                const float2 sl2 = make_float2(mul, mul), nb2 = make_float2(-ref, -ref);
+#pragma unroll
+                for (int c = 0; c < TK / 32; ++c) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float2 z = __ffma2_rn(make_float2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), sl2, nb2);
+                        const float2 w = (e & 7) == 7 ? ex2_poly2(z) : make_float2(ex2(z.x), ex2(z.y));
+                        if (!p.fmt) lsa[e & 3] = __fadd2_rn(lsa[e & 3], w);
+                        xb[c * 32 + e] = pack2(w.x, w.y, p.fmt);
                     }
-                } else {  // boxes of 32 f32 values
-                    unsigned char* dst = stage + c * (TQ * 128) + row * 128;
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        *reinterpret_cast<float4*>(dst + ((q ^ swz) * 16)) =
-                            make_float4(__uint_as_float(r[4 * q]) * inv, __uint_as_float(r[4 * q + 1]) * inv,
-                                        __uint_as_float(r[4 * q + 2]) * inv, __uint_as_float(r[4 * q + 3]) * inv);
+                    tmem_st16(tm_s + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&xb[c * 32]));
                 }
-            }
-            tc_fence_before();
-            fence_proxy_async_smem();
-            asm volatile("bar.sync 1, 256;" ::: "memory");  // every softmax warp's rows are staged
-            if (warp == 2 && lane == 0) {
-                const int boxes = p.out_low ? D / 64 : D / 32;
+                if (__any_sync(0xffffffffu, rescale)) {
+                    const float f = rescale ? alpha : 1.0f;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32(tm_o + c * 32, r);
+                        tmem_wait_ld();
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
-                    for (int bx = 0; bx < boxes && real[tt]; ++bx)
-                        tma_store_4d(&tmO, bx * (p.out_low ? 64 : 32), (int32_t)head0, (int32_t)l0[tt], (int32_t)b0[tt],
-                                     sKV + tt * (TQ * D * esz) + bx * (TQ * 128));
-                bulk_commit_group();
-                bulk_wait_read_all();
+                        for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * f);
+                        tmem_st32(tm_o + c * 32, r);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[t]);
+                if (p.fmt) {  // BF16 P -> f32 is exact: the high half of the pattern
+#pragma unroll
+                    for (int e = 0; e < TK / 2; ++e) {
+                        const uint32_t w = xb[(e / 16) * 32 + (e % 16)];
+                        lsa[e & 3] = __fadd2_rn(lsa[e & 3], make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)));
+                    }
+                }
+                const float2 l2 = __fadd2_rn(__fadd2_rn(lsa[0], lsa[1]), __fadd2_rn(lsa[2], lsa[3]));
+                lsum = lsum * alpha + (l2.x + l2.y);
             }
-        } else {
+            if (ok && n > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[t], outs & 1))) ok = false;
             if (!ok) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
             tc_fence_after();
             const bool load = ok && n > 0;
+            const uint32_t head = it.head0 + row % p.GB, l = it.l0[t] + row / p.GB % p.LB, b = it.b0[t] + row / (p.GB * p.LB);
+            const bool valid = it.real[t] && row < p.rows && l < p.L && b < p.B;
             float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
-            // (worked out here again: kept through the loop they would spill)
-            uint32_t r0 = row;
-            asm volatile("" : "+r"(r0));
-            const uint32_t head = head0 + r0 % p.GB, l = (t ? l0[1] : l0[0]) + r0 / p.GB % p.LB,
-                           b = (t ? b0[1] : b0[0]) + r0 / (p.GB * p.LB);
-            const bool valid = (t ? real[1] : real[0]) && r0 < p.rows && l < p.L && b < p.B;
-            float* rec = nullptr;
+            unsigned char* dst;  // this row's next 32 columns
             if (p.part) {
                 inv = 1.0f;
-                rec = p.part + ((((uint64_t)b * p.H + head) * p.L + l) * p.part_stride + p.part_first + split) * REC<D>;
-                if (valid) {
-                    rec[0] = m_used == NEG ? 0.0f : m_used + p.shift;
-                    rec[1] = load ? lsum : 0.0f;
-                }
-                rec += 4;
+                float* rec = p.part + ((((uint64_t)b * p.H + head) * p.L + l) * p.part_stride + p.part_first + it.split) * REC<D>;
+                if (valid) *reinterpret_cast<float2*>(rec) = make_float2(m_used == NEG ? 0.0f : m_used + p.shift, load ? lsum : 0.0f);
+                dst = reinterpret_cast<unsigned char*>(rec + 4);
+            } else {
+                const uint64_t at = (uint64_t)b * p.o_sb + (uint64_t)head * p.o_sh + (uint64_t)l * p.o_sl;
+                dst = static_cast<unsigned char*>(p.out) + at * (p.out_low ? 2 : 4);
             }
-            const uint64_t at = (uint64_t)b * p.o_sb + (uint64_t)head * p.o_sh + (uint64_t)l * p.o_sl;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&plan_empty[turn % PLANS]);  // the plan is no longer needed
+            const bool low_rows = !p.part && p.out_low;
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t r[32];
                 if (load) {
-                    tmem_ld32(tmem + lane_base + C::o_col(t) + c * 32, r);
+                    tmem_ld32(tm_o + c * 32, r);
                     tmem_wait_ld();
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) r[e] = 0u;
                 }
-                if (!valid) continue;
-                if (p.part) {
+                if (c == D / 32 - 1 && load) {
+                    tc_fence_before();
+                    mbar_arrive(&o_free[t]);  // O_t is out of TMEM
+                }
+                if (valid && low_rows) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            w[e] = pack2(__uint_as_float(r[h * 16 + 2 * e]) * inv, __uint_as_float(r[h * 16 + 2 * e + 1]) * inv, p.fmt);
+                        if (p.wide) {
+                            store32(dst + c * 64 + h * 32, w);
+                        } else {
+                            *reinterpret_cast<uint4*>(dst + c * 64 + h * 32) = make_uint4(w[0], w[1], w[2], w[3]);
+                            *reinterpret_cast<uint4*>(dst + c * 64 + h * 32 + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                } else if (valid) {
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<uint4*>(rec + c * 32 + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
-                } else if (p.out_low) {  // rows 16-byte aligned (host)
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + c * 32);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        dst[e / 8] = make_uint4(
-                            encode_low_pair(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv, p.out_low),
-                            encode_low_pair(__uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv, p.out_low),
-                            encode_low_pair(__uint_as_float(r[e + 4]) * inv, __uint_as_float(r[e + 5]) * inv, p.out_low),
-                            encode_low_pair(__uint_as_float(r[e + 6]) * inv, __uint_as_float(r[e + 7]) * inv, p.out_low));
-                } else {
-                    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + c * 32);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        dst[e / 4] = make_float4(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv,
-                                                 __uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv);
+                        *reinterpret_cast<float4*>(dst + c * 128 + e * 4) =
+                            make_float4(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv,
+                                        __uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv);
                 }
             }
-            tc_fence_before();
+            if (n > 0) ++outs;
         }
+        tc_fence_before();
     }
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // in a chain: ends after the launch before it
 }
 
 // ------------------------------------------------------ joining records
@@ -706,6 +715,7 @@ struct SpanMergeParams {
 
 template <int D>
 __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the records are written
     const uint64_t w = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (w >= p.rows) return;
     float M = -__int_as_float(0x7f800000), L = 0.0f, o[D / 32];
@@ -1160,27 +1170,85 @@ uint64_t largest_divisor(uint64_t n, uint64_t most) {
     return d;
 }
 
+// How span_tile_kernel covers a call's query rows, and its key ranges.
+struct TileGrid {
+    uint64_t GB, LB, NB;     // the tile's box
+    uint64_t tiles, units;   // tiles per unit
+    uint64_t splits;
+};
+
+// The box: all heads of a group (their largest divisor up to 128) and, over
+// the shared prefix, whose mask does not depend on the row, the LB queries x
+// NB sequences that make the fewest tiles (33 queries of 16 sequences, groups
+// of 4: 2 x 16, 17 tiles; 32 x 1 would make 32, half of them nearly empty).
+// Key ranges when the pairs of tiles alone do not fill the GPU: about one CTA
+// per SM, at least two key tiles each.  (A key tile takes a CTA 1.5 us with two
+// tiles of rows and 1.7 us with one, so rows are always paired.)
+TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared) {
+    TileGrid g{};
+    g.GB = largest_divisor(a.G, TQ);
+    const uint64_t room = TQ / g.GB;
+    g.LB = std::min(a.L, room), g.NB = 1;
+    auto count = [&](uint64_t lb, uint64_t nb) { return (a.L + lb - 1) / lb * ((a.B + nb - 1) / nb); };
+    if (shared) {
+        for (uint64_t lb = 1; lb <= std::min(a.L, room); ++lb) {
+            const uint64_t nb = std::min(a.B, room / lb);
+            if (lb == 1 || count(lb, nb) < count(g.LB, g.NB)) g.LB = lb, g.NB = nb;
+        }
+    }
+    g.tiles = shared ? count(g.LB, g.NB) : (a.L + g.LB - 1) / g.LB;
+    g.units = a.H / g.GB * (shared ? 1 : a.B);
+    uint64_t keys = ((shared ? s.prefix_keys : a.Lk) + TK - 1) / TK;  // tiles that a CTA walks at most
+    if (!shared)
+        keys = std::min(keys, (std::min(s.sinks, a.Lk) + TK - 1) / TK + (std::min(s.window, a.Lk) + 2 * g.LB + TK - 1) / TK + 1);
+    const uint64_t sms = (uint64_t)sm_count();
+    auto ranges = [&](uint64_t ctas) -> uint64_t {
+        if (ctas >= sms || keys < 4) return 1;
+        const uint64_t want = std::min<uint64_t>(sms / ctas, keys / 2);
+        if (want <= 1) return 1;
+        const uint64_t per = (keys + want - 1) / want;
+        return (keys + per - 1) / per;
+    };
+    g.splits = ranges(g.units * ((g.tiles + 1) / 2));
+    return g;
+}
+
+// A launch that may begin while the stream's previous kernel ends (overlap):
+// the kernel waits for it with griddepcontrol.wait before it touches anything
+// that depends on it, and every one of a chain does so before it ends.
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, bool overlap, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap ? 1 : 0;
+    (void)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // The tcgen05 kernel over the shared prefix (shared = true) or over the
 // sequences' own keys.  part: records are written there (stride and first
 // index given; `splits` ranges), else output rows.
 template <int D>
 int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* part, uint32_t part_stride, uint32_t part_first,
-                 uint32_t splits, float shift, cudaStream_t st) {
+                 const TileGrid& g, float shift, bool overlap, cudaStream_t st) {
     using C = TCfg<D>;
     SpanTileParams p{};
     p.fmt = a.fmt;
     p.B = (uint32_t)a.B, p.H = (uint32_t)a.H, p.L = (uint32_t)a.L;
     p.Lk = (uint32_t)(shared ? s.prefix_keys : a.Lk);
     p.group = (uint32_t)a.G;
-    p.GB = (uint32_t)largest_divisor(a.G, TQ);
-    p.LB = (uint32_t)std::min<uint64_t>(a.L, TQ / p.GB);
-    p.NB = shared ? (uint32_t)std::min<uint64_t>(a.B, std::max<uint64_t>(1, a.L == p.LB ? TQ / (p.GB * p.LB) : 1)) : 1u;
+    p.GB = (uint32_t)g.GB, p.LB = (uint32_t)g.LB, p.NB = (uint32_t)g.NB;
     p.rows = p.GB * p.LB * p.NB;
     p.l_tiles = (p.L + p.LB - 1) / p.LB;
-    p.tiles = shared ? p.l_tiles * ((p.B + p.NB - 1) / p.NB) : p.l_tiles;
-    p.pairs = (p.tiles + 1) / 2;
+    p.tiles = (uint32_t)g.tiles;
+    p.groups = (p.tiles + 1) / 2;
     p.head_blocks = p.H / p.GB;
-    p.units = shared ? p.head_blocks : p.head_blocks * p.B;
     p.shared_keys = shared ? 1 : 0;
     p.k_batch_bcast = a.k.batch_bcast ? 1 : 0, p.v_batch_bcast = a.v.batch_bcast ? 1 : 0;
     p.lengths = shared ? nullptr : s.lengths;
@@ -1188,11 +1256,13 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
     p.offset = s.offset, p.window = (int64_t)s.window, p.sinks = (int64_t)s.sinks;
     p.scale_log2 = s.base.scale * 1.4426950408889634f;
     p.shift = shift;
-    p.splits = splits;
+    p.hidden = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;
+    p.sinks32 = (int32_t)std::min<uint64_t>(s.sinks, 0x7fffffff);
+    p.splits = (uint32_t)g.splits;
     p.part = part, p.part_stride = part_stride, p.part_first = part_first;
     p.out = a.op, p.out_low = s.base.out_low;
     p.o_sb = a.o.s_batch, p.o_sh = a.o.s_head, p.o_sl = a.o.s_row;
-    CUtensorMap tq, tk, tv, to{};
+    CUtensorMap tq, tk, tv;
     const uint32_t dt = a.fmt ? FB_BF16 : FB_F16;
     const uint32_t qbox[3] = {p.GB, p.LB, p.NB}, kbox[3] = {TK, 1, 1};
     if (!span_map(&tq, a.qp, dt, D, {a.H, a.L, a.B}, {a.q.s_head, a.q.s_row, a.q.s_batch}, qbox, true)) return FB_ERR_UNSUPPORTED;
@@ -1207,46 +1277,17 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
             !span_map(&tv, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox, true))
             return FB_ERR_UNSUPPORTED;
     }
-    if (!part)
-        p.tma_out = span_map(&to, a.op, s.base.out_low ? s.base.out_low : (uint32_t)FB_F32, D, {a.H, a.L, a.B},
-                             {a.o.s_head, a.o.s_row, a.o.s_batch}, qbox, false)
-                        ? 1
-                        : 0;
-    const uint64_t grid = (uint64_t)p.units * p.pairs * splits;
-    if (grid > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
+    auto runs32 = [](uint64_t n, uint64_t stride) { return n <= 1 || stride % 16 == 0; };
+    p.wide = reinterpret_cast<uintptr_t>(a.op) % 32 == 0 && runs32(a.B, a.o.s_batch) && runs32(a.H, a.o.s_head) && runs32(a.L, a.o.s_row);
+    const uint64_t items = g.units * p.groups * p.splits;
+    if (items > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
+    p.items = (uint32_t)items;
+    const uint64_t grid = std::min<uint64_t>(items, (uint64_t)sm_count());
     if (cudaFuncSetAttribute(span_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
         return launch_status("shared-memory attribute");
-    span_tile_kernel<D><<<(unsigned)grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, to, p);
+    launch_after(span_tile_kernel<D>, (unsigned)grid, C::THREADS, C::SMEM, overlap, st, tq, tk, tv, p);
     count_launch(kernel_name("span_tile_kernel", {D, shared ? 1 : 0}).c_str());
     return launch_status("kernel launch");
-}
-
-// CTAs of one key range and the key tiles that such a CTA walks at most.
-template <int D>
-void tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared, uint64_t* ctas, uint64_t* key_tiles) {
-    const uint64_t GB = largest_divisor(a.G, TQ), LB = std::min<uint64_t>(a.L, TQ / GB);
-    const uint64_t l_tiles = (a.L + LB - 1) / LB;
-    if (shared) {
-        const uint64_t NB = std::min<uint64_t>(a.B, std::max<uint64_t>(1, a.L == LB ? TQ / (GB * LB) : 1));
-        *ctas = a.H / GB * ((l_tiles * ((a.B + NB - 1) / NB) + 1) / 2);
-        *key_tiles = (s.prefix_keys + TK - 1) / TK;
-    } else {
-        *ctas = a.B * (a.H / GB) * ((l_tiles + 1) / 2);
-        const uint64_t all = (a.Lk + TK - 1) / TK;
-        const uint64_t seen = (std::min(s.sinks, a.Lk) + TK - 1) / TK + (std::min(s.window, a.Lk) + 2 * LB + TK - 1) / TK + 1;
-        *key_tiles = std::min(all, seen);
-    }
-}
-
-// Key ranges that fill the GPU when the pairs alone do not: about one CTA
-// per SM, at least two key tiles each.
-uint64_t tile_splits(uint64_t ctas, uint64_t key_tiles) {
-    const uint64_t sms = (uint64_t)sm_count();
-    if (ctas >= sms || key_tiles < 4) return 1;
-    const uint64_t splits = std::min<uint64_t>(sms / ctas, key_tiles / 2);
-    if (splits <= 1) return 1;
-    const uint64_t per = (key_tiles + splits - 1) / splits;
-    return (key_tiles + per - 1) / per;
 }
 
 template <int D>
@@ -1259,7 +1300,7 @@ int launch_merge(const SpanArgs& s, const SpanOperands& a, const float* part, ui
     m.out = a.op, m.out_low = s.base.out_low;
     m.o_sb = a.o.s_batch, m.o_sh = a.o.s_head, m.o_sl = a.o.s_row;
     if ((m.rows + 7) / 8 > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
-    span_merge_kernel<D><<<(unsigned)((m.rows + 7) / 8), 256, 0, st>>>(m);
+    launch_after(span_merge_kernel<D>, (unsigned)((m.rows + 7) / 8), 256, 0, true, st, m);
     count_launch(kernel_name("span_merge_kernel", {D}).c_str());
     return launch_status("kernel launch");
 }
@@ -1295,17 +1336,7 @@ int launch_decode(const SpanArgs& s, const SpanOperands& a, const float* prefix,
     auto kernel = a.fmt ? span_decode_kernel<D, 1> : span_decode_kernel<D, 0>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DCfg<D>::SMEM) != cudaSuccess)
         return launch_status("shared-memory attribute");
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(32 * DEC_WARPS);
-    cfg.dynamicSmemBytes = DCfg<D>::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = prefix ? 1 : 0;
-    (void)cudaLaunchKernelEx(&cfg, kernel, d);
+    launch_after(kernel, (unsigned)grid, 32 * DEC_WARPS, DCfg<D>::SMEM, prefix != nullptr, st, d);
     count_launch(kernel_name("span_decode_kernel", {D, (int)a.fmt}).c_str());
     return launch_status("kernel launch");
 }
@@ -1314,28 +1345,26 @@ template <int D>
 int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
     const bool prefix = s.prefix_keys > 0, own = a.Lk > 0;
     const float shift = weight_shift(a.fmt, a.Lk + s.prefix_keys);
-    uint64_t pc = 0, pt = 0, oc = 0, ot = 0;
-    if (prefix) tile_grid<D>(s, a, true, &pc, &pt);
-    if (own) tile_grid<D>(s, a, false, &oc, &ot);
-    const uint64_t ps = prefix ? tile_splits(pc, pt) : 0;
+    const TileGrid pg = prefix ? tile_grid(s, a, true) : TileGrid{};
+    const uint64_t ps = pg.splits;
     if (a.G * a.L <= 16) {  // few rows: the own keys streamed, the prefix's records joined there
         float* part = nullptr;
         if (prefix) {
             part = static_cast<float*>(scratch(st, a.B * a.H * a.L * ps * REC<D> * sizeof(float), SCRATCH_SPAN));
             if (!part) return FB_ERR_DRIVER;
-            if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)ps, 0, (uint32_t)ps, shift, st); r != FB_OK) return r;
+            if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)ps, 0, pg, shift, false, st); r != FB_OK) return r;
         }
         return launch_decode<D>(s, a, part, (uint32_t)ps, shift, st);
     }
-    const uint64_t os = own ? tile_splits(oc, ot) : 0;
-    if (ps + os <= 1) return launch_tiles<D>(s, a, prefix, nullptr, 0, 0, 1, shift, st);
-    const uint64_t count = ps + os;
+    const TileGrid og = own ? tile_grid(s, a, false) : TileGrid{};
+    const uint64_t count = ps + og.splits;
+    if (count <= 1) return launch_tiles<D>(s, a, prefix, nullptr, 0, 0, prefix ? pg : og, shift, false, st);
     float* part = static_cast<float*>(scratch(st, a.B * a.H * a.L * count * REC<D> * sizeof(float), SCRATCH_SPAN));
     if (!part) return FB_ERR_DRIVER;
     if (prefix)
-        if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)count, 0, (uint32_t)ps, shift, st); r != FB_OK) return r;
+        if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)count, 0, pg, shift, false, st); r != FB_OK) return r;
     if (own)
-        if (int r = launch_tiles<D>(s, a, false, part, (uint32_t)count, (uint32_t)ps, (uint32_t)os, shift, st); r != FB_OK) return r;
+        if (int r = launch_tiles<D>(s, a, false, part, (uint32_t)count, (uint32_t)ps, og, shift, prefix, st); r != FB_OK) return r;
     return launch_merge<D>(s, a, part, (uint32_t)count, st);
 }
 
