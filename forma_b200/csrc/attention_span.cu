@@ -47,18 +47,18 @@ constexpr int REC = D + 4;
 // x LB consecutive queries x NB sequences, gathered by one 4-D TMA box over
 // {depth, heads, queries, batch}, so that grouped heads share the key tiles
 // whatever Q's strides are.  A work item is two tiles and the key tiles that
-// either sees, in order: those of the first keys, then those of the two
-// windows; a tile of rows takes part only in the key tiles that it sees.
+// either sees; a tile of rows takes part only in the key tiles that it sees.
 // CTAs are persistent, one per SM: the next item's loads start while this
 // one's last products and epilogue run (an item's own start and end cost
 // 12 us when each was a CTA, eight key tiles' time).
 //   warp 0      TMA: both Q tiles, then K and V tiles of 128 keys through
 //               rings of 2 (D = 128) or 4 (D = 64) slots
+//   warp 2      the items' plans
 //   warp 1      TMEM and MMA issue: S_t = Q_t K^T, O_t += P_t V, the two
 //               tiles in turn so that one's products run during the other's
 //               softmax; value rows past the filled keys are zeroed in shared
 //               memory first (a weight of 0 does not hide a NaN there)
-//   warps 2-9   softmax, one query row per thread: lazy running maximum
+//   warps 4-11  softmax, one query row per thread: lazy running maximum
 //               (raised, and O rescaled, only past 2^8), P over S in TMEM; at
 //               an item's end O / l, or a record, straight from registers, a
 //               row's 32 bytes per store
@@ -90,7 +90,7 @@ struct SpanTileParams {
 
 template <int D>
 struct TCfg {
-    static constexpr int THREADS = 64 + 2 * 128;
+    static constexpr int THREADS = 3 * 128;
     static constexpr int BOXES = D / 64;
     static constexpr int Q_BYTES = TQ * D * 2;
     static constexpr int K_BYTES = TK * D * 2;
@@ -101,41 +101,33 @@ struct TCfg {
     static __device__ __forceinline__ uint32_t o_col(int t) { return (uint32_t)(2 * TK + t * 128); }
 };
 
-// The key tiles of a pair of query tiles: joint index j stands for key tile
-// j < s ? j : a + (j - s); query tile t sees key tiles [0, ns[t]) and
-// [a0[t], e[t]).
-struct TilePlan {
-    uint32_t s, a, n;          // joint list length n
-    uint32_t ns[2], a0[2], e[2];
-    __device__ __forceinline__ uint32_t tile(uint32_t j) const { return j < s ? j : a + (j - s); }
-    __device__ __forceinline__ bool sees(int t, uint32_t tile) const { return tile < ns[t] || (tile >= a0[t] && tile < e[t]); }
-    __device__ __forceinline__ uint32_t count(int t, uint32_t j0, uint32_t j1) const {
-        auto overlap = [](uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
-            const uint32_t lo = max(x0, y0), hi = min(x1, y1);
-            return hi > lo ? hi - lo : 0u;
-        };
-        uint32_t c = overlap(0, ns[t], min(j0, s), min(j1, s)) + overlap(a0[t], e[t], min(j0, s), min(j1, s));
-        if (j1 > s) c += overlap(a0[t], e[t], a + max(j0, s) - s, a + (j1 - s));
-        return c;
-    }
-};
-
-// One work item: up to two tiles of a unit and one key range.  The producer
-// works it out and leaves it in shared memory, PLANS items ahead at most.
+// One work item: up to two tiles of a unit and one key range.  A warp of its
+// own works it out and leaves it in shared memory, PLANS items ahead at most
+// (its few hundred dependent integer instructions took the producer 10k cycles
+// per item, most of what an item cost besides its key tiles).
+//
+// Its keys are numbered through: virtual key v is key v below `s16` (the first
+// keys, rounded up to 16) and key v - s16 + lo from there on, lo the earliest
+// window's start; where the two meet, s16 = lo = 0.  Virtual tiles hold 128
+// virtual keys: the one that holds the border is gathered from 16-row boxes,
+// the others are one box at any key, so the first keys cost no tile of their
+// own and a window starts a tile.
 constexpr int PLANS = 4;
 struct TileItem {
     uint32_t split, head0, kv_head, unit_b;
-    uint32_t b0[2], l0[2], n_t[2];  // first sequence, first query, key tiles of each tile
+    uint32_t b0[2], l0[2];          // first sequence and first query of each query tile
     bool real[2];
-    uint32_t j0, n_kv;              // this range of the joint list
+    uint32_t s16, lo;
+    uint32_t j0, n_kv;              // this range of the virtual tiles
+    // Query tile t sees n_t of them: those of index (from j0) below near[t],
+    // then those from far[t] on.
+    uint32_t n_t[2], near[2], far[2];
     int64_t filled, base;
-    TilePlan plan;
-    __device__ __forceinline__ uint32_t key_tile(uint32_t j) const { return plan.tile(j0 + j); }
-    // next joint index >= j of this range that tile t sees (n_kv if none)
-    __device__ __forceinline__ uint32_t next_seen(int t, uint32_t j) const {
-        while (j < n_kv && !plan.sees(t, key_tile(j))) ++j;
-        return j;
+    static __device__ __forceinline__ uint32_t after(uint32_t j, uint32_t near, uint32_t far) {
+        return j + 1 < near ? j + 1 : max(j + 1, far);
     }
+    // virtual key numbers of the keys from lo on: key + shift()
+    __device__ __forceinline__ int32_t shift() const { return (int32_t)s16 - (int32_t)lo; }
     __device__ __forceinline__ void set(const SpanTileParams& p, uint32_t item) {
         // Last queries (the most keys under a long window) of every unit first.
         const uint32_t units = p.items / (p.groups * p.splits);
@@ -150,36 +142,47 @@ struct TileItem {
             base = filled - (int64_t)p.L;
         }
         Reach rc[2];
+        int64_t first = 0, start = (int64_t)1 << 62, last = -1;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint32_t tile = group * 2 + t;
             real[t] = tile < p.tiles;
             b0[t] = p.shared_keys ? tile / p.l_tiles * p.NB : unit_b;
             l0[t] = (p.shared_keys ? tile % p.l_tiles : tile) * p.LB;
-            plan.ns[t] = plan.a0[t] = plan.e[t] = 0;
             rc[t] = Reach{0, 0, -1};
             if (!real[t]) continue;
             if (p.shared_keys) rc[t] = Reach{0, 0, (int64_t)p.Lk - 1};
             else rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
             if (rc[t].hi < 0) continue;
-            plan.ns[t] = (uint32_t)((rc[t].first + TK - 1) / TK);
-            if (rc[t].lo <= rc[t].hi) {
-                plan.a0[t] = max((uint32_t)(rc[t].lo / TK), plan.ns[t]);
-                plan.e[t] = max((uint32_t)(rc[t].hi / TK) + 1, plan.a0[t]);
-            }
+            first = max(first, rc[t].first);
+            if (rc[t].lo <= rc[t].hi) start = min(start, rc[t].lo), last = max(last, rc[t].hi);
         }
-        plan.s = max(plan.ns[0], plan.ns[1]);
-        uint32_t a = 0xffffffffu, e = 0;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            if (plan.e[t] > plan.a0[t]) a = min(a, plan.a0[t]), e = max(e, plan.e[t]);
-        plan.a = e ? max(a, plan.s) : plan.s;
-        plan.n = plan.s + (e > plan.a ? e - plan.a : 0);
-        const uint32_t per = (plan.n + p.splits - 1) / p.splits;
-        j0 = min(split * per, plan.n);
-        const uint32_t j1 = min(j0 + per, plan.n);
+        int64_t s = (first + 15) / 16 * 16, end;
+        if (last < 0) s = 0, start = 0, end = first;              // the first keys alone
+        else if (start <= s) s = 0, start = 0, end = last + 1;    // one run
+        else end = s + last - start + 1;
+        s16 = (uint32_t)s, lo = (uint32_t)start;
+        const uint32_t all = (uint32_t)((end + TK - 1) / TK), per = (all + p.splits - 1) / p.splits;
+        j0 = min(split * per, all);
+        const uint32_t j1 = min(j0 + per, all);
         n_kv = j1 - j0;
-        n_t[0] = plan.count(0, j0, j1), n_t[1] = plan.count(1, j0, j1);
+        auto overlap = [&](uint32_t x0, uint32_t x1) {
+            const uint32_t y0 = max(x0, j0), y1 = min(x1, j1);
+            return y1 > y0 ? y1 - y0 : 0u;
+        };
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            uint32_t ns = 0, a0 = 0, e = 0;
+            if (rc[t].hi >= 0) {
+                ns = (uint32_t)((rc[t].first + TK - 1) / TK);
+                if (rc[t].lo <= rc[t].hi) {
+                    a0 = max((uint32_t)((rc[t].lo - start + s) / TK), ns);
+                    e = max((uint32_t)((rc[t].hi - start + s) / TK) + 1, a0);
+                }
+            }
+            n_t[t] = overlap(0, ns) + overlap(a0, e);
+            near[t] = overlap(0, ns), far[t] = max(a0, j0) - j0;
+        }
     }
 };
 
@@ -192,7 +195,9 @@ __device__ __forceinline__ void store32(void* dst, const uint32_t (&r)[8]) {
 template <int D>
 __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __grid_constant__ CUtensorMap tmQ,
                                                                        const __grid_constant__ CUtensorMap tmK,
-                                                                       const __grid_constant__ CUtensorMap tmV, SpanTileParams p) {
+                                                                       const __grid_constant__ CUtensorMap tmV,
+                                                                       const __grid_constant__ CUtensorMap tmK16,
+                                                                       const __grid_constant__ CUtensorMap tmV16, SpanTileParams p) {
     using C = TCfg<D>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         }
         for (int i = 0; i < PLANS; ++i) {
             mbar_init(&plan_full[i], 1);
-            mbar_init(&plan_empty[i], 9);  // the issuing warp and the softmax warps
+            mbar_init(&plan_empty[i], 10);  // the loading, issuing and softmax warps
         }
         mbar_init(drain, 1);
         fence_barrier_init();
@@ -253,6 +258,11 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
+    // Registers: the block has 3 x 128 x 168; the first four warps keep 104 each
+    // thread and the softmax groups take 200 (104 + 2 x 200 = 3 x 168), which
+    // holds a row of 128 scores without spills.
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0 && lane == 0) {
         // ------------------------------------------------ TMA producer
         // Loads of an item's tiles start as soon as the items before it have
@@ -261,15 +271,12 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         uint32_t g = 0, q_loads[2] = {0, 0};
         uint32_t issued_k = 0, issued_v = 0;
         bool failed = false;
-        for (uint32_t i = 0, item; (item = item_at(i)) < p.items && !failed; ++i) {
-            if (!mbar_wait(&plan_empty[i % PLANS], ((i / PLANS) & 1) ^ 1)) {
+        for (uint32_t i = 0; item_at(i) < p.items && !failed; ++i) {
+            if (!mbar_wait(&plan_full[i % PLANS], (i / PLANS) & 1)) {
                 failed = true;
                 break;
             }
-            TileItem it;
-            it.set(p, item);
-            plans[i % PLANS] = it;
-            mbar_arrive(&plan_full[i % PLANS]);
+            const TileItem& it = plans[i % PLANS];
             const int32_t k_b = p.shared_keys || p.k_batch_bcast ? 0 : (int32_t)it.unit_b;
             const int32_t v_b = p.shared_keys || p.v_batch_bcast ? 0 : (int32_t)it.unit_b;
 #pragma unroll
@@ -287,25 +294,38 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             }
             for (uint32_t j = 0; j < it.n_kv && !failed; ++j, ++g) {
                 const uint32_t s = g % C::STAGES, ph = ((g / C::STAGES) & 1) ^ 1;
-                const int32_t key = (int32_t)(it.key_tile(j) * TK);
+                const uint32_t v0 = (it.j0 + j) * TK;  // virtual tile's first key
+                const bool border = v0 < it.s16 && v0 + TK > it.s16;
+                const int32_t key = (int32_t)(v0 < it.s16 ? v0 : v0 - it.s16 + it.lo);
+                auto load = [&](unsigned char* dst, const CUtensorMap* tm, const CUtensorMap* tm16, int32_t batch, uint64_t* bar) {
+                    mbar_arrive_expect_tx(bar, C::K_BYTES);
+                    for (int b = 0; b < C::BOXES; ++b) {
+                        if (!border) {
+                            tma_load_4d(dst + b * (TK * 128), tm, b * 64, key, (int32_t)it.kv_head, batch, bar);
+                            continue;
+                        }
+                        for (uint32_t r = 0; r < TK; r += 16) {
+                            const uint32_t v = v0 + r;
+                            tma_load_4d(dst + b * (TK * 128) + r * 128, tm16, b * 64, (int32_t)(v < it.s16 ? v : v - it.s16 + it.lo),
+                                        (int32_t)it.kv_head, batch, bar);
+                        }
+                    }
+                };
                 unsigned char* kd = sKV + s * C::STAGE_BYTES;
                 if (!mbar_wait(&k_empty[s], ph)) {
                     failed = true;
                     break;
                 }
-                mbar_arrive_expect_tx(&k_full[s], C::K_BYTES);
-                for (int b = 0; b < C::BOXES; ++b)
-                    tma_load_4d(kd + b * (TK * 128), &tmK, b * 64, key, (int32_t)it.kv_head, k_b, &k_full[s]);
+                load(kd, &tmK, &tmK16, k_b, &k_full[s]);
                 ++issued_k;
                 if (!mbar_wait(&v_empty[s], ph)) {
                     failed = true;
                     break;
                 }
-                mbar_arrive_expect_tx(&v_full[s], C::K_BYTES);
-                for (int b = 0; b < C::BOXES; ++b)
-                    tma_load_4d(kd + C::K_BYTES + b * (TK * 128), &tmV, b * 64, key, (int32_t)it.kv_head, v_b, &v_full[s]);
+                load(kd + C::K_BYTES, &tmV, &tmV16, v_b, &v_full[s]);
                 ++issued_v;
             }
+            mbar_arrive(&plan_empty[i % PLANS]);
         }
         // the copies still in flight land (bounded) before the block ends
         if (failed) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
@@ -315,6 +335,16 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             (void)mbar_wait(&v_full[j % C::STAGES], (j / C::STAGES) & 1);
         for (int t = 0; t < 2 && failed; ++t)
             if (q_loads[t]) (void)mbar_wait(&q_full[t], (q_loads[t] - 1) & 1);
+    } else if (warp == 2 && lane == 0) {
+        // ------------------------------------------------ planner
+        for (uint32_t i = 0, item; (item = item_at(i)) < p.items; ++i) {
+            if (!mbar_wait(&plan_empty[i % PLANS], ((i / PLANS) & 1) ^ 1)) {
+                atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
+                break;
+            }
+            plans[i % PLANS].set(p, item);
+            mbar_arrive(&plan_full[i % PLANS]);
+        }
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         const uint32_t idesc_s = f16_idesc(p.fmt, TQ, TK);
@@ -326,9 +356,9 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         uint32_t g = 0, taken[2] = {0, 0}, outs[2] = {0, 0};
         for (uint32_t n = 0; item_at(n) < p.items; ++n) {
             if (!(ok = ok && wait(&plan_full[n % PLANS], (n / PLANS) & 1))) break;
-            const TileItem it = plans[n % PLANS];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&plan_empty[n % PLANS]);
+            const TileItem& it = plans[n % PLANS];
+            const uint32_t n_kv = it.n_kv, n_t[2] = {it.n_t[0], it.n_t[1]}, near[2] = {it.near[0], it.near[1]},
+                           far[2] = {it.far[0], it.far[1]};
             // left: S_t still to come in this item
             auto issue_s = [&](int t, uint32_t j, uint32_t left) -> bool {
                 const uint32_t s = (g + j) % C::STAGES;
@@ -358,7 +388,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 umma_f16_ts_warp(d, a, vd, idesc_o, i != 0);
 #pragma unroll
                 for (int k = 1; k < TK / 16; ++k) umma_f16_ts_warp(d, a + k * 8, desc_add(vd, k * 16 * 128), idesc_o, 1u);
-                if (i + 1 == it.n_t[t]) {
+                if (i + 1 == n_t[t]) {
                     umma_commit_warp(&o_done[t]);
                     ++outs[t];
                 }
@@ -368,18 +398,18 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             uint32_t at[2], done[2] = {0, 0};
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                at[t] = it.n_t[t] ? it.next_seen(t, 0) : it.n_kv;
-                if (!ok || at[t] >= it.n_kv) continue;
-                ok = wait(&q_full[t], outs[t] & 1) && issue_s(t, at[t], it.n_t[t] - 1);
+                at[t] = n_t[t] ? (near[t] ? 0 : far[t]) : n_kv;
+                if (!ok || at[t] >= n_kv) continue;
+                ok = wait(&q_full[t], outs[t] & 1) && issue_s(t, at[t], n_t[t] - 1);
             }
-            if (ok && it.n_kv > 0) umma_commit_warp(&k_empty[g % C::STAGES]);  // the first K consumed by every S of it
-            for (uint32_t j = 0; ok && j < it.n_kv; ++j) {
+            if (ok && n_kv > 0) umma_commit_warp(&k_empty[g % C::STAGES]);  // the first K consumed by every S of it
+            for (uint32_t j = 0; ok && j < n_kv; ++j) {
                 const uint32_t s = (g + j) % C::STAGES;
                 ok = wait(&v_full[s], ((g + j) / C::STAGES) & 1);
-                const int64_t key0 = (int64_t)it.key_tile(j) * TK;
-                if (ok && p.lengths && !p.shared_keys && key0 + TK > it.filled) {
-                    // value rows past the filled keys: zeros
-                    const uint32_t from = (uint32_t)(it.filled - key0);
+                if (ok && p.lengths && j + 1 == n_kv && it.filled + it.shift() < (int64_t)(it.j0 + n_kv) * TK) {
+                    // value rows past the filled keys (in the last tile, if any): zeros
+                    const int64_t live = it.filled + it.shift() - (int64_t)(it.j0 + j) * TK;
+                    const uint32_t from = (uint32_t)max(live, (int64_t)0);
                     unsigned char* v = sKV + s * C::STAGE_BYTES + C::K_BYTES;
                     for (int b = 0; b < C::BOXES; ++b)
                         for (uint32_t o = from * 128 + lane * 16; o < TK * 128; o += 512)
@@ -392,53 +422,57 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                     if (!ok || at[t] != j) continue;
                     ok = issue_pv(t, j, done[t]);
                     ++done[t];
-                    at[t] = done[t] < it.n_t[t] ? it.next_seen(t, j + 1) : it.n_kv;
-                    if (ok && at[t] < it.n_kv) ok = issue_s(t, at[t], it.n_t[t] - done[t] - 1);
+                    at[t] = done[t] < n_t[t] ? TileItem::after(j, near[t], far[t]) : n_kv;
+                    if (ok && at[t] < n_kv) ok = issue_s(t, at[t], n_t[t] - done[t] - 1);
                 }
                 // V(j) is free once every PV(j) has completed, K(j + 1) once
                 // every S(j + 1) has (each was issued by now)
                 if (ok) umma_commit_warp(&v_empty[s]);
-                if (ok && j + 1 < it.n_kv) umma_commit_warp(&k_empty[(g + j + 1) % C::STAGES]);
+                if (ok && j + 1 < n_kv) umma_commit_warp(&k_empty[(g + j + 1) % C::STAGES]);
             }
-            g += it.n_kv;
+            g += n_kv;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&plan_empty[n % PLANS]);
         }
         if (!ok && lane == 0) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
         umma_commit_warp(drain);
         (void)wait(drain, 0);
-    } else if (warp >= 2) {
+    }
+    } else {
         // ------------------------------------------------ softmax / epilogue
-        const int t = (warp - 2) / 4;
-        const int quarter = warp & 3;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int t = (warp - 4) / 4, quarter = warp & 3;
         const uint32_t row = (uint32_t)(quarter * 32 + lane);
         const uint32_t tm_s = tmem + ((uint32_t)(quarter * 32) << 16) + C::s_col(t);
         const uint32_t tm_o = tmem + ((uint32_t)(quarter * 32) << 16) + C::o_col(t);
         const float NEG = -__int_as_float(0x7f800000);
         const float sl = p.scale_log2;
+        // the row's place in the box: head, query and sequence, 8 bits each
+        const uint32_t place = row % p.GB | row / p.GB % p.LB << 8 | row / (p.GB * p.LB) << 16;
         uint32_t steps = 0, outs = 0;  // S_t taken, items with any, over all items
         bool ok = true;
         for (uint32_t turn = 0; item_at(turn) < p.items; ++turn) {
-            if (!(ok = ok && __all_sync(0xffffffffu, mbar_wait(&plan_full[turn % PLANS], (turn / PLANS) & 1)))) {
+            if (!(ok = __all_sync(0xffffffffu, ok && mbar_wait(&plan_full[turn % PLANS], (turn / PLANS) & 1)))) {
                 atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
                 break;
             }
-            // this tile's key tiles: [0, ns) and then from a0 on, n in all from kt
             const TileItem& it = plans[turn % PLANS];
             const uint32_t n = it.n_t[t];
-            uint32_t kt;
-            int32_t high, low;
+            uint32_t j = it.near[t] ? 0 : it.far[t];  // this tile's key tiles, n in all
+            // virtual keys of this row: below vsink, and [vlow, vhigh]
+            int32_t vsink, vlow, vhigh;
             {
-                // keys of this row: [0, sinks) and [low, high]
-                const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1
-                                                  : it.base + (int64_t)(it.l0[t] + row / p.GB % p.LB);
-                high = (int32_t)max((int64_t)-1, min(pos, it.filled - 1));
-                low = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
-                kt = n ? it.key_tile(it.next_seen(t, 0)) : 0;
+                const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1 : it.base + (int64_t)(it.l0[t] + (place >> 8 & 0xffu));
+                const int32_t high = (int32_t)max((int64_t)-1, min(pos, it.filled - 1));
+                vsink = p.shared_keys ? 0 : min(p.sinks32, high + 1);
+                vlow = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x3fffffff, pos - p.window + 1)) + it.shift();
+                vhigh = high + it.shift();
             }
             float m_used = NEG;  // running max (log2 units)
             float lsum = 0.0f;
             for (uint32_t i = 0; i < n && ok; ++i, ++steps) {
-                const int32_t key0 = (int32_t)(kt * TK);
-                kt = kt + 1 < it.plan.ns[t] ? kt + 1 : max(kt + 1, it.plan.a0[t]);
+                const int32_t v0 = (int32_t)((it.j0 + j) * TK);
+                j = TileItem::after(j, it.near[t], it.far[t]);
                 // Wait outcomes are made warp-uniform: tcgen05.ld/st are .sync.aligned.
                 if (!__all_sync(0xffffffffu, mbar_wait(&s_full[t], steps & 1))) {
                     ok = false;
@@ -449,34 +483,24 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 {
                     uint32_t r[TK];
 #pragma unroll
-                    for (int c = 0; c < TK / 32; ++c)
-                        tmem_ld32(tm_s + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[c * 32]));
+                    for (int c = 0; c < TK; c += 32) tmem_ld32(tm_s + c, *reinterpret_cast<uint32_t(*)[32]>(&r[c]));
                     tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < TK; ++e) x[e] = __uint_as_float(r[e]);
                 }
                 // Hidden keys are masked in the raw scores, only in the tiles that
                 // hold some: past the row's position or the filled keys, or between
-                // the first keys and the window.  A warp's rows are neighbours, so
-                // most 32-key chunks are seen, or hidden, by all of them.
-                if (__any_sync(0xffffffffu, key0 + TK - 1 > high || (key0 < low && key0 + TK > p.sinks32))) {
-                    int32_t lim = high + 1 - key0, lo = low - key0;
-                    const int32_t sk = p.sinks32 - key0;
-                    if (lo > 0 && sk > 0) {
-                        if (lo >= TK) {
-                            lim = min(lim, sk), lo = 0;  // first keys only
-                        } else {  // first keys and the window in one tile
-#pragma unroll
-                            for (int e = 0; e < TK; ++e) x[e] = e < sk || e >= lo ? x[e] : p.hidden;
-                            lo = 0;
-                        }
-                    }
-                    const int32_t lim0 = __reduce_min_sync(0xffffffffu, lim), lo1 = __reduce_max_sync(0xffffffffu, lo);
+                // the first keys and the window.  A word of bits per 32 keys says
+                // which are seen; a warp's rows are neighbours, so most words are
+                // whole in all of them.
+                if (__any_sync(0xffffffffu, v0 + TK - 1 > vhigh || v0 < vlow)) {
+                    auto below = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };
 #pragma unroll
                     for (int c = 0; c < TK; c += 32) {
-                        if (lim0 < c + 32 || lo1 > c) {
+                        const uint32_t seen = below(vsink - v0 - c) | (below(vhigh + 1 - v0 - c) & ~below(vlow - v0 - c));
+                        if (__any_sync(0xffffffffu, seen != 0xffffffffu)) {
 #pragma unroll
-                            for (int e = c; e < c + 32; ++e) x[e] = e >= lo && e < lim ? x[e] : p.hidden;
+                            for (int e = 0; e < 32; ++e) x[c + e] = seen & (1u << e) ? x[c + e] : p.hidden;
                         }
                     }
                 }
@@ -484,10 +508,10 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
 #pragma unroll
                     for (int e = 0; e < TK; ++e) x[e] = x[e] == NEG ? NEG : 0.0f * x[e];
                 }
-                const bool use_min = sl < 0.0f;
-                // Four chains of three-input extremes: 64 instructions per row.
+                // Four chains of three-input extremes of the raw scores (the
+                // logits' maximum is the minimum under a negative scale).
                 float mx[4] = {x[0], x[1], x[2], x[3]};
-                if (use_min) {
+                if (sl < 0.0f) {
 #pragma unroll
                     for (int e = 4; e < TK - 4; e += 8)
 #pragma unroll
@@ -502,14 +526,14 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                     mx[0] = max3n(mx[0], x[TK - 4], x[TK - 3]);
                     mx[1] = max3n(mx[1], x[TK - 2], x[TK - 1]);
                 }
-                float mt = use_min ? min3n(min3n(mx[0], mx[1], mx[2]), mx[3], mx[3])
-                                   : max3n(max3n(mx[0], mx[1], mx[2]), mx[3], mx[3]);
-                if (sl != 0.0f) mt *= sl;  // raw extreme -> logit maximum
+                const float mul = sl == 0.0f ? 1.0f : sl;
+                float mt = (sl < 0.0f ? min3n(min3n(mx[0], mx[1], mx[2]), mx[3], mx[3])
+                                      : max3n(max3n(mx[0], mx[1], mx[2]), mx[3], mx[3])) * mul;
                 float alpha = 1.0f;
                 bool rescale = false;
                 if (mt > m_used + 8.0f) {
                     alpha = m_used == NEG ? 0.0f : ex2(m_used - mt);
-                    rescale = i > 0 && lsum > 0.0f;
+                    rescale = i > 0 && m_used != NEG;
                     m_used = mt;
                 }
                 const float ref = m_used == NEG ? 0.0f : m_used + p.shift;
@@ -517,7 +541,6 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 // Packed pairs overwrite the scores they came from, so P needs no
                 // registers of its own; one pair in eight takes the polynomial.
                 uint32_t* xb = reinterpret_cast<uint32_t*>(x);
-                const float mul = sl == 0.0f ? 1.0f : sl;
                 const float2 sl2 = make_float2(mul, mul), nb2 = make_float2(-ref, -ref);
 #pragma unroll
                 for (int c = 0; c < TK / 32; ++c) {
@@ -531,6 +554,8 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                     tmem_st16(tm_s + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&xb[c * 32]));
                 }
                 if (__any_sync(0xffffffffu, rescale)) {
+                    // O_t is quiescent: S_t of this step completed after PV_t
+                    // of the last, and PV_t of this one waits for the arrivals.
                     const float f = rescale ? alpha : 1.0f;
 #pragma unroll 1
                     for (int c = 0; c < D / 32; ++c) {
@@ -559,14 +584,15 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             if (!ok) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
             tc_fence_after();
             const bool load = ok && n > 0;
-            const uint32_t head = it.head0 + row % p.GB, l = it.l0[t] + row / p.GB % p.LB, b = it.b0[t] + row / (p.GB * p.LB);
+            const uint32_t head = it.head0 + (place & 0xffu), l = it.l0[t] + (place >> 8 & 0xffu), b = it.b0[t] + (place >> 16);
             const bool valid = it.real[t] && row < p.rows && l < p.L && b < p.B;
             float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
             unsigned char* dst;  // this row's next 32 columns
             if (p.part) {
                 inv = 1.0f;
                 float* rec = p.part + ((((uint64_t)b * p.H + head) * p.L + l) * p.part_stride + p.part_first + it.split) * REC<D>;
-                if (valid) *reinterpret_cast<float2*>(rec) = make_float2(m_used == NEG ? 0.0f : m_used + p.shift, load ? lsum : 0.0f);
+                if (valid)
+                    *reinterpret_cast<float2*>(rec) = make_float2(m_used == NEG ? 0.0f : m_used + p.shift, load ? lsum : 0.0f);
                 dst = reinterpret_cast<unsigned char*>(rec + 4);
             } else {
                 const uint64_t at = (uint64_t)b * p.o_sb + (uint64_t)head * p.o_sh + (uint64_t)l * p.o_sl;
@@ -1200,7 +1226,7 @@ TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared) {
     g.units = a.H / g.GB * (shared ? 1 : a.B);
     uint64_t keys = ((shared ? s.prefix_keys : a.Lk) + TK - 1) / TK;  // tiles that a CTA walks at most
     if (!shared)
-        keys = std::min(keys, (std::min(s.sinks, a.Lk) + TK - 1) / TK + (std::min(s.window, a.Lk) + 2 * g.LB + TK - 1) / TK + 1);
+        keys = std::min(keys, (std::min(s.sinks, a.Lk) + std::min(s.window, a.Lk) + 2 * g.LB + 16 + TK - 1) / TK);
     const uint64_t sms = (uint64_t)sm_count();
     auto ranges = [&](uint64_t ctas) -> uint64_t {
         if (ctas >= sms || keys < 4) return 1;
@@ -1262,9 +1288,9 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
     p.part = part, p.part_stride = part_stride, p.part_first = part_first;
     p.out = a.op, p.out_low = s.base.out_low;
     p.o_sb = a.o.s_batch, p.o_sh = a.o.s_head, p.o_sl = a.o.s_row;
-    CUtensorMap tq, tk, tv;
+    CUtensorMap tq, tk, tv, tk16{}, tv16{};
     const uint32_t dt = a.fmt ? FB_BF16 : FB_F16;
-    const uint32_t qbox[3] = {p.GB, p.LB, p.NB}, kbox[3] = {TK, 1, 1};
+    const uint32_t qbox[3] = {p.GB, p.LB, p.NB}, kbox[3] = {TK, 1, 1}, kbox16[3] = {16, 1, 1};
     if (!span_map(&tq, a.qp, dt, D, {a.H, a.L, a.B}, {a.q.s_head, a.q.s_row, a.q.s_batch}, qbox, true)) return FB_ERR_UNSUPPORTED;
     if (shared) {
         const uint16_t* pk = static_cast<const uint16_t*>(s.pk) + s.pk_offset;
@@ -1274,7 +1300,9 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
             return FB_ERR_UNSUPPORTED;
     } else {
         if (!span_map(&tk, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox, true) ||
-            !span_map(&tv, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox, true))
+            !span_map(&tv, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox, true) ||
+            !span_map(&tk16, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox16, true) ||
+            !span_map(&tv16, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox16, true))
             return FB_ERR_UNSUPPORTED;
     }
     auto runs32 = [](uint64_t n, uint64_t stride) { return n <= 1 || stride % 16 == 0; };
@@ -1285,7 +1313,7 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
     const uint64_t grid = std::min<uint64_t>(items, (uint64_t)sm_count());
     if (cudaFuncSetAttribute(span_tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
         return launch_status("shared-memory attribute");
-    launch_after(span_tile_kernel<D>, (unsigned)grid, C::THREADS, C::SMEM, overlap, st, tq, tk, tv, p);
+    launch_after(span_tile_kernel<D>, (unsigned)grid, C::THREADS, C::SMEM, overlap, st, tq, tk, tv, tk16, tv16, p);
     count_launch(kernel_name("span_tile_kernel", {D, shared ? 1 : 0}).c_str());
     return launch_status("kernel launch");
 }
