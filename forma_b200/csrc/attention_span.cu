@@ -34,12 +34,10 @@ __device__ __forceinline__ Reach reach(int64_t pa, int64_t pb, int64_t n, int64_
     return r;
 }
 
-// What a key range leaves for a query row: {base, l, -, -, O[D]}, O = sum P V
-// and l = sum P unnormalised, base the log2 reference of P's exponentials
+// What a key range leaves for a query row: O[D] = sum P V unnormalised, and a
+// head {base, l}, l = sum P, base the log2 reference of P's exponentials
 // (l = 0: no key seen).  Joined, with M the largest base of those with l > 0:
 // O = sum O_r 2^(base_r - M) / sum l_r 2^(base_r - M).
-template <int D>
-constexpr int REC = D + 4;
 
 // --------------------------------------------------------- tcgen05 tiles
 //
@@ -60,8 +58,8 @@ constexpr int REC = D + 4;
 //               memory first (a weight of 0 does not hide a NaN there)
 //   warps 4-11  softmax, one query row per thread: lazy running maximum
 //               (raised, and O rescaled, only past 2^8), P over S in TMEM; at
-//               an item's end O / l, or a record, straight from registers, a
-//               row's 32 bytes per store
+//               an item's end O / l, or a record, through shared memory and
+//               TMA stores of 128 bytes per row
 // P is handed over in two halves, so that the products of its first 64 keys run
 // while the others' exponentials are taken (with the sums below, 164 -> 149 us
 // for 8192 queries, window 1024, 32/8 heads, D = 128).
@@ -83,11 +81,12 @@ struct SpanTileParams {
     float hidden;                  // what a hidden key's raw score becomes: its logit is -inf whatever the scale's sign
     int32_t sinks32;               // sinks, at most 2^31 - 1
     uint32_t splits;               // key ranges of a pair
-    float* part;                   // records: ((b * H + h) * L + l) * part_stride + part_first + split
-    uint32_t part_stride, part_first;
-    void* out;                     // part == null: output rows
-    uint32_t out_low, wide;        // wide: rows of whole, aligned 32-byte runs
-    uint64_t o_sb, o_sh, o_sl;
+    // Output: through tmO, a 5-D map {D, records, heads, queries, batch}; for
+    // records (heads not null) the one at index first + split of each row, its
+    // head at ((b * H + h) * L + l) * stride + first + split.
+    float2* heads;
+    uint32_t stride, first;
+    uint32_t out_low;              // 16-bit output: FB_BF16 / FB_F16
 };
 
 template <int D>
@@ -98,7 +97,8 @@ struct TCfg {
     static constexpr int K_BYTES = TK * D * 2;
     static constexpr int STAGE_BYTES = 2 * K_BYTES;
     static constexpr int STAGES = D == 64 ? 4 : 2;
-    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + 384;
+    static constexpr int OUT_BYTES = TQ * 128;     // a tile's rows, 128 bytes of each on their way out
+    static constexpr int SMEM = 1024 + 2 * Q_BYTES + STAGES * STAGE_BYTES + 2 * OUT_BYTES + 384;
     static __device__ __forceinline__ uint32_t s_col(int t) { return (uint32_t)(t * TK); }
     static __device__ __forceinline__ uint32_t o_col(int t) { return (uint32_t)(2 * TK + t * 128); }
 };
@@ -188,9 +188,24 @@ struct TileItem {
     }
 };
 
-__device__ __forceinline__ void store32(void* dst, const uint32_t (&r)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+// Whether `v` holds in all 128 threads of named barrier `id`.
+__device__ __forceinline__ bool tile_all(int id, bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred q, a;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred a, %2, 128, q;\n\tselp.u32 %0, 1, 0, a;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "r"(id)
+        : "memory");
+    return r != 0;
+}
+
+// TMA tensor store shared -> global through a 5-D map; elements outside the
+// map's extents are not written.
+__device__ __forceinline__ void tma_store_5d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w, int32_t v,
+                                             const void* src) {
+    asm volatile("cp.async.bulk.tensor.5d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4, %5}], [%6];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(src))
                  : "memory");
 }
 
@@ -199,13 +214,15 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                                                                        const __grid_constant__ CUtensorMap tmK,
                                                                        const __grid_constant__ CUtensorMap tmV,
                                                                        const __grid_constant__ CUtensorMap tmK16,
-                                                                       const __grid_constant__ CUtensorMap tmV16, SpanTileParams p) {
+                                                                       const __grid_constant__ CUtensorMap tmV16,
+                                                                       const __grid_constant__ CUtensorMap tmO, SpanTileParams p) {
     using C = TCfg<D>;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* sQ = smem;
     unsigned char* sKV = sQ + 2 * C::Q_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::STAGES * C::STAGE_BYTES);
+    unsigned char* sOut = sKV + C::STAGES * C::STAGE_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sOut + 2 * C::OUT_BYTES);
     uint64_t* k_full = bars;
     uint64_t* k_empty = k_full + C::STAGES;
     uint64_t* v_full = k_empty + C::STAGES;
@@ -462,7 +479,8 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         uint32_t steps = 0, outs = 0;  // S_t taken, items with any, over all items
         bool ok = true;
         for (uint32_t turn = 0; item_at(turn) < p.items; ++turn) {
-            if (!(ok = __all_sync(0xffffffffu, ok && mbar_wait(&plan_full[turn % PLANS], (turn / PLANS) & 1)))) {
+            // (the tile's four warps go on or none does: they meet at barriers)
+            if (!(ok = tile_all(1 + t, ok && mbar_wait(&plan_full[turn % PLANS], (turn / PLANS) & 1)))) {
                 atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
                 break;
             }
@@ -596,61 +614,73 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             if (!ok) atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
             tc_fence_after();
             const bool load = ok && n > 0;
-            const uint32_t head = it.head0 + (place & 0xffu), l = it.l0[t] + (place >> 8 & 0xffu), b = it.b0[t] + (place >> 16);
-            const bool valid = it.real[t] && row < p.rows && l < p.L && b < p.B;
+            const bool real = it.real[t];
+            const uint32_t head0 = it.head0, l0 = it.l0[t], b0 = it.b0[t], record = p.first + it.split;
             float inv = load && (lsum > 0.0f || lsum != lsum) ? 1.0f / lsum : 0.0f;
-            unsigned char* dst;  // this row's next 32 columns
-            if (p.part) {
+            if (p.heads) {
                 inv = 1.0f;
-                float* rec = p.part + ((((uint64_t)b * p.H + head) * p.L + l) * p.part_stride + p.part_first + it.split) * REC<D>;
-                if (valid)
-                    *reinterpret_cast<float2*>(rec) = make_float2(m_used == NEG ? 0.0f : m_used + p.shift, load ? lsum : 0.0f);
-                dst = reinterpret_cast<unsigned char*>(rec + 4);
-            } else {
-                const uint64_t at = (uint64_t)b * p.o_sb + (uint64_t)head * p.o_sh + (uint64_t)l * p.o_sl;
-                dst = static_cast<unsigned char*>(p.out) + at * (p.out_low ? 2 : 4);
+                const uint32_t head = head0 + (place & 0xffu), l = l0 + (place >> 8 & 0xffu), b = b0 + (place >> 16);
+                if (real && row < p.rows && l < p.L && b < p.B)
+                    p.heads[(((uint64_t)b * p.H + head) * p.L + l) * p.stride + record] =
+                        make_float2(m_used == NEG ? 0.0f : m_used + p.shift, load ? lsum : 0.0f);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&plan_empty[turn % PLANS]);  // the plan is no longer needed
-            const bool low_rows = !p.part && p.out_low;
+            // 128 bytes of every row at a time: staged in shared memory under
+            // the map's swizzle, written by one TMA store per tile.  (Stores
+            // from registers, one row per lane, hold the load/store unit for a
+            // line per lane: 6k to 9k cycles per tile against 2k.)
+            const uint32_t step = p.out_low ? 64 : 32;  // columns
+            unsigned char* stage = sOut + t * C::OUT_BYTES;
+            const uint32_t swz = row & 7u;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                if (load) {
-                    tmem_ld32(tm_o + c * 32, r);
-                    tmem_wait_ld();
-                } else {
+            for (uint32_t c = 0; c < (uint32_t)D; c += step) {
+                // the staged bytes of the store before this one have been read
+                if (threadIdx.x % 128 == 0) bulk_wait_read_all();
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) r[e] = 0u;
+                for (int h = 0; h < 2; ++h) {
+                    if (h * 32 >= (int)step) break;
+                    uint32_t r[32];
+                    if (load) {
+                        tmem_ld32(tm_o + c + h * 32, r);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) r[e] = 0u;
+                    }
+                    if (p.out_low) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                w[k] = pack2(__uint_as_float(r[8 * e + 2 * k]) * inv, __uint_as_float(r[8 * e + 2 * k + 1]) * inv, FMT);
+                            *reinterpret_cast<uint4*>(stage + row * 128 + (((uint32_t)(h * 4 + e) ^ swz) * 16)) =
+                                make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            *reinterpret_cast<float4*>(stage + row * 128 + (((uint32_t)e ^ swz) * 16)) =
+                                make_float4(__uint_as_float(r[4 * e]) * inv, __uint_as_float(r[4 * e + 1]) * inv,
+                                            __uint_as_float(r[4 * e + 2]) * inv, __uint_as_float(r[4 * e + 3]) * inv);
+                    }
                 }
-                if (c == D / 32 - 1 && load) {
+                if (c + step == (uint32_t)D && load) {
                     tc_fence_before();
                     mbar_arrive(&o_free[t]);  // O_t is out of TMEM
                 }
-                if (valid && low_rows) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            w[e] = pack2(__uint_as_float(r[h * 16 + 2 * e]) * inv, __uint_as_float(r[h * 16 + 2 * e + 1]) * inv, FMT);
-                        if (p.wide) {
-                            store32(dst + c * 64 + h * 32, w);
-                        } else {
-                            *reinterpret_cast<uint4*>(dst + c * 64 + h * 32) = make_uint4(w[0], w[1], w[2], w[3]);
-                            *reinterpret_cast<uint4*>(dst + c * 64 + h * 32 + 16) = make_uint4(w[4], w[5], w[6], w[7]);
-                        }
-                    }
-                } else if (valid) {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4*>(dst + c * 128 + e * 4) =
-                            make_float4(__uint_as_float(r[e]) * inv, __uint_as_float(r[e + 1]) * inv,
-                                        __uint_as_float(r[e + 2]) * inv, __uint_as_float(r[e + 3]) * inv);
+                fence_proxy_async_smem();  // the staged rows are visible to the TMA store
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + t) : "memory");
+                if (threadIdx.x % 128 == 0 && real) {
+                    tma_store_5d(&tmO, (int32_t)c, (int32_t)record, (int32_t)head0, (int32_t)l0, (int32_t)b0, stage);
+                    bulk_commit_group();
                 }
             }
             if (n > 0) ++outs;
         }
+        if (threadIdx.x % 128 == 0) bulk_wait_read_all();  // shared memory stays valid until the stores have read it
         tc_fence_before();
     }
     __syncthreads();
@@ -669,13 +699,13 @@ struct RowPiece {  // the D / 32 columns lane * D / 32 .. of one row
     float v[N];
 };
 template <int D>
-__device__ __forceinline__ RowPiece<D> load_piece(const float* rec, uint32_t lane) {
+__device__ __forceinline__ RowPiece<D> load_piece(const float* row, uint32_t lane) {
     RowPiece<D> r;
     if constexpr (D == 128) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(rec + 4) + lane);
+        const float4 f = __ldcg(reinterpret_cast<const float4*>(row) + lane);
         r.v[0] = f.x, r.v[1] = f.y, r.v[2] = f.z, r.v[3] = f.w;
     } else {
-        const float2 f = __ldcg(reinterpret_cast<const float2*>(rec + 4) + lane);
+        const float2 f = __ldcg(reinterpret_cast<const float2*>(row) + lane);
         r.v[0] = f.x, r.v[1] = f.y;
     }
     return r;
@@ -696,46 +726,40 @@ __device__ __forceinline__ void store_piece(void* out, uint32_t out_low, uint64_
     }
 }
 
-// A warp joins the records rec(0) .. rec(n - 1) of one row in order, after the
-// state {M, L, o} it has (L = 0, M = -inf: none).  Headers are read by the
-// lanes in parallel, then the rows with eight loads in flight.
-template <int D, typename Rec>
-__device__ __forceinline__ void join_records(uint32_t n, Rec rec, float& M, float& L, float (&o)[D / 32]) {
+// A warp joins the records 0 .. n - 1 of one row, in order, to the state
+// {M, L, o} it has (L = 0: nothing yet); head(i) and row(i) are where record i
+// lies.  Eight records at a time, all their loads in flight together.
+template <int D, typename Head, typename Row>
+__device__ __forceinline__ void join_records(uint32_t n, Head head, Row row, float& M, float& L, float (&o)[D / 32]) {
     const uint32_t lane = threadIdx.x & 31;
     const float NEG = -__int_as_float(0x7f800000);
-    float top = M;
-    for (uint32_t i = lane; i < n; i += 32) {
-        const float2 h = __ldcg(reinterpret_cast<const float2*>(rec(i)));
-        if (h.y != 0.0f) top = fmaxf(top, h.x);
-    }
-#pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    if (top == NEG) return;
-    const float keep = L == 0.0f ? 0.0f : exp2f(M - top);
-    L *= keep;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] *= keep;
-    M = top;
-    for (uint32_t i0 = 0; i0 < n; i0 += 32) {
+    for (uint32_t i0 = 0; i0 < n; i0 += 8) {
+        const uint32_t m = min(n - i0, 8u);
         float2 h = make_float2(0.0f, 0.0f);
-        if (i0 + lane < n) h = __ldcg(reinterpret_cast<const float2*>(rec(i0 + lane)));
-        const float w = h.y == 0.0f ? 0.0f : exp2f(h.x - M);
-        const float lw = h.y * w;
-        const uint32_t m = min(n - i0, 32u);
-        for (uint32_t c = 0; c < m; c += 8) {
-            RowPiece<D> r[8];
+        if (lane < m) h = __ldcg(head(i0 + lane));
+        RowPiece<D> r[8];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                if (c + e < m) r[e] = load_piece<D>(rec(i0 + c + e), lane);
+        for (uint32_t e = 0; e < 8; ++e)
+            if (e < m) r[e] = load_piece<D>(row(i0 + e), lane);
+        float top = h.y == 0.0f ? NEG : h.x;
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) {
-                if (c + e >= m) break;
-                const float wr = __shfl_sync(0xffffffffu, w, c + e);
-                L += __shfl_sync(0xffffffffu, lw, c + e);
-                if (wr == 0.0f) continue;  // nothing seen, or underflow: O is not multiplied by 0
+        for (int x = 4; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(__shfl_sync(0xffffffffu, top, 0), L == 0.0f ? NEG : M);
+        if (top == NEG) continue;
+        const float keep = L == 0.0f ? 0.0f : exp2f(M - top);
+        L *= keep;
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[i] = fmaf(r[e].v[i], wr, o[i]);
-            }
+        for (int i = 0; i < D / 32; ++i) o[i] *= keep;
+        M = top;
+        const float w = h.y == 0.0f ? 0.0f : exp2f(h.x - M), lw = h.y * w;
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+            if (e >= m) break;
+            const float we = __shfl_sync(0xffffffffu, w, e);
+            L += __shfl_sync(0xffffffffu, lw, e);
+            if (we == 0.0f) continue;  // nothing seen, or underflow: O is not multiplied by 0
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) o[i] = fmaf(r[e].v[i], we, o[i]);
         }
     }
 }
@@ -743,6 +767,7 @@ __device__ __forceinline__ float inverse(float l) { return l > 0.0f || l != l ? 
 
 // One warp per row.
 struct SpanMergeParams {
+    const float2* heads;
     const float* part;
     uint64_t rows;
     uint32_t count, H, L;
@@ -759,8 +784,9 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
     float M = -__int_as_float(0x7f800000), L = 0.0f, o[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
-    const float* part = p.part + w * p.count * REC<D>;
-    join_records<D>(p.count, [&](uint32_t i) { return part + i * REC<D>; }, M, L, o);
+    const float2* heads = p.heads + w * p.count;
+    const float* part = p.part + w * p.count * D;
+    join_records<D>(p.count, [&](uint32_t i) { return heads + i; }, [&](uint32_t i) { return part + i * D; }, M, L, o);
     const uint64_t q = w % p.L, h = w / p.L % p.H, b = w / p.L / p.H;
     store_piece<D>(p.out, p.out_low, b * p.o_sb + h * p.o_sh + q * p.o_sl, threadIdx.x & 31, o, inverse(L));
 }
@@ -778,7 +804,7 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // of their concatenation, whatever unit borders fall inside, so that ragged
 // lengths and unit counts that do not divide the GPU leave no SM idle.  Each
 // CTA finds its first unit from a block scan over the lengths.  Per unit that
-// a CTA enters, its four warps take a quarter of the keys each through
+// a CTA enters, its two warps take half of the keys each through
 // three-stage cp.async rings and combine in shared memory.  A unit inside one
 // CTA is finished there; otherwise its CTAs leave records and the last to
 // arrive (a counter per unit, reset by it) joins them in CTA order, so results
@@ -786,7 +812,8 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // span_tile_kernel just before, are joined at the same place; the launch
 // overlaps that kernel's end (programmatic dependent launch).
 // Bound: HBM, the visible keys and values once.
-constexpr int DTILE = 64;  // keys: 16 per warp and step
+constexpr int DTILE = 64;  // keys
+constexpr int SPAN_WARPS = 4;
 
 struct SpanDecodeParams {
     const uint16_t* q;
@@ -798,9 +825,12 @@ struct SpanDecodeParams {
     uint64_t length_stride;
     int64_t offset, window, sinks;
     float scale_log2, shift;
-    float* part;          // two records x 16 rows per CTA
+    uint32_t whole_units; // 1: CTA i takes all of unit i
+    float2* part_heads;   // two records x 16 rows per CTA
+    float* part;
     uint32_t* arrived;    // per unit, 0 between launches
-    const float* prefix;  // ((b * H + h) * L + l) * prefix_count + i, or null
+    const float2* prefix_heads;  // records of the shared prefix: ((b * H + h) * L + l) * prefix_count + i, or null
+    const float* prefix;
     uint32_t prefix_count;
     void* out;
     uint32_t out_low;
@@ -833,35 +863,39 @@ struct DCfg {
     static constexpr int CPR = D / 8;            // 16-byte chunks per K / V row
     static constexpr int STAGE = 2 * 16 * CPR;   // chunks per stage: 16 K rows, 16 V rows
     static constexpr int RING = DEC_STAGES * STAGE;
-    static constexpr int SMEM = DEC_WARPS * RING * 16;
-    static_assert(RING * 16 >= (16 * (D + 2) + 16 * REC<D>) * 4, "the combine's records fit a warp's ring");
+    static constexpr int SMEM = SPAN_WARPS * RING * 16;
+    static_assert(RING * 16 >= 16 * (2 * D + 2) * 4, "a warp's rows and the CTA's fit a ring");
 };
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeParams p) {
+__global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecodeParams p) {
     using C = DCfg<D>;
     constexpr int QW = D / 8, KS = D / 16, NJ = D / 8, CPR = C::CPR, STAGE = C::STAGE;
     extern __shared__ uint4 dsm[];
-    __shared__ uint32_t scan[DEC_WARPS], found[2], last;
+    __shared__ uint32_t scan[SPAN_WARPS], found[2], last;
+    __shared__ float2 heads[16];             // the CTA's combined records: heads, and rows in
+    __shared__ float wts[16][SPAN_WARPS];    // the upper part of warp 0's ring
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     uint4* ring = dsm + (size_t)warp * C::RING;
     const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-    // the CTA's combined records: the upper half of warp 0's ring
-    float* cmb = reinterpret_cast<float*>(dsm) + ((16 * (D + 2) + 3) / 4) * 4;
+    float* cmb = reinterpret_cast<float*>(dsm) + 16 * (D + 2);
     const uint32_t R = p.G * p.L;
     const float NEG = -__int_as_float(0x7f800000);
 
     // This CTA's tiles and its first unit.
     uint32_t T, t_begin, b, hkv, tin;
-    if (!p.lengths) {
+    if (p.whole_units) {
+        b = blockIdx.x / p.Hkv, hkv = blockIdx.x % p.Hkv, tin = 0;
+        t_begin = 0, T = unit_keys(p, b).tiles;
+    } else if (!p.lengths) {
         const uint32_t tpu = unit_keys(p, 0).tiles;
         T = p.B * p.Hkv * tpu;
         const uint32_t q = (T + gridDim.x - 1) / gridDim.x;
         t_begin = blockIdx.x * q;
         b = t_begin / (tpu * p.Hkv), hkv = t_begin / tpu % p.Hkv, tin = t_begin % tpu;
     } else {
-        const uint32_t per = (p.B + 32 * DEC_WARPS - 1) / (32 * DEC_WARPS);
+        const uint32_t per = (p.B + 32 * SPAN_WARPS - 1) / (32 * SPAN_WARPS);
         const uint32_t b0 = min(threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
         uint32_t mine = 0;
         for (uint32_t i = b0; i < b1; ++i) mine += unit_keys(p, i).tiles * p.Hkv;
@@ -876,7 +910,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
         uint32_t before = incl - mine;
         T = 0;
 #pragma unroll
-        for (int w = 0; w < DEC_WARPS; ++w) {
+        for (int w = 0; w < SPAN_WARPS; ++w) {
             if (w < warp) before += scan[w];
             T += scan[w];
         }
@@ -896,7 +930,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
         const uint32_t tpu = t_begin < T ? unit_keys(p, b).tiles : 1u;
         hkv = found[1] / tpu, tin = found[1] % tpu;
     }
-    const uint32_t per_cta = (T + gridDim.x - 1) / gridDim.x;
+    const uint32_t per_cta = p.whole_units ? T : (T + gridDim.x - 1) / gridDim.x;
     if (t_begin >= T) return;
     const uint32_t t_end = min(t_begin + per_cta, T);
 
@@ -904,7 +938,7 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
         const UnitKeys u = unit_keys(p, b);
         const uint32_t seg = min(u.tiles - tin, t_end - t);
         const uint32_t v_begin = tin * DTILE, v_end = min((tin + seg) * DTILE, u.count);
-        const uint32_t quarter = ((v_end > v_begin ? v_end - v_begin : 0u) + 16 * DEC_WARPS - 1) / (16 * DEC_WARPS) * 16;
+        const uint32_t quarter = ((v_end > v_begin ? v_end - v_begin : 0u) + 16 * SPAN_WARPS - 1) / (16 * SPAN_WARPS) * 16;
         const uint32_t k_begin = min(v_begin + warp * quarter, v_end), k_end = min(k_begin + quarter, v_end);
         // Q fragments of rows g and g + 8 (zeros past R); row r is query head r / L, query r % L
         uint32_t qa[2][QW];
@@ -929,17 +963,37 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
             }
         }
         const uint32_t skip = u.lo - u.s;
+        // Virtual keys [open, shut) are seen by every row: from the last
+        // query's window on, up to the first query's position.
+        const uint32_t last_low = (uint32_t)max((int64_t)u.lo, min((int64_t)0x7fffffff, u.base + (int64_t)p.L - p.window));
+        const uint32_t open = last_low - skip, shut = (uint32_t)max((int64_t)0, min((int64_t)k_end, u.base + 1 - (int64_t)skip));
         const int32_t sinks = (int32_t)min((int64_t)0x7fffffff, p.sinks);
         const uint16_t* kbase = p.k + (uint64_t)b * p.k_sb + (uint64_t)hkv * p.k_sh;
         const uint16_t* vbase = p.v + (uint64_t)b * p.v_sb + (uint64_t)hkv * p.v_sh;
-        // One stage: virtual keys v0 .. v0 + 15 of K then V, 16 bytes per copy;
-        // keys past the range are zero-filled (source size 0, address in bounds).
+        // One stage: virtual keys v0 .. v0 + 15 of K then V, 16 bytes per copy.
+        // Copy n of a lane is chunk lane % CPR of row lane / CPR + n * RPC.
+        // Stages inside the window and the range step a pointer; the others
+        // number each key, those past the range zero-filled (source size 0,
+        // address in bounds).
+        constexpr int RPC = 32 / CPR, COPIES = 16 / RPC;
+        const uint32_t crow = (uint32_t)lane / CPR, chunk = (uint32_t)lane % CPR;
+        const uint64_t k_step = (uint64_t)RPC * p.k_sk, v_step = (uint64_t)RPC * p.v_sk;
         auto issue = [&](uint32_t v0, int slot) {
             const uint32_t dst0 = ring_s + (uint32_t)(slot * STAGE * 16);
+            if (v0 >= u.s && v0 + 16 <= k_end) {
+                const uint16_t* ks = kbase + (uint64_t)(v0 + skip + crow) * p.k_sk + chunk * 8;
+                const uint16_t* vs = vbase + (uint64_t)(v0 + skip + crow) * p.v_sk + chunk * 8;
 #pragma unroll
-            for (int n = 0; n < STAGE / 32; ++n) {
-                const uint32_t e = (uint32_t)(lane + 32 * n);
-                const uint32_t kv = e / (16 * CPR), row = (e / CPR) % 16, chunk = e % CPR;
+                for (int n = 0; n < COPIES; ++n, ks += k_step)
+                    cp_async16(dst0 + ((crow + n * RPC) * CPR + k_chunk<D>(crow + n * RPC, chunk)) * 16, ks, 16u);
+#pragma unroll
+                for (int n = 0; n < COPIES; ++n, vs += v_step)
+                    cp_async16(dst0 + (16 * CPR + (crow + n * RPC) * CPR + v_chunk(crow + n * RPC, chunk)) * 16, vs, 16u);
+                return;
+            }
+#pragma unroll
+            for (int n = 0; n < 2 * COPIES; ++n) {
+                const uint32_t kv = n / COPIES, row = crow + (n % COPIES) * RPC;
                 const bool in = v0 + row < k_end;
                 const uint32_t vk = in ? v0 + row : k_begin, key = vk < u.s ? vk : vk + skip;
                 const uint16_t* src = kv ? vbase + (uint64_t)key * p.v_sk + chunk * 8 : kbase + (uint64_t)key * p.k_sk + chunk * 8;
@@ -972,11 +1026,17 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
                     const uint4 w = kst[row * CPR + k_chunk<D>(row, (uint32_t)(c * (QW / 4) + i))];
                     kw[4 * i] = w.x, kw[4 * i + 1] = w.y, kw[4 * i + 2] = w.z, kw[4 * i + 3] = w.w;
                 }
+                // two chains of dependent products instead of one
+                float s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    mma16816<FMT>(s[n], qa[0][2 * ks], qa[1][2 * ks], qa[0][2 * ks + 1], qa[1][2 * ks + 1], kw[2 * ks],
-                                  kw[2 * ks + 1]);
+                for (int ks = 0; ks < KS; ks += 2) {
+                    mma16816<FMT>(s[n], qa[0][2 * ks], qa[1][2 * ks], qa[0][2 * ks + 1], qa[1][2 * ks + 1], kw[2 * ks], kw[2 * ks + 1]);
+                    mma16816<FMT>(s2, qa[0][2 * ks + 2], qa[1][2 * ks + 2], qa[0][2 * ks + 3], qa[1][2 * ks + 3], kw[2 * ks + 2],
+                                  kw[2 * ks + 3]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] += s2[e];
             }
             // V words of keys 2c, 2c+1, 2c+8, 2c+9 at columns g*D/8 ..
             uint32_t vw[4][NJ / 2];
@@ -1001,18 +1061,26 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
             slot = slot + 1 == DEC_STAGES ? 0 : slot + 1;
             // scores in log2 units, masked: s[n][e] is row g + 8 * (e >> 1), virtual key v0 + 8n + 2c + (e & 1)
             float mx[2] = {NEG, NEG};
+            if (v0 >= open && v0 + 16 <= shut) {  // seen by every row
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int rr = e >> 1;
-                    const uint32_t vk = v0 + 8 * n + 2 * c + (e & 1);
-                    const int32_t key = (int32_t)(vk < u.s ? vk : vk + skip);
-                    const bool seen = vk < k_end && key <= high[rr] && (key >= low[rr] || key < sinks);
-                    const float x = seen ? s[n][e] * p.scale_log2 : NEG;
-                    s[n][e] = x;
-                    mx[rr] = fmaxf(mx[rr], x);
-                }
+                    for (int e = 0; e < 4; ++e) s[n][e] *= p.scale_log2;
+            } else {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int rr = e >> 1;
+                        const uint32_t vk = v0 + 8 * n + 2 * c + (e & 1);
+                        const int32_t key = (int32_t)(vk < u.s ? vk : vk + skip);
+                        const bool seen = vk < k_end && key <= high[rr] && (key >= low[rr] || key < sinks);
+                        s[n][e] = seen ? s[n][e] * p.scale_log2 : NEG;
+                    }
+            }
+#pragma unroll
+            for (int rr = 0; rr < 2; ++rr)
+                mx[rr] = fmaxf(fmaxf(s[0][2 * rr], s[0][2 * rr + 1]), fmaxf(s[1][2 * rr], s[1][2 * rr + 1]));
             float alpha[2], base[2];
 #pragma unroll
             for (int rr = 0; rr < 2; ++rr) {
@@ -1072,33 +1140,34 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
         }
         __syncthreads();
         const bool whole = tin == 0 && seg == u.tiles;
-        float* part = p.part + ((uint64_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * 16 * REC<D>;
-        for (uint32_t r = 0; r < R; ++r) {
-            float mw[DEC_WARPS], lw[DEC_WARPS], M = NEG;
+        const uint64_t slot0 = ((uint64_t)blockIdx.x * 2 + (t == t_begin ? 0 : 1)) * 16;  // this segment's records
+        auto warp_row = [&](uint32_t w, uint32_t r) { return reinterpret_cast<const float*>(dsm + (size_t)w * C::RING) + r * (D + 2); };
+        if (threadIdx.x < R) {
+            const uint32_t r = threadIdx.x;
+            float M = NEG, Lr = 0.0f;
 #pragma unroll
-            for (int w = 0; w < DEC_WARPS; ++w) {
-                const float* x = reinterpret_cast<const float*>(dsm + (size_t)w * C::RING) + r * (D + 2);
-                mw[w] = x[0], lw[w] = x[1];
-                if (lw[w] != 0.0f) M = fmaxf(M, mw[w]);
-            }
-            float wt[DEC_WARPS], Lr = 0.0f;
+            for (int w = 0; w < SPAN_WARPS; ++w)
+                if (warp_row(w, r)[1] != 0.0f) M = fmaxf(M, warp_row(w, r)[0]);
 #pragma unroll
-            for (int w = 0; w < DEC_WARPS; ++w) {
-                wt[w] = lw[w] != 0.0f ? exp2f(mw[w] - M) : 0.0f;
-                Lr = fmaf(lw[w], wt[w], Lr);
+            for (int w = 0; w < SPAN_WARPS; ++w) {
+                const float lw = warp_row(w, r)[1], wt = lw != 0.0f ? exp2f(warp_row(w, r)[0] - M) : 0.0f;
+                wts[r][w] = wt;
+                Lr = fmaf(lw, wt, Lr);
             }
-            float* rec = (whole ? cmb : part) + r * REC<D>;
-            if (threadIdx.x == 0) {
-                rec[0] = M == NEG ? 0.0f : M + p.shift;
-                rec[1] = Lr;
-            }
-            for (uint32_t d = threadIdx.x; d < (uint32_t)D; d += 32 * DEC_WARPS) {
+            const float2 h = make_float2(M == NEG ? 0.0f : M + p.shift, Lr);
+            if (whole) heads[r] = h;
+            else p.part_heads[slot0 + r] = h;
+        }
+        __syncthreads();
+        {
+            float* rows = whole ? cmb : p.part + slot0 * D;
+            for (uint32_t i = threadIdx.x; i < R * D; i += 32 * SPAN_WARPS) {
+                const uint32_t r = i / D, d = i % D;
                 float acc = 0.0f;
 #pragma unroll
-                for (int w = 0; w < DEC_WARPS; ++w)
-                    if (wt[w] != 0.0f)
-                        acc = fmaf(reinterpret_cast<const float*>(dsm + (size_t)w * C::RING)[r * (D + 2) + 2 + d], wt[w], acc);
-                rec[4 + d] = acc;
+                for (int w = 0; w < SPAN_WARPS; ++w)
+                    if (wts[r][w] != 0.0f) acc = fmaf(warp_row(w, r)[2 + d], wts[r][w], acc);
+                rows[i] = acc;
             }
         }
         // Which CTAs share the unit: those of its first and last tiles.
@@ -1121,31 +1190,27 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
         }
         if (finish) {
             if (p.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's records are written
-            for (uint32_t r = warp; r < R; r += DEC_WARPS) {
+            for (uint32_t r = warp; r < R; r += SPAN_WARPS) {
                 float M = NEG, Lr = 0.0f, acc[D / 32];
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
                 if (whole) {
-                    const float* rec = cmb + r * REC<D>;
-                    if (rec[1] != 0.0f) {
-                        M = rec[0], Lr = rec[1];
+                    M = heads[r].x, Lr = heads[r].y;
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i) acc[i] = rec[4 + lane * (D / 32) + i];
-                    }
+                    for (int i = 0; i < D / 32; ++i) acc[i] = cmb[r * D + lane * (D / 32) + i];
                 } else {
                     // CTA c0 entered the unit as its first segment only if the
                     // unit begins at the CTA's first tile
                     const uint32_t second = u_begin == c0 * per_cta ? 0u : 1u;
-                    join_records<D>(c1 - c0 + 1,
-                                    [&](uint32_t i) {
-                                        return p.part + (((uint64_t)(c0 + i) * 2 + (i == 0 ? second : 0u)) * 16 + r) * REC<D>;
-                                    },
-                                    M, Lr, acc);
+                    auto place = [&](uint32_t i) { return ((uint64_t)(c0 + i) * 2 + (i == 0 ? second : 0u)) * 16 + r; };
+                    join_records<D>(c1 - c0 + 1, [&](uint32_t i) { return p.part_heads + place(i); },
+                                    [&](uint32_t i) { return p.part + place(i) * D; }, M, Lr, acc);
                 }
                 const uint32_t h = hkv * p.G + r / p.L, q = r % p.L;
                 if (p.prefix) {
-                    const float* pre = p.prefix + (((uint64_t)b * p.H + h) * p.L + q) * p.prefix_count * REC<D>;
-                    join_records<D>(p.prefix_count, [&](uint32_t i) { return pre + i * REC<D>; }, M, Lr, acc);
+                    const uint64_t at = (((uint64_t)b * p.H + h) * p.L + q) * p.prefix_count;
+                    join_records<D>(p.prefix_count, [&](uint32_t i) { return p.prefix_heads + at + i; },
+                                    [&](uint32_t i) { return p.prefix + (at + i) * D; }, M, Lr, acc);
                 }
                 store_piece<D>(p.out, p.out_low, (uint64_t)b * p.o_sb + (uint64_t)h * p.o_sh + (uint64_t)q * p.o_sl, lane, acc,
                                inverse(Lr));
@@ -1161,30 +1226,32 @@ __global__ void __launch_bounds__(32 * DEC_WARPS) span_decode_kernel(SpanDecodeP
 
 // ------------------------------------------------------------------ host
 
-// A rank-4 map {D, n1, n2, n3} with element strides s[0..2] of the outer axes
-// (unit axes: any) and 128-byte boxes {128 / esz, box[0..2]}; false when the
+// A map {D, n...} with element strides s of the outer axes (unit axes: any)
+// and 128-byte boxes {128 / esz, box...}; false when the
 // strides or the base do not suit TMA.
-bool span_map(CUtensorMap* map, const void* ptr, uint32_t dtype, uint64_t D, const uint64_t (&n)[3], const uint64_t (&s)[3],
-              const uint32_t (&box)[3], bool promote) {
+template <int N>
+bool span_map(CUtensorMap* map, const void* ptr, uint32_t dtype, uint64_t D, const uint64_t (&n)[N], const uint64_t (&s)[N],
+              const uint32_t (&box)[N], bool promote) {
     auto enc = encode_tiled_attn();
     if (!enc || reinterpret_cast<uintptr_t>(ptr) % 16) return false;
     const uint64_t esz = dtype == FB_F32 ? 4 : 2;
-    cuuint64_t dims[4] = {D, n[0], n[1], n[2]}, strides[3];
+    cuuint64_t dims[N + 1] = {D}, strides[N];
+    cuuint32_t boxes[N + 1] = {(cuuint32_t)(128 / esz)}, estr[N + 1] = {1};
     uint64_t filler = (D * esz + 15) / 16 * 16;
-    for (int i = 0; i < 3; ++i) {
+    for (int i = 0; i < N; ++i) {
         uint64_t sb = s[i] * esz;
         if (n[i] == 0 || n[i] > (1ull << 31)) return false;
         if (n[i] == 1 && (sb == 0 || sb % 16 || sb >= (1ull << 40))) sb = filler;
         if (sb == 0 || sb % 16 || sb >= (1ull << 40)) return false;
         strides[i] = sb;
+        dims[i + 1] = n[i], boxes[i + 1] = box[i], estr[i + 1] = 1;
         filler = (sb * n[i] + 15) / 16 * 16;
         if (filler >= (1ull << 40)) filler = 16;
     }
-    const cuuint32_t b4[4] = {(cuuint32_t)(128 / esz), box[0], box[1], box[2]}, estr[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = dtype == FB_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : dtype == FB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    return enc(map, type, 4, const_cast<void*>(ptr), dims, strides, b4, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    return enc(map, type, N + 1, const_cast<void*>(ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, promote ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_NONE,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1269,12 +1336,27 @@ void launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t 
     (void)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// The tcgen05 kernel over the shared prefix (shared = true) or over the
-// sequences' own keys.  part: records are written there (stride and first
-// index given; `splits` ranges), else output rows.
+// Records of every query row, `count` each: heads, then rows; heads null: none.
+struct Records {
+    float2* heads = nullptr;
+    float* rows = nullptr;
+    uint32_t count = 0;
+};
 template <int D>
-int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* part, uint32_t part_stride, uint32_t part_first,
-                 const TileGrid& g, float shift, bool overlap, cudaStream_t st) {
+bool get_records(cudaStream_t st, const SpanOperands& a, uint64_t count, int slot, uint64_t n, Records* r) {
+    const uint64_t heads = (n * count * sizeof(float2) + 255) / 256 * 256;
+    char* p = static_cast<char*>(scratch(st, heads + n * count * D * sizeof(float), slot));
+    r->heads = reinterpret_cast<float2*>(p);
+    r->rows = reinterpret_cast<float*>(p + heads);
+    r->count = (uint32_t)count;
+    return p != nullptr;
+}
+
+// The tcgen05 kernel over the shared prefix (shared = true) or over the
+// sequences' own keys: records from index `first` on, or output rows.
+template <int D>
+int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, const Records& rec, uint32_t first, const TileGrid& g,
+                 float shift, bool overlap, cudaStream_t st) {
     using C = TCfg<D>;
     SpanTileParams p{};
     p.B = (uint32_t)a.B, p.H = (uint32_t)a.H, p.L = (uint32_t)a.L;
@@ -1296,28 +1378,31 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
     p.hidden = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;
     p.sinks32 = (int32_t)std::min<uint64_t>(s.sinks, 0x7fffffff);
     p.splits = (uint32_t)g.splits;
-    p.part = part, p.part_stride = part_stride, p.part_first = part_first;
-    p.out = a.op, p.out_low = s.base.out_low;
-    p.o_sb = a.o.s_batch, p.o_sh = a.o.s_head, p.o_sl = a.o.s_row;
-    CUtensorMap tq, tk, tv, tk16{}, tv16{};
+    p.heads = rec.heads, p.stride = rec.count, p.first = first;
+    p.out_low = rec.heads ? 0 : s.base.out_low;
+    CUtensorMap tq, tk, tv, tk16{}, tv16{}, to;
     const uint32_t dt = a.fmt ? FB_BF16 : FB_F16;
     const uint32_t qbox[3] = {p.GB, p.LB, p.NB}, kbox[3] = {TK, 1, 1}, kbox16[3] = {16, 1, 1};
-    if (!span_map(&tq, a.qp, dt, D, {a.H, a.L, a.B}, {a.q.s_head, a.q.s_row, a.q.s_batch}, qbox, true)) return FB_ERR_UNSUPPORTED;
+    if (!span_map<3>(&tq, a.qp, dt, D, {a.H, a.L, a.B}, {a.q.s_head, a.q.s_row, a.q.s_batch}, qbox, true)) return FB_ERR_UNSUPPORTED;
     if (shared) {
         const uint16_t* pk = static_cast<const uint16_t*>(s.pk) + s.pk_offset;
         const uint16_t* pv = static_cast<const uint16_t*>(s.pv) + s.pv_offset;
-        if (!span_map(&tk, pk, dt, D, {s.prefix_keys, a.Hkv, 1}, {s.pk_stride_key, s.pk_stride_head, 0}, kbox, true) ||
-            !span_map(&tv, pv, dt, D, {s.prefix_keys, a.Hkv, 1}, {s.pv_stride_key, s.pv_stride_head, 0}, kbox, true))
+        if (!span_map<3>(&tk, pk, dt, D, {s.prefix_keys, a.Hkv, 1}, {s.pk_stride_key, s.pk_stride_head, 0}, kbox, true) ||
+            !span_map<3>(&tv, pv, dt, D, {s.prefix_keys, a.Hkv, 1}, {s.pv_stride_key, s.pv_stride_head, 0}, kbox, true))
             return FB_ERR_UNSUPPORTED;
     } else {
-        if (!span_map(&tk, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox, true) ||
-            !span_map(&tv, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox, true) ||
-            !span_map(&tk16, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox16, true) ||
-            !span_map(&tv16, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox16, true))
+        if (!span_map<3>(&tk, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox, true) ||
+            !span_map<3>(&tv, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox, true) ||
+            !span_map<3>(&tk16, a.kp, dt, D, {a.Lk, a.Hkv, a.k.batch}, {a.k.s_row, a.k.s_head, a.k.s_batch}, kbox16, true) ||
+            !span_map<3>(&tv16, a.vp, dt, D, {a.Lk, a.Hkv, a.v.batch}, {a.v.s_row, a.v.s_head, a.v.s_batch}, kbox16, true))
             return FB_ERR_UNSUPPORTED;
     }
-    auto runs32 = [](uint64_t n, uint64_t stride) { return n <= 1 || stride % 16 == 0; };
-    p.wide = reinterpret_cast<uintptr_t>(a.op) % 32 == 0 && runs32(a.B, a.o.s_batch) && runs32(a.H, a.o.s_head) && runs32(a.L, a.o.s_row);
+    const uint32_t obox[4] = {1, p.GB, p.LB, p.NB};
+    const uint64_t row = (uint64_t)rec.count * D;
+    if (rec.heads ? !span_map<4>(&to, rec.rows, FB_F32, D, {rec.count, a.H, a.L, a.B}, {(uint64_t)D, a.L * row, row, a.H * a.L * row}, obox, false)
+                  : !span_map<4>(&to, a.op, s.base.out_low ? s.base.out_low : (uint32_t)FB_F32, D, {1, a.H, a.L, a.B},
+                                 {0, a.o.s_head, a.o.s_row, a.o.s_batch}, obox, false))
+        return FB_ERR_UNSUPPORTED;
     const uint64_t items = g.units * p.groups * p.splits;
     if (items > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
     p.items = (uint32_t)items;
@@ -1325,17 +1410,17 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, float* p
     auto kernel = a.fmt ? span_tile_kernel<D, 1> : span_tile_kernel<D, 0>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
         return launch_status("shared-memory attribute");
-    launch_after(kernel, (unsigned)grid, C::THREADS, C::SMEM, overlap, st, tq, tk, tv, tk16, tv16, p);
+    launch_after(kernel, (unsigned)grid, C::THREADS, C::SMEM, overlap, st, tq, tk, tv, tk16, tv16, to, p);
     count_launch(kernel_name("span_tile_kernel", {D, shared ? 1 : 0}).c_str());
     return launch_status("kernel launch");
 }
 
 template <int D>
-int launch_merge(const SpanArgs& s, const SpanOperands& a, const float* part, uint32_t count, cudaStream_t st) {
+int launch_merge(const SpanArgs& s, const SpanOperands& a, const Records& rec, cudaStream_t st) {
     SpanMergeParams m{};
-    m.part = part;
+    m.heads = rec.heads, m.part = rec.rows;
     m.rows = a.B * a.H * a.L;
-    m.count = count;
+    m.count = rec.count;
     m.H = (uint32_t)a.H, m.L = (uint32_t)a.L;
     m.out = a.op, m.out_low = s.base.out_low;
     m.o_sb = a.o.s_batch, m.o_sh = a.o.s_head, m.o_sl = a.o.s_row;
@@ -1346,20 +1431,27 @@ int launch_merge(const SpanArgs& s, const SpanOperands& a, const float* part, ui
 }
 
 template <int D>
-int launch_decode(const SpanArgs& s, const SpanOperands& a, const float* prefix, uint32_t prefix_count, float shift,
-                  cudaStream_t st) {
+int launch_decode(const SpanArgs& s, const SpanOperands& a, const Records& prefix, float shift, cudaStream_t st) {
     const uint64_t units = a.B * a.Hkv;
     // The most 64-key tiles that a unit can have, over all lengths.
     const uint64_t seen = std::min<uint64_t>(a.Lk, std::min(s.sinks, a.Lk) + std::min(s.window, a.Lk) + a.L);
     const uint64_t tiles = units * std::max<uint64_t>(1, (seen + DTILE - 1) / DTILE);
     if (tiles > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
-    // Two CTAs per SM, at least two tiles each once every SM has one.
+    // A unit of at most 512 keys is one CTA's (a CTA of four warps streams it
+    // in the time that joining two CTAs' records takes); longer ones are dealt
+    // out to two CTAs per SM, at least two tiles each once every SM has one.
     const uint64_t sms = (uint64_t)sm_count();
-    const uint64_t grid = tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
+    const bool whole = seen <= 8 * DTILE && units <= 0x7fffffffull;
+    const uint64_t grid = whole ? units : tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
     SpanDecodeParams d{};
-    d.part = static_cast<float*>(scratch(st, grid * 2 * 16 * REC<D> * sizeof(float), SCRATCH_SPAN_PART));
-    d.arrived = static_cast<uint32_t*>(scratch(st, units * sizeof(uint32_t), SCRATCH_SPAN_COUNT));
-    if (!d.part || !d.arrived) return FB_ERR_DRIVER;
+    d.whole_units = whole ? 1 : 0;
+    if (!whole) {
+        Records own;
+        if (!get_records<D>(st, a, 1, SCRATCH_SPAN_PART, grid * 2 * 16, &own)) return FB_ERR_DRIVER;
+        d.part_heads = own.heads, d.part = own.rows;
+        d.arrived = static_cast<uint32_t*>(scratch(st, units * sizeof(uint32_t), SCRATCH_SPAN_COUNT));
+        if (!d.arrived) return FB_ERR_DRIVER;
+    }
     d.q = static_cast<const uint16_t*>(a.qp), d.k = static_cast<const uint16_t*>(a.kp), d.v = static_cast<const uint16_t*>(a.vp);
     d.q_sb = a.q.s_batch, d.q_sh = a.q.s_head, d.q_sl = a.q.s_row;
     d.k_sb = a.k.batch_bcast ? 0 : a.k.s_batch, d.k_sh = a.k.s_head, d.k_sk = a.k.s_row;
@@ -1370,13 +1462,13 @@ int launch_decode(const SpanArgs& s, const SpanOperands& a, const float* prefix,
     d.offset = s.offset, d.window = (int64_t)s.window, d.sinks = (int64_t)s.sinks;
     d.scale_log2 = s.base.scale * 1.4426950408889634f;
     d.shift = shift;
-    d.prefix = prefix, d.prefix_count = prefix_count;
+    d.prefix_heads = prefix.heads, d.prefix = prefix.rows, d.prefix_count = prefix.count;
     d.out = a.op, d.out_low = s.base.out_low;
     d.o_sb = a.o.s_batch, d.o_sh = a.o.s_head, d.o_sl = a.o.s_row;
     auto kernel = a.fmt ? span_decode_kernel<D, 1> : span_decode_kernel<D, 0>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DCfg<D>::SMEM) != cudaSuccess)
         return launch_status("shared-memory attribute");
-    launch_after(kernel, (unsigned)grid, 32 * DEC_WARPS, DCfg<D>::SMEM, prefix != nullptr, st, d);
+    launch_after(kernel, (unsigned)grid, 32 * SPAN_WARPS, DCfg<D>::SMEM, prefix.heads != nullptr, st, d);
     count_launch(kernel_name("span_decode_kernel", {D, (int)a.fmt}).c_str());
     return launch_status("kernel launch");
 }
@@ -1387,25 +1479,24 @@ int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
     const float shift = weight_shift(a.fmt, a.Lk + s.prefix_keys);
     const TileGrid pg = prefix ? tile_grid(s, a, true) : TileGrid{};
     const uint64_t ps = pg.splits;
+    const uint64_t rows = a.B * a.H * a.L;
+    Records rec;
     if (a.G * a.L <= 16) {  // few rows: the own keys streamed, the prefix's records joined there
-        float* part = nullptr;
         if (prefix) {
-            part = static_cast<float*>(scratch(st, a.B * a.H * a.L * ps * REC<D> * sizeof(float), SCRATCH_SPAN));
-            if (!part) return FB_ERR_DRIVER;
-            if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)ps, 0, pg, shift, false, st); r != FB_OK) return r;
+            if (!get_records<D>(st, a, ps, SCRATCH_SPAN, rows, &rec)) return FB_ERR_DRIVER;
+            if (int r = launch_tiles<D>(s, a, true, rec, 0, pg, shift, false, st); r != FB_OK) return r;
         }
-        return launch_decode<D>(s, a, part, (uint32_t)ps, shift, st);
+        return launch_decode<D>(s, a, rec, shift, st);
     }
     const TileGrid og = own ? tile_grid(s, a, false) : TileGrid{};
     const uint64_t count = ps + og.splits;
-    if (count <= 1) return launch_tiles<D>(s, a, prefix, nullptr, 0, 0, prefix ? pg : og, shift, false, st);
-    float* part = static_cast<float*>(scratch(st, a.B * a.H * a.L * count * REC<D> * sizeof(float), SCRATCH_SPAN));
-    if (!part) return FB_ERR_DRIVER;
+    if (count <= 1) return launch_tiles<D>(s, a, prefix, rec, 0, prefix ? pg : og, shift, false, st);
+    if (!get_records<D>(st, a, count, SCRATCH_SPAN, rows, &rec)) return FB_ERR_DRIVER;
     if (prefix)
-        if (int r = launch_tiles<D>(s, a, true, part, (uint32_t)count, 0, pg, shift, false, st); r != FB_OK) return r;
+        if (int r = launch_tiles<D>(s, a, true, rec, 0, pg, shift, false, st); r != FB_OK) return r;
     if (own)
-        if (int r = launch_tiles<D>(s, a, false, part, (uint32_t)count, (uint32_t)ps, og, shift, prefix, st); r != FB_OK) return r;
-    return launch_merge<D>(s, a, part, (uint32_t)count, st);
+        if (int r = launch_tiles<D>(s, a, false, rec, (uint32_t)ps, og, shift, prefix, st); r != FB_OK) return r;
+    return launch_merge<D>(s, a, rec, st);
 }
 
 }  // namespace
