@@ -139,6 +139,20 @@ struct TileItem {
         head0 = unit % p.head_blocks * p.GB, kv_head = head0 / p.group;
         unit_b = unit / p.head_blocks;  // 0 with shared keys
         filled = p.Lk, base = p.offset;
+        if (p.shared_keys) {  // every row of every tile sees all keys
+            const uint32_t all = (p.Lk + TK - 1) / TK, per = (all + p.splits - 1) / p.splits;
+            j0 = min(split * per, all);
+            n_kv = min(per, all - j0);
+            s16 = lo = 0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t tile = group * 2 + t;
+                real[t] = tile < p.tiles;
+                b0[t] = tile / p.l_tiles * p.NB, l0[t] = tile % p.l_tiles * p.LB;
+                n_t[t] = real[t] ? n_kv : 0, near[t] = 0, far[t] = 0;
+            }
+            return;
+        }
         if (p.lengths) {
             filled = min(filled, (int64_t)p.lengths[unit_b * p.length_stride]);
             base = filled - (int64_t)p.L;
@@ -149,12 +163,10 @@ struct TileItem {
         for (int t = 0; t < 2; ++t) {
             const uint32_t tile = group * 2 + t;
             real[t] = tile < p.tiles;
-            b0[t] = p.shared_keys ? tile / p.l_tiles * p.NB : unit_b;
-            l0[t] = (p.shared_keys ? tile % p.l_tiles : tile) * p.LB;
+            b0[t] = unit_b, l0[t] = tile * p.LB;
             rc[t] = Reach{0, 0, -1};
             if (!real[t]) continue;
-            if (p.shared_keys) rc[t] = Reach{0, 0, (int64_t)p.Lk - 1};
-            else rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
+            rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
             if (rc[t].hi < 0) continue;
             first = max(first, rc[t].first);
             if (rc[t].lo <= rc[t].hi) start = min(start, rc[t].lo), last = max(last, rc[t].hi);
@@ -808,9 +820,10 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // three-stage cp.async rings and combine in shared memory.  A unit inside one
 // CTA is finished there; otherwise its CTAs leave records and the last to
 // arrive (a counter per unit, reset by it) joins them in CTA order, so results
-// do not depend on who is last.  Records of the shared prefix, written by
-// span_tile_kernel just before, are joined at the same place; the launch
-// overlaps that kernel's end (programmatic dependent launch).
+// do not depend on who is last.  After a span_tile_kernel over a shared prefix
+// the launch overlaps that kernel (programmatic dependent launch) on the SMs it
+// leaves free; its records are joined at the same place where all CTAs fit
+// there, else by a launch of their own (waiting CTAs would keep others out).
 // Bound: HBM, the visible keys and values once.
 constexpr int DTILE = 64;  // keys
 constexpr int SPAN_WARPS = 4;
@@ -829,9 +842,12 @@ struct SpanDecodeParams {
     float2* part_heads;   // two records x 16 rows per CTA
     float* part;
     uint32_t* arrived;    // per unit, 0 between launches
-    const float2* prefix_heads;  // records of the shared prefix: ((b * H + h) * L + l) * prefix_count + i, or null
-    const float* prefix;
-    uint32_t prefix_count;
+    // Records of the shared prefix, ((b * H + h) * L + l) * records + i, or null:
+    // the first `records` are joined here (join), or this kernel's results
+    // become the last of them and another launch joins all.
+    float2* prefix_heads;
+    float* prefix;
+    uint32_t records, join;
     void* out;
     uint32_t out_low;
     uint64_t o_sb, o_sh, o_sl;
@@ -931,7 +947,10 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         hkv = found[1] / tpu, tin = found[1] % tpu;
     }
     const uint32_t per_cta = p.whole_units ? T : (T + gridDim.x - 1) / gridDim.x;
-    if (t_begin >= T) return;
+    if (t_begin >= T) {
+        if (p.prefix && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const uint32_t t_end = min(t_begin + per_cta, T);
 
     for (uint32_t t = t_begin; t < t_end;) {
@@ -1189,7 +1208,7 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
             __syncthreads();  // cmb
         }
         if (finish) {
-            if (p.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's records are written
+            if (p.join) asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's records are written
             for (uint32_t r = warp; r < R; r += SPAN_WARPS) {
                 float M = NEG, Lr = 0.0f, acc[D / 32];
 #pragma unroll
@@ -1208,8 +1227,14 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
                 }
                 const uint32_t h = hkv * p.G + r / p.L, q = r % p.L;
                 if (p.prefix) {
-                    const uint64_t at = (((uint64_t)b * p.H + h) * p.L + q) * p.prefix_count;
-                    join_records<D>(p.prefix_count, [&](uint32_t i) { return p.prefix_heads + at + i; },
+                    const uint64_t at = (((uint64_t)b * p.H + h) * p.L + q) * p.records;
+                    if (!p.join) {
+                        const uint64_t mine = at + p.records - 1;
+                        if (lane == 0) p.prefix_heads[mine] = make_float2(M == NEG ? 0.0f : M, Lr);
+                        store_piece<D>(p.prefix, 0, mine * D, lane, acc, 1.0f);
+                        continue;
+                    }
+                    join_records<D>(p.records, [&](uint32_t i) { return p.prefix_heads + at + i; },
                                     [&](uint32_t i) { return p.prefix + (at + i) * D; }, M, Lr, acc);
                 }
                 store_piece<D>(p.out, p.out_low, (uint64_t)b * p.o_sb + (uint64_t)h * p.o_sh + (uint64_t)q * p.o_sl, lane, acc,
@@ -1221,7 +1246,8 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         tin = 0;
         if (++hkv == p.Hkv) hkv = 0, ++b;
     }
-    if (p.prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+    // One CTA that ends after the prefix's launch is enough for the grid to.
+    if (p.prefix && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ host
@@ -1259,7 +1285,7 @@ bool span_map(CUtensorMap* map, const void* ptr, uint32_t dtype, uint64_t D, con
 // Operands of a call the tensor cores take: layouts with merged batch axes.
 struct SpanOperands {
     RowsLayout q, k, v, o;
-    uint64_t B, H, Hkv, L, Lk, G;
+    uint64_t B, H, Hkv, L, Lk, G, D;
     uint32_t fmt;
     const void *qp, *kp, *vp;
     void* op;
@@ -1289,7 +1315,12 @@ struct TileGrid {
 // Key ranges when the pairs of tiles alone do not fill the GPU: about one CTA
 // per SM, at least two key tiles each.  (A key tile takes a CTA 1.5 us with two
 // tiles of rows and 1.7 us with one, so rows are always paired.)
-TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared) {
+// Where span_decode_kernel streams the own keys meanwhile (`streamed` bytes of
+// them) on the SMs that the tiles leave free, the number of ranges that ends
+// both soonest: a key tile takes 2.2 us (5 us more for a CTA's start and end),
+// the stream 5.8 TB/s, which 70% of the SMs keep up, a record a write and a read
+// (64 sequences x 8192 shared keys + 512 own: 8 ranges, 64 CTAs, not 16).
+TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared, double streamed = 0.0) {
     TileGrid g{};
     g.GB = largest_divisor(a.G, TQ);
     const uint64_t room = TQ / g.GB;
@@ -1307,14 +1338,19 @@ TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared) {
     if (!shared)
         keys = std::min(keys, (std::min(s.sinks, a.Lk) + std::min(s.window, a.Lk) + 2 * g.LB + 16 + TK - 1) / TK);
     const uint64_t sms = (uint64_t)sm_count();
-    auto ranges = [&](uint64_t ctas) -> uint64_t {
-        if (ctas >= sms || keys < 4) return 1;
-        const uint64_t want = std::min<uint64_t>(sms / ctas, keys / 2);
-        if (want <= 1) return 1;
-        const uint64_t per = (keys + want - 1) / want;
-        return (keys + per - 1) / per;
-    };
-    g.splits = ranges(g.units * ((g.tiles + 1) / 2));
+    const uint64_t ctas = g.units * ((g.tiles + 1) / 2);
+    g.splits = 1;
+    if (ctas < sms && keys >= 4) {
+        const double stream = streamed / 5.8e6, record = (double)(a.B * a.H * a.L) * a.D * 8 / 5.0e6;
+        double least = INFINITY;
+        for (uint64_t want = 1; want <= std::min<uint64_t>(sms / ctas, keys / 2); ++want) {
+            const uint64_t per = (keys + want - 1) / want, n = (keys + per - 1) / per;
+            const double tiles = (double)per * 2.2 + 5.0, done = (double)(sms - std::min(sms, ctas * n)) * tiles;
+            const double left = std::max(0.0, (stream * 0.7 * (double)sms - done) / (double)sms);
+            const double cost = std::max(stream, tiles + left) + record * (double)n;
+            if (cost < least) least = cost, g.splits = n;
+        }
+    }
     return g;
 }
 
@@ -1430,19 +1466,30 @@ int launch_merge(const SpanArgs& s, const SpanOperands& a, const Records& rec, c
     return launch_status("kernel launch");
 }
 
-template <int D>
-int launch_decode(const SpanArgs& s, const SpanOperands& a, const Records& prefix, float shift, cudaStream_t st) {
-    const uint64_t units = a.B * a.Hkv;
-    // The most 64-key tiles that a unit can have, over all lengths.
+// span_decode_kernel's CTAs.  A unit of at most 512 keys is one CTA's (four
+// warps stream it in the time that joining two CTAs' records takes); longer
+// ones are dealt out to two CTAs per SM, at least two tiles each once every SM
+// has one.
+struct DecodeGrid {
+    uint64_t ctas = 0;
+    bool whole = false;
+};
+bool decode_grid(const SpanArgs& s, const SpanOperands& a, DecodeGrid* g) {
+    const uint64_t units = a.B * a.Hkv, sms = (uint64_t)sm_count();
+    // the most 64-key tiles that a unit can have, over all lengths
     const uint64_t seen = std::min<uint64_t>(a.Lk, std::min(s.sinks, a.Lk) + std::min(s.window, a.Lk) + a.L);
     const uint64_t tiles = units * std::max<uint64_t>(1, (seen + DTILE - 1) / DTILE);
-    if (tiles > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
-    // A unit of at most 512 keys is one CTA's (a CTA of four warps streams it
-    // in the time that joining two CTAs' records takes); longer ones are dealt
-    // out to two CTAs per SM, at least two tiles each once every SM has one.
-    const uint64_t sms = (uint64_t)sm_count();
-    const bool whole = seen <= 8 * DTILE && units <= 0x7fffffffull;
-    const uint64_t grid = whole ? units : tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
+    if (tiles > 0x7fffffffull) return false;
+    g->whole = seen <= 8 * DTILE;
+    g->ctas = g->whole ? units : tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
+    return true;
+}
+
+template <int D>
+int launch_decode(const SpanArgs& s, const SpanOperands& a, const DecodeGrid& g, const Records& prefix, bool join, float shift,
+                  cudaStream_t st) {
+    const bool whole = g.whole;
+    const uint64_t grid = g.ctas, units = a.B * a.Hkv;
     SpanDecodeParams d{};
     d.whole_units = whole ? 1 : 0;
     if (!whole) {
@@ -1462,7 +1509,7 @@ int launch_decode(const SpanArgs& s, const SpanOperands& a, const Records& prefi
     d.offset = s.offset, d.window = (int64_t)s.window, d.sinks = (int64_t)s.sinks;
     d.scale_log2 = s.base.scale * 1.4426950408889634f;
     d.shift = shift;
-    d.prefix_heads = prefix.heads, d.prefix = prefix.rows, d.prefix_count = prefix.count;
+    d.prefix_heads = prefix.heads, d.prefix = prefix.rows, d.records = prefix.count, d.join = join ? 1 : 0;
     d.out = a.op, d.out_low = s.base.out_low;
     d.o_sb = a.o.s_batch, d.o_sh = a.o.s_head, d.o_sl = a.o.s_row;
     auto kernel = a.fmt ? span_decode_kernel<D, 1> : span_decode_kernel<D, 0>;
@@ -1477,16 +1524,22 @@ template <int D>
 int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
     const bool prefix = s.prefix_keys > 0, own = a.Lk > 0;
     const float shift = weight_shift(a.fmt, a.Lk + s.prefix_keys);
-    const TileGrid pg = prefix ? tile_grid(s, a, true) : TileGrid{};
+    const double streamed = a.G * a.L <= 16 ? (double)(a.B * a.Hkv * a.Lk) * a.D * 4 : 0.0;
+    const TileGrid pg = prefix ? tile_grid(s, a, true, streamed) : TileGrid{};
     const uint64_t ps = pg.splits;
     const uint64_t rows = a.B * a.H * a.L;
     Records rec;
     if (a.G * a.L <= 16) {  // few rows: the own keys streamed, the prefix's records joined there
-        if (prefix) {
-            if (!get_records<D>(st, a, ps, SCRATCH_SPAN, rows, &rec)) return FB_ERR_DRIVER;
-            if (int r = launch_tiles<D>(s, a, true, rec, 0, pg, shift, false, st); r != FB_OK) return r;
-        }
-        return launch_decode<D>(s, a, rec, shift, st);
+        DecodeGrid dg;
+        if (!decode_grid(s, a, &dg)) return FB_ERR_UNSUPPORTED;
+        if (!prefix) return launch_decode<D>(s, a, dg, rec, false, shift, st);
+        const uint64_t sms = (uint64_t)sm_count(), busy = std::min(sms, pg.units * ((pg.tiles + 1) / 2) * ps);
+        const bool join = dg.ctas <= 2 * (sms - busy) || !own;
+        if (!get_records<D>(st, a, join ? ps : ps + 1, SCRATCH_SPAN, rows, &rec)) return FB_ERR_DRIVER;
+        if (int r = launch_tiles<D>(s, a, true, rec, 0, pg, shift, false, st); r != FB_OK) return r;
+        if (!own) return launch_merge<D>(s, a, rec, st);
+        if (int r = launch_decode<D>(s, a, dg, rec, join, shift, st); r != FB_OK) return r;
+        return join ? FB_OK : launch_merge<D>(s, a, rec, st);
     }
     const TileGrid og = own ? tile_grid(s, a, false) : TileGrid{};
     const uint64_t count = ps + og.splits;
@@ -1518,7 +1571,7 @@ int launch_span_tc(const SpanArgs& s, void* stream) {
     if (s.prefix_keys > 0 && (s.pk_stride_d != 1 || s.pv_stride_d != 1)) return FB_ERR_UNSUPPORTED;
     const int r = (int)a.row_rank;
     SpanOperands x;
-    x.L = a.row_dims[r - 1], x.H = a.row_dims[r - 2], x.Lk = a.keys, x.G = a.group_size;
+    x.L = a.row_dims[r - 1], x.H = a.row_dims[r - 2], x.Lk = a.keys, x.G = a.group_size, x.D = a.depth;
     x.Hkv = x.H / x.G;
     x.fmt = a.dtype == FB_BF16 ? 1 : 0;
     if (x.L > (1u << 30) || x.Lk > (1u << 30) || s.prefix_keys > (1u << 30)) return FB_ERR_UNSUPPORTED;
