@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // of their concatenation, whatever unit borders fall inside, so that ragged
 // lengths and unit counts that do not divide the GPU leave no SM idle.  Each
 // CTA finds its first unit from a block scan over the lengths.  Per unit that
-// a CTA enters, its two warps take half of the keys each through
+// a CTA enters, its NW warps take a share of the keys each through
 // three-stage cp.async rings and combine in shared memory.  A unit inside one
 // CTA is finished there; otherwise its CTAs leave records and the last to
 // arrive (a counter per unit, reset by it) joins them in CTA order, so results
@@ -826,7 +826,6 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // there, else by a launch of their own (waiting CTAs would keep others out).
 // Bound: HBM, the visible keys and values once.
 constexpr int DTILE = 64;  // keys
-constexpr int SPAN_WARPS = 4;
 
 struct SpanDecodeParams {
     const uint16_t* q;
@@ -874,23 +873,23 @@ __device__ __forceinline__ UnitKeys unit_keys(const SpanDecodeParams& p, uint32_
     return u;
 }
 
-template <int D>
+template <int D, int NW>  // NW warps
 struct DCfg {
     static constexpr int CPR = D / 8;            // 16-byte chunks per K / V row
     static constexpr int STAGE = 2 * 16 * CPR;   // chunks per stage: 16 K rows, 16 V rows
     static constexpr int RING = DEC_STAGES * STAGE;
-    static constexpr int SMEM = SPAN_WARPS * RING * 16;
+    static constexpr int SMEM = NW * RING * 16;
     static_assert(RING * 16 >= 16 * (2 * D + 2) * 4, "a warp's rows and the CTA's fit a ring");
 };
 
-template <int D, int FMT>
-__global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecodeParams p) {
-    using C = DCfg<D>;
+template <int D, int FMT, int NW>
+__global__ void __launch_bounds__(32 * NW) span_decode_kernel(SpanDecodeParams p) {
+    using C = DCfg<D, NW>;
     constexpr int QW = D / 8, KS = D / 16, NJ = D / 8, CPR = C::CPR, STAGE = C::STAGE;
     extern __shared__ uint4 dsm[];
-    __shared__ uint32_t scan[SPAN_WARPS], found[2], last;
+    __shared__ uint32_t scan[NW], found[2], last;
     __shared__ float2 heads[16];             // the CTA's combined records: heads, and rows in
-    __shared__ float wts[16][SPAN_WARPS];    // the upper part of warp 0's ring
+    __shared__ float wts[16][NW];    // the upper part of warp 0's ring
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     uint4* ring = dsm + (size_t)warp * C::RING;
@@ -911,7 +910,7 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         t_begin = blockIdx.x * q;
         b = t_begin / (tpu * p.Hkv), hkv = t_begin / tpu % p.Hkv, tin = t_begin % tpu;
     } else {
-        const uint32_t per = (p.B + 32 * SPAN_WARPS - 1) / (32 * SPAN_WARPS);
+        const uint32_t per = (p.B + 32 * NW - 1) / (32 * NW);
         const uint32_t b0 = min(threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
         uint32_t mine = 0;
         for (uint32_t i = b0; i < b1; ++i) mine += unit_keys(p, i).tiles * p.Hkv;
@@ -926,7 +925,7 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         uint32_t before = incl - mine;
         T = 0;
 #pragma unroll
-        for (int w = 0; w < SPAN_WARPS; ++w) {
+        for (int w = 0; w < NW; ++w) {
             if (w < warp) before += scan[w];
             T += scan[w];
         }
@@ -957,7 +956,7 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         const UnitKeys u = unit_keys(p, b);
         const uint32_t seg = min(u.tiles - tin, t_end - t);
         const uint32_t v_begin = tin * DTILE, v_end = min((tin + seg) * DTILE, u.count);
-        const uint32_t quarter = ((v_end > v_begin ? v_end - v_begin : 0u) + 16 * SPAN_WARPS - 1) / (16 * SPAN_WARPS) * 16;
+        const uint32_t quarter = ((v_end > v_begin ? v_end - v_begin : 0u) + 16 * NW - 1) / (16 * NW) * 16;
         const uint32_t k_begin = min(v_begin + warp * quarter, v_end), k_end = min(k_begin + quarter, v_end);
         // Q fragments of rows g and g + 8 (zeros past R); row r is query head r / L, query r % L
         uint32_t qa[2][QW];
@@ -1165,10 +1164,10 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
             const uint32_t r = threadIdx.x;
             float M = NEG, Lr = 0.0f;
 #pragma unroll
-            for (int w = 0; w < SPAN_WARPS; ++w)
+            for (int w = 0; w < NW; ++w)
                 if (warp_row(w, r)[1] != 0.0f) M = fmaxf(M, warp_row(w, r)[0]);
 #pragma unroll
-            for (int w = 0; w < SPAN_WARPS; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float lw = warp_row(w, r)[1], wt = lw != 0.0f ? exp2f(warp_row(w, r)[0] - M) : 0.0f;
                 wts[r][w] = wt;
                 Lr = fmaf(lw, wt, Lr);
@@ -1180,11 +1179,11 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         __syncthreads();
         {
             float* rows = whole ? cmb : p.part + slot0 * D;
-            for (uint32_t i = threadIdx.x; i < R * D; i += 32 * SPAN_WARPS) {
+            for (uint32_t i = threadIdx.x; i < R * D; i += 32 * NW) {
                 const uint32_t r = i / D, d = i % D;
                 float acc = 0.0f;
 #pragma unroll
-                for (int w = 0; w < SPAN_WARPS; ++w)
+                for (int w = 0; w < NW; ++w)
                     if (wts[r][w] != 0.0f) acc = fmaf(warp_row(w, r)[2 + d], wts[r][w], acc);
                 rows[i] = acc;
             }
@@ -1209,7 +1208,7 @@ __global__ void __launch_bounds__(32 * SPAN_WARPS) span_decode_kernel(SpanDecode
         }
         if (finish) {
             if (p.join) asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's records are written
-            for (uint32_t r = warp; r < R; r += SPAN_WARPS) {
+            for (uint32_t r = warp; r < R; r += NW) {
                 float M = NEG, Lr = 0.0f, acc[D / 32];
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) acc[i] = 0.0f;
@@ -1467,12 +1466,14 @@ int launch_merge(const SpanArgs& s, const SpanOperands& a, const Records& rec, c
 }
 
 // span_decode_kernel's CTAs.  A unit of at most 512 keys is one CTA's (four
-// warps stream it in the time that joining two CTAs' records takes); longer
+// warps stream it in the time that joining two CTAs' records takes), of two
+// warps when there are more units than CTAs of four fit the GPU at once; longer
 // ones are dealt out to two CTAs per SM, at least two tiles each once every SM
 // has one.
 struct DecodeGrid {
     uint64_t ctas = 0;
     bool whole = false;
+    unsigned warps = 4;
 };
 bool decode_grid(const SpanArgs& s, const SpanOperands& a, DecodeGrid* g) {
     const uint64_t units = a.B * a.Hkv, sms = (uint64_t)sm_count();
@@ -1481,6 +1482,7 @@ bool decode_grid(const SpanArgs& s, const SpanOperands& a, DecodeGrid* g) {
     const uint64_t tiles = units * std::max<uint64_t>(1, (seen + DTILE - 1) / DTILE);
     if (tiles > 0x7fffffffull) return false;
     g->whole = seen <= 8 * DTILE;
+    g->warps = g->whole && units > 2 * sms ? 2 : 4;
     g->ctas = g->whole ? units : tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
     return true;
 }
@@ -1512,11 +1514,14 @@ int launch_decode(const SpanArgs& s, const SpanOperands& a, const DecodeGrid& g,
     d.prefix_heads = prefix.heads, d.prefix = prefix.rows, d.records = prefix.count, d.join = join ? 1 : 0;
     d.out = a.op, d.out_low = s.base.out_low;
     d.o_sb = a.o.s_batch, d.o_sh = a.o.s_head, d.o_sl = a.o.s_row;
-    auto kernel = a.fmt ? span_decode_kernel<D, 1> : span_decode_kernel<D, 0>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DCfg<D>::SMEM) != cudaSuccess)
+    const bool two = g.warps == 2;
+    auto kernel = two ? a.fmt ? span_decode_kernel<D, 1, 2> : span_decode_kernel<D, 0, 2>
+                      : a.fmt ? span_decode_kernel<D, 1, 4> : span_decode_kernel<D, 0, 4>;
+    const int smem = two ? DCfg<D, 2>::SMEM : DCfg<D, 4>::SMEM;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return launch_status("shared-memory attribute");
-    launch_after(kernel, (unsigned)grid, 32 * SPAN_WARPS, DCfg<D>::SMEM, prefix.heads != nullptr, st, d);
-    count_launch(kernel_name("span_decode_kernel", {D, (int)a.fmt}).c_str());
+    launch_after(kernel, (unsigned)grid, 32 * g.warps, smem, prefix.heads != nullptr, st, d);
+    count_launch(kernel_name("span_decode_kernel", {D, (int)a.fmt, (int)g.warps}).c_str());
     return launch_status("kernel launch");
 }
 
