@@ -160,12 +160,15 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
 // flushes to 0) where that matters, which keeps a masked class's 0 * -inf out
 // of S1; the NaN-propagating clamp keeps a NaN in it.
 //
-// Alternatives.  The k-th largest of the 256 threads' maxima (to 16 bits, by a
-// binary search in one warp) is a lower bound t of the row's k-th largest value, and the maxima of the row's segments
-// (kept in shared memory) say where values >= t lie: about k segments are
-// read again (L2), the values >= t collected with their indices and put in
-// order by counting.  More than CAND of them (a row of few distinct values),
-// and rows with NaN or infinities, take a scan per alternative instead.
+// Alternatives.  The k-th largest of the maxima of disjoint sets of lanes (to 16
+// bits, by a binary search over ballots) is a lower bound t of the row's k-th
+// largest value, and the maxima of the row's segments (kept in shared memory)
+// say where values >= t lie: about k segments are read again (L2), the values
+// >= t collected with their indices and put in order by counting.  More than
+// CAND of them (a row of few distinct values), and rows with NaN or +inf, take a
+// scan per alternative instead.  (Keeping a maximum per lane and segment, to
+// read 64 bytes again instead of a segment, measured slower up to 5
+// alternatives and no faster at 20 for rows under 50k classes.)
 //
 // Bound: HBM (the ex2 unit is 3/4 busy at the full rate with 16-bit logits).
 // Few rows are split over the CTAs of a cluster, each with its own sums and
@@ -329,12 +332,12 @@ template <typename T, int VPL>
 __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
     using W = Words<T>;
     constexpr int NW = VPL * 4;
-    __shared__ __align__(16) uint32_t tkey[BLOCK];
-    __shared__ uint32_t seg_max[MAX_SEGS], sel[MAX_SEGS];
+    __shared__ uint32_t tkey[BLOCK], okey[32];  // maxima of the threads, and of eight lanes each
+    __shared__ uint32_t seg_max[MAX_SEGS];
     __shared__ uint64_t cand[CAND];
     __shared__ uint64_t scan_keys[WARPS];
     __shared__ float wsum[3][WARPS];
-    __shared__ uint32_t n_sel, n_cand, tau;
+    __shared__ uint32_t n_cand;
     __shared__ TokenPartial mine;
     const uint32_t parts = a.parts, mult = a.mult;
     const uint64_t row = blockIdx.x / parts;
@@ -345,11 +348,11 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
     const uint32_t nseg = (uint32_t)((rv.vectors() + 32 * VPL - 1) / (32 * VPL));
     const uint32_t seg0 = min(part * a.part_segs, nseg), seg1 = min(seg0 + a.part_segs, nseg);
     const uint32_t groups = (seg1 - seg0 + mult - 1) / mult;
-    if (a.top) {
-        for (uint32_t i = threadIdx.x; i < groups; i += BLOCK) seg_max[i] = 0u;
-        if (threadIdx.x == 0) n_sel = n_cand = 0u;
-        __syncthreads();
-    }
+    if (threadIdx.x == 0) n_cand = 0u;
+    // A warp takes groups of `mult` segments in turn with the others.
+    auto seg_after = [&](uint32_t seg) {
+        return mult == 1 ? seg + WARPS : (seg - seg0 + 1) % mult ? seg + 1 : seg + 1 + (WARPS - 1) * mult;
+    };
     // segments [in0, in1) lie inside the row: no vector of theirs is partial
     const uint32_t per_seg = 32 * VPL * W::E;
     const uint32_t in0 = rv.head ? 1u : 0u, in1 = (uint32_t)(rv.end / per_seg);
@@ -374,16 +377,22 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
     float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);
     uint32_t run = 0u, own_max = W::LOWEST;
     uint32_t w[NW];
-    if (seg0 + warp < seg1) load_seg(seg0 + warp, w);
-    for (uint32_t seg = seg0 + warp; seg < seg1; seg += WARPS) {
+    uint32_t group_max = 0u;
+    if (seg0 + warp * mult < seg1) load_seg(seg0 + warp * mult, w);
+    for (uint32_t seg = seg0 + warp * mult, after; seg < seg1; seg = after) {
         uint32_t next[NW];  // the next segment's loads are in flight while this one is summed
-        if (seg + WARPS < seg1) load_seg(seg + WARPS, next);
+        after = seg_after(seg);
+        if (after < seg1) load_seg(after, next);
         uint32_t mx = w[0];
 #pragma unroll
         for (int i = 1; i < NW; ++i) mx = W::maximum(mx, w[i]);
         own_max = W::maximum(own_max, mx);
         const uint32_t top = __reduce_max_sync(0xffffffffu, Bits<T>::key(W::top(mx)));
-        if (a.top && lane == 0) atomicMax(&seg_max[(seg - seg0) / mult], top);
+        if (a.top) {
+            const uint32_t i = mult == 1 ? seg - seg0 : (seg - seg0) / mult;
+            group_max = mult == 1 || (seg - seg0) % mult == 0 ? top : max(group_max, top);
+            if (lane == 0) seg_max[i] = group_max;
+        }
         if (top > run) {
             run = top;
             const float v = Bits<T>::value(Bits<T>::pattern(top));
@@ -424,7 +433,13 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
     {
         const float t0 = warp_sum_f(s0.x + s0.y), t1 = warp_sum_f(s1.x + s1.y);
         if (lane == 0) wsum[0][warp] = m, wsum[1][warp] = t0, wsum[2][warp] = t1;
-        if (a.top) tkey[threadIdx.x] = Bits<T>::key(W::top(own_max));
+        if (a.top) {
+            uint32_t key = Bits<T>::key(W::top(own_max));
+            tkey[threadIdx.x] = key;
+#pragma unroll
+            for (int o = 1; o < 8; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+            if (lane % 8 == 0) okey[threadIdx.x / 8] = key;
+        }
     }
     __syncthreads();
     // The warps' sums, joined by each warp's first lanes.
@@ -445,71 +460,87 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         }
     }
 
+    const float ls = S0 == 0.0f ? row_nan() : logf(S0);  // log S0
     if (a.top) {
         const uint32_t k = a.top;
-        if (threadIdx.x < FB_MAX_TOP) mine.top[threadIdx.x] = 0ull;
-        if (warp == 0) {
-            // the k-th largest of the threads' maxima, its upper 16 bits: the
-            // largest value that at least k of them reach, bit by bit
-            uint32_t mine[8];
+        if (parts > 1 && threadIdx.x < FB_MAX_TOP) mine.top[threadIdx.x] = 0ull;
+        // t: the largest 16-bit prefix that k maxima reach, bit by bit, found
+        // by each warp for itself: of the octets' 32 maxima for few
+        // alternatives (k = 20 leaves about 30 values to put in order), else of
+        // the 256 threads'.
+        constexpr int SHIFT = W::E == 8 ? 0 : 16;
+        uint32_t t = 0;
+        if (k <= 20) {
+            const uint32_t v = okey[lane] >> SHIFT;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint4 v = *reinterpret_cast<const uint4*>(&tkey[lane * 8 + i * 4]);
-                mine[4 * i] = v.x, mine[4 * i + 1] = v.y, mine[4 * i + 2] = v.z, mine[4 * i + 3] = v.w;
-            }
-            constexpr int SHIFT = W::E == 8 ? 0 : 16;
-            uint32_t best = 0;
+            for (uint32_t bit = 0x8000u; bit; bit >>= 1)
+                if (__popc(__ballot_sync(0xffffffffu, v >= (t | bit))) >= k) t |= bit;
+        } else {
+            uint32_t v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = tkey[i * 32 + lane] >> SHIFT;
 #pragma unroll 1
             for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
-                const uint32_t want = (best | bit) << SHIFT;
                 uint32_t n = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) n += mine[i] >= want;
-                if (__reduce_add_sync(0xffffffffu, n) >= k) best |= bit;
+                for (int i = 0; i < 8; ++i) n += v[i] >= (t | bit);
+                if (__reduce_add_sync(0xffffffffu, n) >= k) t |= bit;
             }
-            if (lane == 0) tau = best << SHIFT;
         }
-        __syncthreads();
-        const uint32_t t = tau;
-        for (uint32_t i = threadIdx.x; i < groups; i += BLOCK)
-            if (seg_max[i] >= t) sel[atomicAdd(&n_sel, 1u)] = i;
-        __syncthreads();
-        bool ordered = S0 == S0;  // no NaN and no +inf among the values
-        if (ordered) {
-            const uint32_t reads = n_sel * mult;
-            for (uint32_t i = warp; i < reads; i += WARPS) {
-                const uint32_t seg = seg0 + sel[i / mult] * mult + i % mult;
-                if (seg >= seg1) continue;
-                uint32_t w[NW];
-                load_seg(seg, w);
-                uint32_t mx = w[0];
+        t <<= SHIFT;
+        const bool fine = S0 == S0;  // no NaN and no +inf among the values
+        if (fine) {
+            // The segments that reach t are read again; values at least t (as
+            // numbers: a zero of the other sign comes along) are collected.
+            float tv = Bits<T>::value(Bits<T>::pattern(t));
+            if (tv != tv) tv = -__int_as_float(0x7f800000);  // a prefix of -inf names a NaN
+            for (uint32_t g0 = 0; g0 < groups; g0 += 32 * WARPS) {
+                const uint32_t lane_g = g0 + lane * WARPS + warp;
+                uint32_t hits = __ballot_sync(0xffffffffu, lane_g < groups && seg_max[min(lane_g, MAX_SEGS - 1u)] >= t);
+                for (; hits; hits &= hits - 1) {
+                    const uint32_t g = g0 + (__ffs(hits) - 1) * WARPS + warp;
+                    for (uint32_t seg = seg0 + g * mult; seg < min(seg0 + (g + 1) * mult, seg1); ++seg) {
+                        uint32_t y[NW];
+                        load_seg(seg, y);
+                        const uint64_t v0 = ((uint64_t)seg * (32 * VPL) + lane) * W::E;
+                        auto take = [&](uint32_t bits, int e) {
+                            const uint64_t v = v0 + (uint64_t)(e / W::E) * 32 * W::E + e % W::E;
+                            if (v < rv.head || v >= rv.end) return;
+                            const uint32_t n = atomicAdd(&n_cand, 1u);
+                            if (n < CAND) cand[n] = ((uint64_t)Bits<T>::key(bits) << 32) | (0xffffffffu - (uint32_t)(v - rv.head));
+                        };
 #pragma unroll
-                for (int j = 1; j < NW; ++j) mx = W::maximum(mx, w[j]);
-                if (Bits<T>::key(W::top(mx)) < t) continue;
-                const uint64_t v0 = ((uint64_t)seg * (32 * VPL) + lane) * W::E;
-#pragma unroll
-                for (int e = 0; e < VPL * W::E; ++e) {
-                    uint32_t b;
-                    if constexpr (W::E == 8) b = e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
-                    else b = w[e];
-                    const uint32_t key = Bits<T>::key(b);
-                    const uint64_t v = v0 + (uint64_t)(e / W::E) * 32 * W::E + e % W::E;
-                    if (key >= t && v >= rv.head && v < rv.end) {
-                        const uint32_t n = atomicAdd(&n_cand, 1u);
-                        if (n < CAND) cand[n] = ((uint64_t)key << 32) | (0xffffffffu - (uint32_t)(v - rv.head));
+                        for (int i = 0; i < NW; ++i) {
+                            if constexpr (W::E == 8) {
+                                const float2 f = W::widen(y[i]);
+                                if (fmaxf(f.x, f.y) >= tv) {
+                                    if (f.x >= tv) take(y[i] & 0xffffu, 2 * i);
+                                    if (f.y >= tv) take(y[i] >> 16, 2 * i + 1);
+                                }
+                            } else if (__uint_as_float(y[i]) >= tv) {
+                                take(y[i], i);
+                            }
+                        }
                     }
                 }
             }
-            __syncthreads();
-            ordered = n_cand <= CAND;
         }
-        if (ordered) {
-            const uint32_t n = n_cand;
+        __syncthreads();
+        const uint32_t n = n_cand;
+        if (fine && n <= CAND) {
+            // Places by counting; a whole row's go out from here.
             for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
                 const uint64_t me = cand[i];
                 uint32_t rank = 0;
+#pragma unroll 4
                 for (uint32_t j = 0; j < n; ++j) rank += cand[j] > me;
-                if (rank < k) mine.top[rank] = me;
+                if (rank >= k) continue;
+                if (parts > 1) {
+                    mine.top[rank] = me;
+                } else {
+                    a.top_index[row * k + rank] = 0xffffffffu - (uint32_t)me;
+                    a.top_logprob[row * k + rank] = (Bits<T>::value(Bits<T>::pattern((uint32_t)(me >> 32))) - M) - ls;
+                }
             }
         } else {
             const uint64_t v0 = max((uint64_t)seg0 * (32 * VPL) * W::E, (uint64_t)rv.head);
@@ -523,69 +554,58 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
                     if (q < bound && q > best) best = q;
                 }
                 bound = block_max_u64<BLOCK>(best, scan_keys);
-                if (threadIdx.x == 0) mine.top[r] = bound;
-            }
-        }
-        __syncthreads();
-    }
-    if (parts > 1) {
-        if (threadIdx.x == 0) mine.m = M, mine.s0 = S0, mine.s1 = S1;
-        sync_cluster();
-        if (part == 0) {
-            const uint32_t at = (uint32_t)__cvta_generic_to_shared(&mine);
-            for (uint32_t p = 1; p < parts; ++p) {
-                const uint32_t peer = mapa_rank(at, p);
-                join_sums(M, S0, S1, ld_peer_f32(peer), ld_peer_f32(peer + 4), ld_peer_f32(peer + 8));
-            }
-            if (a.top) {
-                // the parts' alternatives in one list: their order by counting
-                const uint32_t n = parts * a.top;
-                const uint32_t off = (uint32_t)(reinterpret_cast<const char*>(mine.top) - reinterpret_cast<const char*>(&mine));
-                for (uint32_t i = threadIdx.x; i < n; i += BLOCK)
-                    cand[i] = ld_peer_u64(mapa_rank(at + off, i / a.top) + (i % a.top) * 8);
-                __syncthreads();
-                uint64_t me[2];
-                uint32_t rank[2];
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t i = threadIdx.x + h * BLOCK;
-                    rank[h] = a.top;
-                    if (i < n && cand[i]) {
-                        me[h] = cand[i], rank[h] = 0;
-                        for (uint32_t j = 0; j < n; ++j) rank[h] += cand[j] > me[h];
-                    }
+                if (threadIdx.x != 0) continue;
+                if (parts > 1) {
+                    mine.top[r] = bound;
+                } else {
+                    a.top_index[row * k + r] = 0xffffffffu - (uint32_t)bound;
+                    a.top_logprob[row * k + r] = (Bits<T>::value(Bits<T>::pattern((uint32_t)(bound >> 32))) - M) - ls;
                 }
-                sync_cluster();  // every peer's list has been read
-                for (int h = 0; h < 2; ++h)
-                    if (rank[h] < a.top) mine.top[rank[h]] = me[h];
-                __syncthreads();
-            } else {
-                sync_cluster();
             }
-        } else {
-            sync_cluster();  // this CTA's sums and list stay until they are read
-            return;
         }
     }
-    if (threadIdx.x >= FB_MAX_TOP) return;
-    // One row's results, in f64 from here.
-    const double ls = S0 == 0.0f ? (double)row_nan() : log((double)S0), lse = (double)M + ls;
-    if (threadIdx.x == 0) {
-        if (a.lse.p) a.lse.at<float>(row) = (float)lse;
-        if (a.entropy.p) a.entropy.at<float>(row) = (float)(ls - (double)S1 / (double)S0 * 0.6931471805599453);
+    auto store_row = [&](float ls) {
+        if (a.lse.p) a.lse.at<float>(row) = M + ls;
+        if (a.entropy.p) a.entropy.at<float>(row) = ls - S1 / S0 * 0.6931471805599453f;
         if (a.logprob.p) {
             const uint32_t t = a.targets.at<uint32_t>(row);
             float r = 0.0f;
-            if (t != FB_NO_TOKEN) r = t < a.cols ? (float)((double)Elem<T>::load(x + t) - lse) : row_nan();
+            if (t != FB_NO_TOKEN) r = t < a.cols ? (Elem<T>::load(x + t) - M) - ls : row_nan();
             a.logprob.at<float>(row) = r;
         }
+    };
+    if (parts == 1) {
+        if (threadIdx.x == BLOCK - 1) store_row(ls);
+        return;
     }
-    if (threadIdx.x < a.top) {
-        const uint64_t q = mine.top[threadIdx.x];
-        a.top_index[row * a.top + threadIdx.x] = 0xffffffffu - (uint32_t)q;
-        a.top_logprob[row * a.top + threadIdx.x] =
-            (float)((double)Bits<T>::value(Bits<T>::pattern((uint32_t)(q >> 32))) - lse);
+    if (threadIdx.x == 0) mine.m = M, mine.s0 = S0, mine.s1 = S1;
+    sync_cluster();  // every part's sums and list are in its shared memory
+    if (part == 0) {
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(&mine);
+        const uint32_t off = (uint32_t)(reinterpret_cast<const char*>(mine.top) - reinterpret_cast<const char*>(&mine));
+        const uint32_t n = parts * a.top;
+        for (uint32_t i = threadIdx.x; i < n; i += BLOCK)
+            cand[i] = ld_peer_u64(mapa_rank(at + off, i / a.top) + (i % a.top) * 8);
+        for (uint32_t p = 1; p < parts; ++p) {
+            const uint32_t peer = mapa_rank(at, p);
+            join_sums(M, S0, S1, ld_peer_f32(peer), ld_peer_f32(peer + 4), ld_peer_f32(peer + 8));
+        }
+        const float lsr = S0 == 0.0f ? row_nan() : logf(S0);
+        if (threadIdx.x == BLOCK - 1) store_row(lsr);
+        __syncthreads();
+        // the parts' alternatives in one list: places by counting
+        for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
+            const uint64_t me = cand[i];
+            if (me == 0) continue;
+            uint32_t rank = 0;
+#pragma unroll 4
+            for (uint32_t j = 0; j < n; ++j) rank += cand[j] > me;
+            if (rank >= a.top) continue;
+            a.top_index[row * a.top + rank] = 0xffffffffu - (uint32_t)me;
+            a.top_logprob[row * a.top + rank] = (Bits<T>::value(Bits<T>::pattern((uint32_t)(me >> 32))) - M) - lsr;
+        }
     }
+    sync_cluster();  // a part's sums and list stay until they are read
 }
 
 template <typename T, int VPL>
