@@ -23,14 +23,36 @@ __device__ uint32_t g_span_status;
 // A block of queries at positions pa .. pb (pa <= pb) over n filled keys sees
 // no key outside [0, first) and [lo, hi], first <= lo: hi = min(pb, n - 1),
 // lo = max(0, pa - window + 1).  hi < 0: nothing at all; lo > hi: only first.
-struct Reach {
-    int64_t first, lo, hi;
+//
+// 32 bits hold all of it: L and Lk are at most 2^30, so positions and window
+// starts clamped to +-2^30 by the host select the same keys.
+struct SpanKeys {
+    int32_t pos0, low0;     // without lengths: query 0's position, its window's first key (may be negative)
+    int32_t window, sinks;  // at most 2^30
+    const uint32_t* lengths;
+    uint64_t length_stride;
 };
-__device__ __forceinline__ Reach reach(int64_t pa, int64_t pb, int64_t n, int64_t window, int64_t sinks) {
+struct SpanBase {  // of one sequence
+    int32_t filled, pos0, low0;
+};
+__device__ __forceinline__ SpanBase span_base(const SpanKeys& k, uint32_t b, uint32_t L, uint32_t Lk) {
+    SpanBase s{(int32_t)Lk, k.pos0, k.low0};
+    if (k.lengths) {
+        s.filled = (int32_t)min(Lk, k.lengths[b * k.length_stride]);
+        s.pos0 = s.filled - (int32_t)L;
+        s.low0 = s.pos0 - k.window + 1;
+    }
+    return s;
+}
+struct Reach {
+    int32_t first, lo, hi;
+};
+// of queries la .. lb
+__device__ __forceinline__ Reach reach(const SpanBase& s, int32_t la, int32_t lb, int32_t sinks) {
     Reach r;
-    r.hi = min(pb, n - 1);
-    r.lo = max((int64_t)0, pa - window + 1);
-    r.first = max((int64_t)0, min(min(sinks, r.lo), r.hi + 1));
+    r.hi = min(s.pos0 + lb, s.filled - 1);
+    r.lo = max(0, s.low0 + la);
+    r.first = max(0, min(min(sinks, r.lo), r.hi + 1));
     return r;
 }
 
@@ -70,16 +92,13 @@ struct SpanTileParams {
     uint32_t group;                // query heads per key/value head
     uint32_t GB, LB, NB, rows;     // the tile's box and its row count GB * LB * NB
     uint32_t l_tiles, tiles;       // tiles along the queries; tiles of one unit
-    uint32_t groups, items;        // pairs of tiles per unit; units x groups x splits
+    uint32_t units, groups, items; // units; pairs of tiles per unit; units x groups x splits
     uint32_t head_blocks;          // H / GB
     uint32_t shared_keys;          // 1: every row sees all Lk keys of batch 0 (the shared prefix)
     uint32_t k_batch_bcast, v_batch_bcast;
-    const uint32_t* lengths;
-    uint64_t length_stride;
-    int64_t offset, window, sinks;
+    SpanKeys keys;
     float scale_log2, shift;
     float hidden;                  // what a hidden key's raw score becomes: its logit is -inf whatever the scale's sign
-    int32_t sinks32;               // sinks, at most 2^31 - 1
     uint32_t splits;               // key ranges of a pair
     // Output: through tmO, a 5-D map {D, records, heads, queries, batch}; for
     // records (heads not null) the one at index first + split of each row, its
@@ -124,7 +143,7 @@ struct TileItem {
     // Query tile t sees n_t of them: those of index (from j0) below near[t],
     // then those from far[t] on.
     uint32_t n_t[2], near[2], far[2];
-    int64_t filled, base;
+    SpanBase base;
     static __device__ __forceinline__ uint32_t after(uint32_t j, uint32_t near, uint32_t far) {
         return j + 1 < near ? j + 1 : max(j + 1, far);
     }
@@ -132,15 +151,15 @@ struct TileItem {
     __device__ __forceinline__ int32_t shift() const { return (int32_t)s16 - (int32_t)lo; }
     __device__ __forceinline__ void set(const SpanTileParams& p, uint32_t item) {
         // Last queries (the most keys under a long window) of every unit first.
-        const uint32_t units = p.items / (p.groups * p.splits);
-        split = item % p.splits;
-        const uint32_t group = p.groups - 1 - item / p.splits / units;
-        const uint32_t unit = item / p.splits % units;
-        head0 = unit % p.head_blocks * p.GB, kv_head = head0 / p.group;
+        uint32_t rest = item;
+        split = 0;
+        if (p.splits > 1) rest = item / p.splits, split = item - rest * p.splits;
+        const uint32_t rank = rest / p.units, unit = rest - rank * p.units, group = p.groups - 1 - rank;
         unit_b = unit / p.head_blocks;  // 0 with shared keys
-        filled = p.Lk, base = p.offset;
+        head0 = (unit - unit_b * p.head_blocks) * p.GB, kv_head = head0 / p.group;
         if (p.shared_keys) {  // every row of every tile sees all keys
-            const uint32_t all = (p.Lk + TK - 1) / TK, per = (all + p.splits - 1) / p.splits;
+            base = SpanBase{(int32_t)p.Lk, 0, 0};
+            const uint32_t all = (p.Lk + TK - 1) / TK, per = p.splits > 1 ? (all + p.splits - 1) / p.splits : all;
             j0 = min(split * per, all);
             n_kv = min(per, all - j0);
             s16 = lo = 0;
@@ -153,12 +172,9 @@ struct TileItem {
             }
             return;
         }
-        if (p.lengths) {
-            filled = min(filled, (int64_t)p.lengths[unit_b * p.length_stride]);
-            base = filled - (int64_t)p.L;
-        }
+        base = span_base(p.keys, unit_b, p.L, p.Lk);
         Reach rc[2];
-        int64_t first = 0, start = (int64_t)1 << 62, last = -1;
+        int32_t first = 0, start = 0x7fffffff, last = -1;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint32_t tile = group * 2 + t;
@@ -166,17 +182,17 @@ struct TileItem {
             b0[t] = unit_b, l0[t] = tile * p.LB;
             rc[t] = Reach{0, 0, -1};
             if (!real[t]) continue;
-            rc[t] = reach(base + l0[t], base + (int64_t)min(l0[t] + p.LB, p.L) - 1, filled, p.window, p.sinks);
+            rc[t] = reach(base, (int32_t)l0[t], (int32_t)min(l0[t] + p.LB, p.L) - 1, p.keys.sinks);
             if (rc[t].hi < 0) continue;
             first = max(first, rc[t].first);
             if (rc[t].lo <= rc[t].hi) start = min(start, rc[t].lo), last = max(last, rc[t].hi);
         }
-        int64_t s = (first + 15) / 16 * 16, end;
-        if (last < 0) s = 0, start = 0, end = first;              // the first keys alone
-        else if (start <= s) s = 0, start = 0, end = last + 1;    // one run
-        else end = s + last - start + 1;
-        s16 = (uint32_t)s, lo = (uint32_t)start;
-        const uint32_t all = (uint32_t)((end + TK - 1) / TK), per = (all + p.splits - 1) / p.splits;
+        uint32_t s = (uint32_t)(first + 15) / 16 * 16, end;
+        if (last < 0) s = 0, start = 0, end = (uint32_t)first;                            // the first keys alone
+        else if ((uint32_t)start <= s) s = 0, start = 0, end = (uint32_t)last + 1;        // one run
+        else end = s + (uint32_t)(last - start) + 1;
+        s16 = s, lo = (uint32_t)start;
+        const uint32_t all = (end + TK - 1) / TK, per = p.splits > 1 ? (all + p.splits - 1) / p.splits : all;
         j0 = min(split * per, all);
         const uint32_t j1 = min(j0 + per, all);
         n_kv = j1 - j0;
@@ -188,10 +204,10 @@ struct TileItem {
         for (int t = 0; t < 2; ++t) {
             uint32_t ns = 0, a0 = 0, e = 0;
             if (rc[t].hi >= 0) {
-                ns = (uint32_t)((rc[t].first + TK - 1) / TK);
+                ns = (uint32_t)(rc[t].first + TK - 1) / TK;
                 if (rc[t].lo <= rc[t].hi) {
-                    a0 = max((uint32_t)((rc[t].lo - start + s) / TK), ns);
-                    e = max((uint32_t)((rc[t].hi - start + s) / TK) + 1, a0);
+                    a0 = max(((uint32_t)(rc[t].lo - start) + s) / TK, ns);
+                    e = max(((uint32_t)(rc[t].hi - start) + s) / TK + 1, a0);
                 }
             }
             n_t[t] = overlap(0, ns) + overlap(a0, e);
@@ -219,6 +235,10 @@ __device__ __forceinline__ void tma_store_5d(const CUtensorMap* map, int32_t x, 
                      reinterpret_cast<uint64_t>(map)),
                  "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(src))
                  : "memory");
+}
+
+__device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
 template <int D, int FMT>
@@ -282,10 +302,17 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         mbar_init(drain, 1);
         fence_barrier_init();
     }
+    if (warp == 3 && lane == 0) {
+        prefetch_tensormap(&tmQ);
+        prefetch_tensormap(&tmK);
+        prefetch_tensormap(&tmV);
+        prefetch_tensormap(&tmO);
+    }
     if (warp == 1) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
+    if (warp == 2 && lane == 0 && item_at(0) < p.items) plans[0].set(p, item_at(0));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -375,7 +402,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 atomicOr(&g_span_status, 1u << DEV_ATTN_TIMEOUT);
                 break;
             }
-            plans[i % PLANS].set(p, item);
+            if (i > 0) plans[i % PLANS].set(p, item);  // (the first was made above)
             mbar_arrive(&plan_full[i % PLANS]);
         }
     } else if (warp == 1) {
@@ -445,10 +472,9 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             for (uint32_t j = 0; ok && j < n_kv; ++j) {
                 const uint32_t s = (g + j) % C::STAGES;
                 ok = wait(&v_full[s], ((g + j) / C::STAGES) & 1);
-                if (ok && p.lengths && j + 1 == n_kv && it.filled + it.shift() < (int64_t)(it.j0 + n_kv) * TK) {
+                if (ok && p.keys.lengths && j + 1 == n_kv && it.base.filled + it.shift() < (int32_t)((it.j0 + n_kv) * TK)) {
                     // value rows past the filled keys (in the last tile, if any): zeros
-                    const int64_t live = it.filled + it.shift() - (int64_t)(it.j0 + j) * TK;
-                    const uint32_t from = (uint32_t)max(live, (int64_t)0);
+                    const uint32_t from = (uint32_t)max(it.base.filled + it.shift() - (int32_t)((it.j0 + j) * TK), 0);
                     unsigned char* v = sKV + s * C::STAGE_BYTES + C::K_BYTES;
                     for (int b = 0; b < C::BOXES; ++b)
                         for (uint32_t o = from * 128 + lane * 16; o < TK * 128; o += 512)
@@ -502,10 +528,10 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             // virtual keys of this row: below vsink, and [vlow, vhigh]
             int32_t vsink, vlow, vhigh;
             {
-                const int64_t pos = p.shared_keys ? (int64_t)p.Lk - 1 : it.base + (int64_t)(it.l0[t] + (place >> 8 & 0xffu));
-                const int32_t high = (int32_t)max((int64_t)-1, min(pos, it.filled - 1));
-                vsink = p.shared_keys ? 0 : min(p.sinks32, high + 1);
-                vlow = p.shared_keys ? 0 : (int32_t)max((int64_t)0, min((int64_t)0x3fffffff, pos - p.window + 1)) + it.shift();
+                const int32_t l = (int32_t)(it.l0[t] + (place >> 8 & 0xffu));
+                const int32_t high = p.shared_keys ? (int32_t)p.Lk - 1 : max(-1, min(it.base.pos0 + l, it.base.filled - 1));
+                vsink = p.shared_keys ? 0 : min(p.keys.sinks, high + 1);
+                vlow = p.shared_keys ? 0 : max(0, min(0x3fffffff, it.base.low0 + l)) + it.shift();
                 vhigh = high + it.shift();
             }
             float m_used = NEG;  // running max (log2 units)
@@ -833,9 +859,7 @@ struct SpanDecodeParams {
     const uint16_t* v;
     uint64_t q_sb, q_sh, q_sl, k_sb, k_sh, k_sk, v_sb, v_sh, v_sk;
     uint32_t B, H, Hkv, G, L, Lk;
-    const uint32_t* lengths;
-    uint64_t length_stride;
-    int64_t offset, window, sinks;
+    SpanKeys keys;
     float scale_log2, shift;
     uint32_t whole_units; // 1: CTA i takes all of unit i
     float2* part_heads;   // two records x 16 rows per CTA
@@ -853,21 +877,16 @@ struct SpanDecodeParams {
 };
 
 struct UnitKeys {
-    int64_t base;             // position of query 0
+    SpanBase base;
     uint32_t s, lo, count;    // first keys, window start, visible keys
     uint32_t tiles;           // at least 1, so that every unit has a CTA
 };
 __device__ __forceinline__ UnitKeys unit_keys(const SpanDecodeParams& p, uint32_t b) {
-    int64_t n = p.Lk;
     UnitKeys u;
-    u.base = p.offset;
-    if (p.lengths) {
-        n = min(n, (int64_t)p.lengths[b * p.length_stride]);
-        u.base = n - (int64_t)p.L;
-    }
-    const Reach r = reach(u.base, u.base + (int64_t)p.L - 1, n, p.window, p.sinks);
+    u.base = span_base(p.keys, b, p.L, p.Lk);
+    const Reach r = reach(u.base, 0, (int32_t)p.L - 1, p.keys.sinks);
     u.s = (uint32_t)r.first;
-    u.lo = (uint32_t)min(r.lo, (int64_t)p.Lk);
+    u.lo = min((uint32_t)r.lo, p.Lk);
     u.count = u.s + (r.hi >= r.lo ? (uint32_t)(r.hi - r.lo + 1) : 0u);
     u.tiles = max(1u, (u.count + DTILE - 1) / DTILE);
     return u;
@@ -903,7 +922,7 @@ __global__ void __launch_bounds__(32 * NW) span_decode_kernel(SpanDecodeParams p
     if (p.whole_units) {
         b = blockIdx.x / p.Hkv, hkv = blockIdx.x % p.Hkv, tin = 0;
         t_begin = 0, T = unit_keys(p, b).tiles;
-    } else if (!p.lengths) {
+    } else if (!p.keys.lengths) {
         const uint32_t tpu = unit_keys(p, 0).tiles;
         T = p.B * p.Hkv * tpu;
         const uint32_t q = (T + gridDim.x - 1) / gridDim.x;
@@ -964,9 +983,9 @@ __global__ void __launch_bounds__(32 * NW) span_decode_kernel(SpanDecodeParams p
 #pragma unroll
         for (int rr = 0; rr < 2; ++rr) {
             const uint32_t r = (uint32_t)(g + 8 * rr);
-            const int64_t pos = u.base + (int64_t)(r % p.L);
-            high[rr] = r < R ? (int32_t)max((int64_t)-1, min(pos, (int64_t)p.Lk)) : -1;
-            low[rr] = (int32_t)max((int64_t)0, min((int64_t)0x7fffffff, pos - p.window + 1));
+            const int32_t lq = (int32_t)(r % p.L);
+            high[rr] = r < R ? max(-1, min(u.base.pos0 + lq, (int32_t)p.Lk)) : -1;
+            low[rr] = max(0, u.base.low0 + lq);
             if (r < R) {
                 const uint32_t h = hkv * p.G + r / p.L, l = r % p.L;
                 const uint4* src = reinterpret_cast<const uint4*>(p.q + b * p.q_sb + h * p.q_sh + l * p.q_sl + c * (D / 4));
@@ -983,9 +1002,9 @@ __global__ void __launch_bounds__(32 * NW) span_decode_kernel(SpanDecodeParams p
         const uint32_t skip = u.lo - u.s;
         // Virtual keys [open, shut) are seen by every row: from the last
         // query's window on, up to the first query's position.
-        const uint32_t last_low = (uint32_t)max((int64_t)u.lo, min((int64_t)0x7fffffff, u.base + (int64_t)p.L - p.window));
-        const uint32_t open = last_low - skip, shut = (uint32_t)max((int64_t)0, min((int64_t)k_end, u.base + 1 - (int64_t)skip));
-        const int32_t sinks = (int32_t)min((int64_t)0x7fffffff, p.sinks);
+        const uint32_t last_low = (uint32_t)max((int32_t)u.lo, u.base.low0 + (int32_t)p.L - 1);
+        const uint32_t open = last_low - skip, shut = (uint32_t)max(0, min((int32_t)k_end, u.base.pos0 + 1 - (int32_t)skip));
+        const int32_t sinks = p.keys.sinks;
         const uint16_t* kbase = p.k + (uint64_t)b * p.k_sb + (uint64_t)hkv * p.k_sh;
         const uint16_t* vbase = p.v + (uint64_t)b * p.v_sb + (uint64_t)hkv * p.v_sh;
         // One stage: virtual keys v0 .. v0 + 15 of K then V, 16 bytes per copy.
@@ -1353,6 +1372,16 @@ TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared, double
     return g;
 }
 
+SpanKeys span_keys(const SpanArgs& s) {
+    const int64_t big = 1ll << 30, far = 1ll << 40;  // (the window is at most 2^33)
+    const int64_t pos0 = std::clamp(s.offset, -far, far), low0 = pos0 - (int64_t)s.window + 1;
+    SpanKeys k{};
+    k.pos0 = (int32_t)std::clamp(pos0, -big, big), k.low0 = (int32_t)std::clamp(low0, -big, big);
+    k.window = (int32_t)std::min<uint64_t>(s.window, 1u << 30), k.sinks = (int32_t)std::min<uint64_t>(s.sinks, 1u << 30);
+    k.lengths = s.lengths, k.length_stride = s.length_stride;
+    return k;
+}
+
 // A launch that may begin while the stream's previous kernel ends (overlap):
 // the kernel waits for it with griddepcontrol.wait before it touches anything
 // that depends on it, and every one of a chain does so before it ends.
@@ -1405,13 +1434,11 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, const Re
     p.head_blocks = p.H / p.GB;
     p.shared_keys = shared ? 1 : 0;
     p.k_batch_bcast = a.k.batch_bcast ? 1 : 0, p.v_batch_bcast = a.v.batch_bcast ? 1 : 0;
-    p.lengths = shared ? nullptr : s.lengths;
-    p.length_stride = s.length_stride;
-    p.offset = s.offset, p.window = (int64_t)s.window, p.sinks = (int64_t)s.sinks;
+    p.keys = span_keys(s);
+    if (shared) p.keys.lengths = nullptr;
     p.scale_log2 = s.base.scale * 1.4426950408889634f;
     p.shift = shift;
     p.hidden = p.scale_log2 < 0.0f ? INFINITY : -INFINITY;
-    p.sinks32 = (int32_t)std::min<uint64_t>(s.sinks, 0x7fffffff);
     p.splits = (uint32_t)g.splits;
     p.heads = rec.heads, p.stride = rec.count, p.first = first;
     p.out_low = rec.heads ? 0 : s.base.out_low;
@@ -1440,7 +1467,7 @@ int launch_tiles(const SpanArgs& s, const SpanOperands& a, bool shared, const Re
         return FB_ERR_UNSUPPORTED;
     const uint64_t items = g.units * p.groups * p.splits;
     if (items > 0x7fffffffull) return FB_ERR_UNSUPPORTED;
-    p.items = (uint32_t)items;
+    p.units = (uint32_t)g.units, p.items = (uint32_t)items;
     const uint64_t grid = std::min<uint64_t>(items, (uint64_t)sm_count());
     auto kernel = a.fmt ? span_tile_kernel<D, 1> : span_tile_kernel<D, 0>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
@@ -1507,8 +1534,7 @@ int launch_decode(const SpanArgs& s, const SpanOperands& a, const DecodeGrid& g,
     d.v_sb = a.v.batch_bcast ? 0 : a.v.s_batch, d.v_sh = a.v.s_head, d.v_sk = a.v.s_row;
     d.B = (uint32_t)a.B, d.H = (uint32_t)a.H, d.Hkv = (uint32_t)a.Hkv, d.G = (uint32_t)a.G;
     d.L = (uint32_t)a.L, d.Lk = (uint32_t)a.Lk;
-    d.lengths = s.lengths, d.length_stride = s.length_stride;
-    d.offset = s.offset, d.window = (int64_t)s.window, d.sinks = (int64_t)s.sinks;
+    d.keys = span_keys(s);
     d.scale_log2 = s.base.scale * 1.4426950408889634f;
     d.shift = shift;
     d.prefix_heads = prefix.heads, d.prefix = prefix.rows, d.records = prefix.count, d.join = join ? 1 : 0;
