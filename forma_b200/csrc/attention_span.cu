@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             mbar_init(&q_full[t], 1);
             mbar_init(&q_empty[t], 1);
             mbar_init(&s_full[t], 1);
-            mbar_init(&p_half[t], 128);
-            mbar_init(&p_full[t], 128);
+            mbar_init(&p_half[t], 4);
+            mbar_init(&p_full[t], 4);
             mbar_init(&o_done[t], 1);
             mbar_init(&o_free[t], 128);
         }
@@ -639,12 +639,14 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                     if (c == TK / 64 - 1) {  // half of P: its products may start
                         tmem_wait_st();
                         tc_fence_before();
-                        mbar_arrive(&p_half[t]);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&p_half[t]);
                     }
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[t]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
                 const float2 l2 = __fadd2_rn(__fadd2_rn(lsa[0], lsa[1]), __fadd2_rn(lsa[2], lsa[3]));
                 lsum = lsum * alpha + (l2.x + l2.y);
             }

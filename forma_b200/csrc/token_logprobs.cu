@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
 // Bound: HBM (the ex2 unit is 3/4 busy at the full rate with 16-bit logits).
 // Few rows are split over the CTAs of a cluster, each with its own sums and
 // alternatives, joined through distributed shared memory.
-constexpr int WARPS = BLOCK / 32;
+constexpr int SM_WARPS = 32;   // resident warps per SM (64 registers a thread)
 constexpr int CAND = 1024;     // candidates that are put in order by counting
 constexpr int MAX_SEGS = 512;  // segment maxima kept per CTA
 constexpr float L2E = 1.4426950408889634f;
@@ -328,11 +328,12 @@ __device__ __forceinline__ void join_sums(float& m, float& s0, float& s1, float 
 
 // `parts` CTAs (a cluster when > 1) per row, `part_segs` segments of 32 * VPL
 // vectors each; `mult` segments share a kept maximum.
-template <typename T, int VPL>
-__global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
+template <typename T, int VPL, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, SM_WARPS / WARPS) token_stream_kernel(StreamArgs a) {
+    constexpr int THREADS = 32 * WARPS;
     using W = Words<T>;
     constexpr int NW = VPL * 4;
-    __shared__ uint32_t tkey[BLOCK], okey[32];  // maxima of the threads, and of eight lanes each
+    __shared__ uint32_t tkey[THREADS], okey[32];  // maxima of the threads, and of WARPS lanes each
     __shared__ uint32_t seg_max[MAX_SEGS];
     __shared__ uint64_t cand[CAND];
     __shared__ uint64_t scan_keys[WARPS];
@@ -437,8 +438,8 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
             uint32_t key = Bits<T>::key(W::top(own_max));
             tkey[threadIdx.x] = key;
 #pragma unroll
-            for (int o = 1; o < 8; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-            if (lane % 8 == 0) okey[threadIdx.x / 8] = key;
+            for (int o = 1; o < WARPS; o <<= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+            if (lane % WARPS == 0) okey[threadIdx.x / WARPS] = key;
         }
     }
     __syncthreads();
@@ -465,9 +466,9 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         const uint32_t k = a.top;
         if (parts > 1 && threadIdx.x < FB_MAX_TOP) mine.top[threadIdx.x] = 0ull;
         // t: the largest 16-bit prefix that k maxima reach, bit by bit, found
-        // by each warp for itself: of the octets' 32 maxima for few
+        // by each warp for itself: of the lane groups' 32 maxima for few
         // alternatives (k = 20 leaves about 30 values to put in order), else of
-        // the 256 threads'.
+        // the threads'.
         constexpr int SHIFT = W::E == 8 ? 0 : 16;
         uint32_t t = 0;
         if (k <= 20) {
@@ -476,14 +477,14 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
             for (uint32_t bit = 0x8000u; bit; bit >>= 1)
                 if (__popc(__ballot_sync(0xffffffffu, v >= (t | bit))) >= k) t |= bit;
         } else {
-            uint32_t v[8];
+            uint32_t v[WARPS];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = tkey[i * 32 + lane] >> SHIFT;
+            for (int i = 0; i < WARPS; ++i) v[i] = tkey[i * 32 + lane] >> SHIFT;
 #pragma unroll 1
             for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
                 uint32_t n = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) n += v[i] >= (t | bit);
+                for (int i = 0; i < WARPS; ++i) n += v[i] >= (t | bit);
                 if (__reduce_add_sync(0xffffffffu, n) >= k) t |= bit;
             }
         }
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         const uint32_t n = n_cand;
         if (fine && n <= CAND) {
             // Places by counting; a whole row's go out from here.
-            for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
+            for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
                 const uint64_t me = cand[i];
                 uint32_t rank = 0;
 #pragma unroll 4
@@ -548,12 +549,12 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
             uint64_t bound = ~0ull;
             for (uint32_t r = 0; r < k && bound; ++r) {
                 uint64_t best = 0;
-                for (uint64_t v = v0 + threadIdx.x; v < v1; v += BLOCK) {
+                for (uint64_t v = v0 + threadIdx.x; v < v1; v += THREADS) {
                     const uint64_t q = ((uint64_t)Bits<T>::key(__ldg(rv.x + (v - rv.head))) << 32) |
                                        (0xffffffffu - (uint32_t)(v - rv.head));
                     if (q < bound && q > best) best = q;
                 }
-                bound = block_max_u64<BLOCK>(best, scan_keys);
+                bound = block_max_u64<THREADS>(best, scan_keys);
                 if (threadIdx.x != 0) continue;
                 if (parts > 1) {
                     mine.top[r] = bound;
@@ -575,7 +576,7 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         }
     };
     if (parts == 1) {
-        if (threadIdx.x == BLOCK - 1) store_row(ls);
+        if (threadIdx.x == THREADS - 1) store_row(ls);
         return;
     }
     if (threadIdx.x == 0) mine.m = M, mine.s0 = S0, mine.s1 = S1;
@@ -584,17 +585,17 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
         const uint32_t at = (uint32_t)__cvta_generic_to_shared(&mine);
         const uint32_t off = (uint32_t)(reinterpret_cast<const char*>(mine.top) - reinterpret_cast<const char*>(&mine));
         const uint32_t n = parts * a.top;
-        for (uint32_t i = threadIdx.x; i < n; i += BLOCK)
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS)
             cand[i] = ld_peer_u64(mapa_rank(at + off, i / a.top) + (i % a.top) * 8);
         for (uint32_t p = 1; p < parts; ++p) {
             const uint32_t peer = mapa_rank(at, p);
             join_sums(M, S0, S1, ld_peer_f32(peer), ld_peer_f32(peer + 4), ld_peer_f32(peer + 8));
         }
         const float lsr = S0 == 0.0f ? row_nan() : logf(S0);
-        if (threadIdx.x == BLOCK - 1) store_row(lsr);
+        if (threadIdx.x == THREADS - 1) store_row(lsr);
         __syncthreads();
         // the parts' alternatives in one list: places by counting
-        for (uint32_t i = threadIdx.x; i < n; i += BLOCK) {
+        for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
             const uint64_t me = cand[i];
             if (me == 0) continue;
             uint32_t rank = 0;
@@ -608,7 +609,7 @@ __global__ void __launch_bounds__(BLOCK, 4) token_stream_kernel(StreamArgs a) {
     sync_cluster();  // a part's sums and list stay until they are read
 }
 
-template <typename T, int VPL>
+template <typename T, int VPL, int WARPS>
 int launch_stream(const TokenArgs& a, cudaStream_t st) {
     const Rows& in = a.logits;
     const uint64_t E = Words<T>::E, seg = 32 * VPL;
@@ -626,7 +627,7 @@ int launch_stream(const TokenArgs& a, cudaStream_t st) {
     if (in.rows * parts > 0x7fffffffull || nseg > 0xffffffffull) return FB_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(in.rows * parts));
-    cfg.blockDim = dim3(BLOCK);
+    cfg.blockDim = dim3(32 * WARPS);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -643,7 +644,7 @@ int launch_stream(const TokenArgs& a, cudaStream_t st) {
         return FB_ERR_UNSUPPORTED;
     k.top_logprob = a.top_logprob, k.top_index = a.top_index, k.top = a.top;
     k.parts = (uint32_t)parts, k.part_segs = (uint32_t)part_segs, k.mult = (uint32_t)mult;
-    (void)cudaLaunchKernelEx(&cfg, token_stream_kernel<T, VPL>, k);
+    (void)cudaLaunchKernelEx(&cfg, token_stream_kernel<T, VPL, WARPS>, k);
     count_launch("token_stream_kernel");
     return launch_status("kernel launch");
 }
@@ -653,7 +654,17 @@ int launch_t(const TokenArgs& a, cudaStream_t st) {
     if (a.logits.contiguous_rows) {
         // Short rows: one vector per lane and segment, so that every warp has
         // one from 8 * 32 vectors on.
-        const int r = a.logits.cols <= (uint64_t)Words<T>::E * 32 * 4 * WARPS ? launch_stream<T, 1>(a, st) : launch_stream<T, 4>(a, st);
+        const bool brief = a.logits.cols <= (uint64_t)Words<T>::E * 32 * 4 * 8;
+        // CTAs of four warps leave less of an SM idle while one of them puts
+        // its alternatives in order; of eight, a last wave is shorter.  Four
+        // where the rows fill the GPU and their waves (twice as long) cost at
+        // most an eighth more.  Top 5, us, four | eight: 8200 x 32000 152 |
+        // 171, 700 x 16000 17 | 19, 740 x 131072 60 | 64, 2048 x 131072 127 |
+        // 127; where the rule keeps eight, 1776 x 131072 118 | 109.
+        const uint64_t slots = (uint64_t)sm_count() * (SM_WARPS / 8), waves = (a.logits.rows + slots - 1) / slots;
+        const bool four = a.logits.rows > slots && 16 * ((waves + 1) / 2) <= 9 * waves;
+        const int r = brief ? four ? launch_stream<T, 1, 4>(a, st) : launch_stream<T, 1, 8>(a, st)
+                            : four ? launch_stream<T, 4, 4>(a, st) : launch_stream<T, 4, 8>(a, st);
         if (r != FB_ERR_UNSUPPORTED) return r;
     }
     const unsigned blocks = (unsigned)std::min<uint64_t>(a.logits.rows, (uint64_t)sm_count() * 32);
