@@ -144,6 +144,14 @@ struct TileItem {
     // then those from far[t] on.
     uint32_t n_t[2], near[2], far[2];
     SpanBase base;
+    // Virtual keys that no query of the item sees although its tiles hold
+    // them: [gap0, gap1), between the first keys and the window (under 16),
+    // and those from stop on.  A weight of 0 does not make up for a NaN or an
+    // infinity in their value rows.  Queries of other items may see some of
+    // them; where the item's last tile holds only such (stop of 2^31 - 1), or
+    // zeros past the tensor's end, they are left as they are.
+    uint32_t gap0, gap1;
+    int32_t stop;
     static __device__ __forceinline__ uint32_t after(uint32_t j, uint32_t near, uint32_t far) {
         return j + 1 < near ? j + 1 : max(j + 1, far);
     }
@@ -163,6 +171,7 @@ struct TileItem {
             j0 = min(split * per, all);
             n_kv = min(per, all - j0);
             s16 = lo = 0;
+            gap0 = gap1 = 0, stop = 0x7fffffff;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const uint32_t tile = group * 2 + t;
@@ -188,10 +197,20 @@ struct TileItem {
             if (rc[t].lo <= rc[t].hi) start = min(start, rc[t].lo), last = max(last, rc[t].hi);
         }
         uint32_t s = (uint32_t)(first + 15) / 16 * 16, end;
-        if (last < 0) s = 0, start = 0, end = (uint32_t)first;                            // the first keys alone
-        else if ((uint32_t)start <= s) s = 0, start = 0, end = (uint32_t)last + 1;        // one run
-        else end = s + (uint32_t)(last - start) + 1;
+        gap0 = gap1 = (uint32_t)first;
+        if (last < 0) {  // the first keys alone
+            s = 0, start = 0, end = (uint32_t)first;
+        } else if ((uint32_t)start <= s) {  // one run
+            gap1 = (uint32_t)max(first, start);
+            s = 0, start = 0, end = (uint32_t)last + 1;
+        } else {
+            gap1 = s;
+            end = s + (uint32_t)(last - start) + 1;
+        }
+        if (base.low0 <= first) gap1 = gap0;  // the call's earliest window reaches down to the first keys
         s16 = s, lo = (uint32_t)start;
+        const int32_t seen = last < 0 ? first : min(base.filled, base.pos0 + (int32_t)p.L);
+        stop = seen < (int32_t)p.Lk ? seen + shift() : 0x7fffffff;
         const uint32_t all = (end + TK - 1) / TK, per = p.splits > 1 ? (all + p.splits - 1) / p.splits : all;
         j0 = min(split * per, all);
         const uint32_t j1 = min(j0 + per, all);
@@ -410,6 +429,12 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
         const uint32_t idesc_s = f16_idesc(FMT, TQ, TK);
         const uint32_t idesc_o = f16_idesc(FMT, TQ, D) | (1u << 16);  // B (V) is MN-major
         auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); };
+        // Descriptors are made where they are used: kept over the loop they
+        // would take more registers than there are.
+        auto opaque = [](uint32_t v) {
+            asm volatile("" : "+r"(v));
+            return v;
+        };
         bool ok = true;
         // g: ring index of the item's first K / V; taken: S_t / PV_t pairs so
         // far; outs: items in which tile t had any
@@ -419,13 +444,14 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             const TileItem& it = plans[n % PLANS];
             const uint32_t n_kv = it.n_kv, n_t[2] = {it.n_t[0], it.n_t[1]}, near[2] = {it.near[0], it.near[1]},
                            far[2] = {it.far[0], it.far[1]};
+            const bool gap = it.gap1 > it.gap0;
             // left: S_t still to come in this item
             auto issue_s = [&](int t, uint32_t j, uint32_t left) -> bool {
                 const uint32_t s = (g + j) % C::STAGES;
                 if (!wait(&k_full[s], ((g + j) / C::STAGES) & 1)) return false;
                 tc_fence_after();
-                const uint64_t qd = sw128_desc(smem_u32(sQ + t * C::Q_BYTES));
-                const uint64_t kd = sw128_desc(smem_u32(sKV + s * C::STAGE_BYTES));
+                const uint64_t qd = sw128_desc(opaque(smem_u32(sQ + t * C::Q_BYTES)));
+                const uint64_t kd = sw128_desc(opaque(smem_u32(sKV + s * C::STAGE_BYTES)));
                 const uint32_t d = tmem + C::s_col(t);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
@@ -443,7 +469,7 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 // before it must have been read out
                 if (i == 0 && !wait(&o_free[t], (outs[t] & 1) ^ 1)) return false;
                 tc_fence_after();
-                const uint64_t vd = sw128_mn_desc(smem_u32(sKV + s * C::STAGE_BYTES + C::K_BYTES), TK * 128);
+                const uint64_t vd = sw128_mn_desc(opaque(smem_u32(sKV + s * C::STAGE_BYTES + C::K_BYTES)), TK * 128);
                 const uint32_t d = tmem + C::o_col(t), a = tmem + C::s_col(t);
                 umma_f16_ts_warp(d, a, vd, idesc_o, i != 0);
 #pragma unroll
@@ -472,13 +498,17 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
             for (uint32_t j = 0; ok && j < n_kv; ++j) {
                 const uint32_t s = (g + j) % C::STAGES;
                 ok = wait(&v_full[s], ((g + j) / C::STAGES) & 1);
-                if (ok && p.keys.lengths && j + 1 == n_kv && it.base.filled + it.shift() < (int32_t)((it.j0 + n_kv) * TK)) {
-                    // value rows past the filled keys (in the last tile, if any): zeros
-                    const uint32_t from = (uint32_t)max(it.base.filled + it.shift() - (int32_t)((it.j0 + j) * TK), 0);
+                if (ok && ((gap && it.gap0 / TK == it.j0 + j) || (j + 1 == n_kv && it.stop < (int32_t)((it.j0 + n_kv) * TK)))) {
+                    // value rows that no query of the item sees: zeros
+                    const uint32_t v0 = (it.j0 + j) * TK;
                     unsigned char* v = sKV + s * C::STAGE_BYTES + C::K_BYTES;
-                    for (int b = 0; b < C::BOXES; ++b)
-                        for (uint32_t o = from * 128 + lane * 16; o < TK * 128; o += 512)
-                            *reinterpret_cast<uint4*>(v + b * (TK * 128) + o) = make_uint4(0u, 0u, 0u, 0u);
+                    auto clear = [&](uint32_t from, uint32_t to) {
+                        for (int b = 0; b < C::BOXES; ++b)
+                            for (uint32_t o = from * 128 + lane * 16; o < to * 128; o += 512)
+                                *reinterpret_cast<uint4*>(v + b * (TK * 128) + o) = make_uint4(0u, 0u, 0u, 0u);
+                    };
+                    if (gap && it.gap0 / TK == it.j0 + j) clear(it.gap0 - v0, min(it.gap1 - v0, (uint32_t)TK));
+                    if (it.stop < (int32_t)(v0 + TK)) clear((uint32_t)max(it.stop - (int32_t)v0, 0), TK);
                     fence_proxy_async_smem();
                     __syncwarp();
                 }

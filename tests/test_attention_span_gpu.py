@@ -333,3 +333,79 @@ def test_refusals(cuda):
     # empty outputs return before any launch
     assert w(q[:, :, :0], k, k, 4).shape == (2, 4, 0, 64)
     assert p(q[:0], pk, pk, k[:0], k[:0]).shape == (0, 4, 3, 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,sinks,window,offset", [(40, 5, 30, 100), (200, 5, 30, 60), (40, 0, 30, 100), (70, 17, 9, 200),
+                                                    (33, 130, 20, 135), (40, 3, 500, 20), (50, 7, 4, 5000), (1, 5, 30, 100)])
+def test_window_keys_hidden_from_every_query_may_hold_anything(cuda, dtype, d, lq, sinks, window, offset):
+    """NaN and infinities between the first keys and the windows and past the
+    last position (a cache whose middle was given away) do not reach the result."""
+    keys = 400
+    q, k, v = rnd((2, 4, lq, d), dtype, 40), rnd((2, 2, keys, d), dtype, 41), rnd((2, 2, keys, d), dtype, 42)
+    seen = seen_mask(2, lq, keys, window, sinks, None, offset)
+    exp = attend64(q, [(k, v, seen)], d**-0.5)
+    top = float(v.double().abs().max())
+    hidden = ~seen.any(1)[0]
+    assert hidden.any()
+    k[:, :, hidden], v[:, :, hidden] = torch.nan, torch.inf
+    v[:, 0, hidden] = torch.nan
+    check(api.attention_window(q, k, v, window, sinks, None, AttentionOptions(causal=offset)), exp, dtype, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lq", [20, 90])
+def test_window_lengths_and_hidden_middle(cuda, dtype, lq):
+    """The same for filled lengths, a sequence each."""
+    keys, sinks, window = 600, 9, 50
+    ln = torch.tensor([600, 333, 150, lq], dtype=torch.int32, device="cuda")
+    q, k, v = rnd((4, 2, lq, 128), dtype, 43), rnd((4, 1, keys, 128), dtype, 44), rnd((4, 1, keys, 128), dtype, 45)
+    seen = seen_mask(4, lq, keys, window, sinks, ln, None)
+    exp = attend64(q, [(k, v, seen)], 128**-0.5)
+    top = float(v.double().abs().max())
+    for b in range(4):
+        hidden = ~seen[b].any(0)
+        k[b, :, hidden], v[b, :, hidden] = torch.inf, torch.nan
+    check(api.attention_window(q, k, v, window, sinks, ln), exp, dtype, top)
+
+
+@pytest.mark.parametrize("lq", [2, 40])
+def test_prefix_keys_past_the_last_query_may_hold_anything(cuda, lq):
+    q, pk, pv = rnd((2, 4, lq, 64), torch.bfloat16, 46), rnd((2, 70, 64), torch.bfloat16, 47), rnd((2, 70, 64), torch.bfloat16, 48)
+    k, v = rnd((2, 2, 100, 64), torch.bfloat16, 49), rnd((2, 2, 100, 64), torch.bfloat16, 50)
+    seen = seen_mask(2, lq, 100, 1 << 30, 0, None, 3)
+    exp = attend64(q, [(pk[None].expand(2, -1, -1, -1), pv[None].expand(2, -1, -1, -1), None), (k, v, seen)], 64**-0.5)
+    top = max(float(v.double().abs().max()), float(pv.double().abs().max()))
+    k[:, :, 3 + lq:], v[:, :, 3 + lq:] = torch.nan, torch.nan
+    check(api.attention_prefix(q, pk, pv, k, v, None, AttentionOptions(causal=3)), exp, torch.bfloat16, top)
+
+
+def routes(fn):
+    fn()
+    return api.last_route()
+
+
+def test_routes(cuda):
+    """Which kernels serve which shapes: tiles from 17 rows per key/value head
+    on, the streaming kernel below, the generic one for other geometries."""
+    def window(lq, d, dtype, keys=300, b=2):
+        q, k = rnd((b, 4, lq, d), dtype, 1), rnd((b, 2, keys, d), dtype, 2)
+        return routes(lambda: api.attention_window(q, k, k, 100, 4))
+
+    def prefix(lq, d, dtype):
+        q, k, pk = rnd((2, 4, lq, d), dtype, 1), rnd((2, 2, 30, d), dtype, 2), rnd((2, 500, d), dtype, 3)
+        return routes(lambda: api.attention_prefix(q, pk, pk, k, k))
+
+    assert window(9, 128, torch.bfloat16) == ["span_tile_kernel<128,0>"]
+    assert window(9, 64, torch.float16) == ["span_tile_kernel<64,0>"]
+    assert window(8, 128, torch.bfloat16) == ["span_decode_kernel<128,1,4>"]
+    assert window(1, 64, torch.float16) == ["span_decode_kernel<64,0,4>"]
+    assert window(1, 64, torch.float16, b=400) == ["span_decode_kernel<64,0,2>"]
+    assert window(9, 40, torch.bfloat16) == ["span_simt_kernel"]
+    assert window(1, 128, torch.float32) == ["span_simt_kernel"]
+    got = prefix(1, 128, torch.bfloat16)
+    assert got[0] == "span_tile_kernel<128,1>" and got[1].startswith("span_decode_kernel<128,1,"), got
+    got = prefix(40, 64, torch.float16)
+    assert got == ["span_tile_kernel<64,1>", "span_tile_kernel<64,0>", "span_merge_kernel<64>"], got
+    assert prefix(3, 24, torch.bfloat16) == ["span_simt_kernel"]
