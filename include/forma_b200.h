@@ -249,7 +249,8 @@ int fb_attention_low(const fb_tensor* query, const fb_tensor* key,
  * Without lengths n_b = Lk and p = i + options.causal when
  * options.has_causal, else Lk - L + i; giving both is
  * FB_ERR_INVALID_ATTENTION.  Keys that a query's mask hides but that another
- * query of the call may see must hold finite values.
+ * query of the call may see must hold finite values; keys that no query of
+ * the call sees may hold anything.
  *
  * fb_attention_window: key j is visible iff j < n_b, j <= p and
  * (j > p - window or j < sinks): the last `window` positions and the first

@@ -409,3 +409,49 @@ def test_routes(cuda):
     got = prefix(40, 64, torch.float16)
     assert got == ["span_tile_kernel<64,1>", "span_tile_kernel<64,0>", "span_merge_kernel<64>"], got
     assert prefix(3, 24, torch.bfloat16) == ["span_simt_kernel"]
+
+
+@pytest.mark.parametrize("lq,d", [(1, 128), (40, 128), (2, 40)])
+def test_caches_past_32_bit_offsets(cuda, lq, d):
+    """Windows behind 2^32 elements of one head's cache; what lies between the
+    first keys and the windows is whatever the memory held."""
+    keys, window, sinks = (1 << 32) // d + 5000, 300, 4
+    q = rnd((1, 2, lq, d), torch.bfloat16, 60)
+    k, v = (torch.empty((1, 1, keys, d), dtype=torch.bfloat16, device=cuda) for _ in range(2))
+    first, tail = sinks, window + lq - 1
+    for t, s in ((k, 61), (v, 62)):
+        t[:, :, :first], t[:, :, keys - tail:] = rnd((1, 1, first, d), torch.bfloat16, s), rnd((1, 1, tail, d), torch.bfloat16, s + 5)
+    got = api.attention_window(q, k, v, window, sinks, torch.tensor([keys], dtype=torch.int32, device=cuda))
+    kk, vv = (torch.cat([t[:, :, :first], t[:, :, keys - tail:]], 2) for t in (k, v))
+    exp = attend64(q, [(kk, vv, seen_mask(1, lq, first + tail, window, sinks, None, None))], d**-0.5)
+    check(got, exp, torch.bfloat16, float(vv.double().abs().max()))
+    assert api.device_status() == 0
+    del k, v
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("b,lq", [(300, 1), (700, 1), (150, 6), (37, 20)])
+def test_window_many_ragged_sequences(cuda, b, lq):
+    """More sequences than a block scans at once, lengths from 0 to all keys."""
+    keys = 900
+    g = torch.Generator().manual_seed(b)
+    ln = torch.randint(0, keys + 1, (b,), generator=g).tolist()
+    ln[0], ln[-1] = 0, keys
+    for dtype in (torch.bfloat16, torch.float16):
+        window_case(b, 4, 2, 64, lq, keys, 200, 3, dtype, ln)
+
+
+@pytest.mark.parametrize("b", [3, 130])
+@pytest.mark.parametrize("lq", [1, 17])
+def test_prefix_ragged_sequences(cuda, b, lq):
+    keys = 600
+    g = torch.Generator().manual_seed(b)
+    ln = torch.randint(0, keys + 1, (b,), generator=g, dtype=torch.int32)
+    ln[0] = 0
+    q, pk, pv = rnd((b, 8, lq, 128), torch.bfloat16, 70), rnd((2, 777, 128), torch.bfloat16, 71), rnd((2, 777, 128), torch.bfloat16, 72)
+    k, v = rnd((b, 2, keys, 128), torch.bfloat16, 73), rnd((b, 2, keys, 128), torch.bfloat16, 74)
+    got = api.attention_prefix(q, pk, pv, k, v, ln.cuda())
+    seen = seen_mask(b, lq, keys, 1 << 30, 0, ln.cuda(), None)
+    exp = attend64(q, [(pk[None].expand(b, -1, -1, -1), pv[None].expand(b, -1, -1, -1), None), (k, v, seen)], 128**-0.5)
+    check(got, exp, torch.bfloat16, max(float(v.double().abs().max()), float(pv.double().abs().max())))
+    assert api.device_status() == 0

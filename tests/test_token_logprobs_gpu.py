@@ -297,3 +297,48 @@ def test_refusals(cuda):
     refused("InvalidInput", g, x, t, st.logsumexp, gl, out=torch.empty((4, 99), dtype=x.dtype, device=cuda))
     both = torch.empty((5, 100), dtype=x.dtype, device=cuda)
     refused("InvalidInput", g, both[:4], t, st.logsumexp, gl, out=both[1:])
+
+
+@pytest.mark.parametrize("dtype,cols", [(torch.float32, 1_100_003), (torch.bfloat16, 2_200_001), (torch.float16, 2_200_000)])
+@pytest.mark.parametrize("top", [1, 20, 64])
+def test_forward_many_classes(cuda, dtype, cols, top):
+    """Rows longer than a maximum per segment is kept for."""
+    x = rnd((2, cols), dtype, 80)
+    check_forward(x, targets_for(x, 81), top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(700, 900), (700, 9001), (1300, 20000)])
+@pytest.mark.parametrize("top", [0, 5, 33])
+def test_forward_rows_that_fill_the_gpu(cuda, dtype, rows, cols, top):
+    """More rows than eight-warp blocks are resident: odd columns break the
+    rows' alignment; a NaN, a -inf and a constant row among them."""
+    x = rnd((rows, cols), dtype, 82)
+    t = targets_for(x, 83)
+    t[3] = NO_TOKEN
+    check_forward(x, t, top)
+    x[5, cols // 2], x[6], x[7] = torch.nan, -torch.inf, 1.5
+    r = api.token_logprobs(x, t, top)
+    assert r.logsumexp[5:7].isnan().all() and r.entropy[5:7].isnan().all()
+    keep = [i for i in range(rows) if i not in (5, 6)]
+    check_forward(x[keep], t[keep], top, api.TokenLogprobs(*(None if f is None else f[keep] for f in vars(r).values())))
+
+
+def test_logits_past_32_bit_offsets(cuda):
+    """More than 2^32 logits: the last rows' results are those of the rows alone."""
+    rows, cols = 33000, 131072
+    x = torch.empty((rows, cols), dtype=torch.bfloat16, device=cuda)
+    for i in range(0, rows, 3000):
+        x[i:i + 3000] = rnd((min(3000, rows - i), cols), torch.bfloat16, 84 + i)
+    t = torch.arange(rows, device=cuda, dtype=torch.int32) % cols
+    r = api.token_logprobs(x, t, 5)
+    for part in (slice(0, 3), slice(rows - 3, rows)):
+        check_forward(x[part], t[part], 5, api.TokenLogprobs(*(f[part] for f in vars(r).values())))
+    gl = torch.ones(rows, device=cuda)
+    ends = x[-3:].clone()
+    exp = api.token_logprobs_grad(ends, t[-3:], r.logsumexp[-3:], gl[-3:], r.entropy[-3:], gl[-3:])
+    api.token_logprobs_grad(x, t, r.logsumexp, gl, r.entropy, gl, out=x)
+    assert torch.equal(x[-3:], exp)
+    assert api.device_status() == 0
+    del x
+    torch.cuda.empty_cache()
