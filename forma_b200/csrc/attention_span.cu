@@ -1432,6 +1432,8 @@ void launch_after(void (*kernel)(P...), unsigned grid, unsigned threads, size_t 
     (void)cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+constexpr uint64_t RECORD_BYTES = 1ull << 30;
+
 // Records of every query row, `count` each: heads, then rows; heads null: none.
 struct Records {
     float2* heads = nullptr;
@@ -1592,6 +1594,28 @@ int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
     const uint64_t ps = pg.splits;
     const uint64_t rows = a.B * a.H * a.L;
     Records rec;
+    // Records of a prefix and of own keys, for as many sequences at a time as
+    // keep them within RECORD_BYTES: a launch fills the GPU long before that.
+    if (prefix && a.B > 1 && rows * (ps + 1) * (D * sizeof(float) + sizeof(float2)) > RECORD_BYTES) {
+        const uint64_t bytes = a.H * a.L * (ps + 1) * (D * sizeof(float) + sizeof(float2));
+        const uint64_t step = std::min(a.B - 1, std::max<uint64_t>(1, RECORD_BYTES / bytes));
+        for (uint64_t b = 0; b < a.B; b += step) {
+            SpanArgs sb = s;
+            SpanOperands ab = a;
+            ab.B = std::min(step, a.B - b);
+            auto part = [&](RowsLayout& l) {
+                if (!l.batch_bcast) l.batch = ab.B;
+                return l.batch_bcast ? 0 : b * l.s_batch;
+            };
+            ab.qp = static_cast<const uint16_t*>(a.qp) + part(ab.q);
+            ab.kp = static_cast<const uint16_t*>(a.kp) + part(ab.k);
+            ab.vp = static_cast<const uint16_t*>(a.vp) + part(ab.v);
+            ab.op = static_cast<char*>(a.op) + part(ab.o) * (s.base.out_low ? 2 : 4);
+            if (s.lengths) sb.lengths = s.lengths + b * s.length_stride;
+            if (int r = launch_span<D>(sb, ab, st); r != FB_OK) return r;
+        }
+        return FB_OK;
+    }
     if (a.G * a.L <= 16) {  // few rows: the own keys streamed, the prefix's records joined there
         DecodeGrid dg;
         if (!decode_grid(s, a, &dg)) return FB_ERR_UNSUPPORTED;

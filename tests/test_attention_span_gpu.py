@@ -455,3 +455,27 @@ def test_prefix_ragged_sequences(cuda, b, lq):
     exp = attend64(q, [(pk[None].expand(b, -1, -1, -1), pv[None].expand(b, -1, -1, -1), None), (k, v, seen)], 128**-0.5)
     check(got, exp, torch.bfloat16, max(float(v.double().abs().max()), float(pv.double().abs().max())))
     assert api.device_status() == 0
+
+
+@pytest.mark.parametrize("lq,b,low", [(300, 900, True), (120, 1300, False)])
+def test_prefix_more_records_than_are_kept_at_once(cuda, lq, b, low):
+    """A batch whose intermediate results exceed the scratch bound runs in
+    parts: sequences of every part against the same sequences alone."""
+    keys = lq + 10
+    g = torch.Generator().manual_seed(9)
+    ln = torch.randint(lq // 2, keys + 1, (b,), generator=g, dtype=torch.int32).cuda()
+    q = rnd((b, 8, lq, 64 if low else 128), torch.bfloat16, 90)
+    d = q.shape[-1]
+    pk, pv = rnd((2, 200, d), torch.bfloat16, 91), rnd((2, 200, d), torch.bfloat16, 92)
+    k, v = rnd((b, 2, keys, d), torch.bfloat16, 93), rnd((b, 2, keys, d), torch.bfloat16, 94)
+    out = torch.full(q.shape, torch.nan, dtype=torch.bfloat16 if low else torch.float32, device=cuda)
+    api.attention_prefix(q, pk, pv, k, v, ln, out=out)
+    assert len(api.last_route()) > 3
+    assert torch.isfinite(out).all()
+    some = [0, 1, b // 3, b // 2, (2 * b) // 3, b - 2, b - 1]
+    exp = attend64(q[some], [(pk[None].expand(len(some), -1, -1, -1), pv[None].expand(len(some), -1, -1, -1), None),
+                             (k[some], v[some], seen_mask(len(some), lq, keys, 1 << 30, 0, ln[some], None))], d**-0.5)
+    top = max(float(v.double().abs().max()), float(pv.double().abs().max()))
+    got = out[some]
+    check(got, exp, torch.bfloat16, top)
+    assert api.device_status() == 0
