@@ -682,11 +682,11 @@ int launch_t(const TokenArgs& a, cudaStream_t st) {
 // 0 or infinity.
 // Bound: HBM, one read and one write.  Loads are issued before the row's
 // scalars arrive; each block does one chunk of 4 vectors per thread.
-template <typename T>
+template <typename T, typename U>  // U: patterns of the output, T's own or f32's
 __global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(GradArgs a) {
     using W = Words<T>;
-    using U = typename Bits<T>::U;
     constexpr int E = W::E, N = 4;
+    constexpr bool LOW = sizeof(U) == 2;
     const uint64_t row = blockIdx.x / a.chunks;
     const uint64_t j0 = (uint64_t)(blockIdx.x % a.chunks) * (N * BLOCK) + threadIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
@@ -727,19 +727,22 @@ __global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(GradArgs a) {
             for (int e = 0; e < E; ++e)
                 if (at == v + e) g[e] += gl;
         }
-        uint32_t o[4];
+        constexpr int WORDS = E * sizeof(U) / 4;
+        uint32_t o[WORDS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (E == 8) o[e] = encode_low_pair(g[2 * e], g[2 * e + 1], std::is_same<T, __half>::value ? FB_F16 : FB_BF16);
+        for (int e = 0; e < WORDS; ++e) {
+            if constexpr (LOW) o[e] = encode_low_pair(g[2 * e], g[2 * e + 1], std::is_same<T, __half>::value ? FB_F16 : FB_BF16);
             else o[e] = __float_as_uint(g[e]);
         }
         if (v >= rv.head && v + E <= rv.end) {
-            __stcs(reinterpret_cast<uint4*>(out + (v - rv.head)), make_uint4(o[0], o[1], o[2], o[3]));
+#pragma unroll
+            for (int e = 0; e < WORDS; e += 4)
+                __stcs(reinterpret_cast<uint4*>(out + (v - rv.head)) + e / 4, make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e)
                 if (v + e >= rv.head && v + e < rv.end) {
-                    if constexpr (E == 8) out[v + e - rv.head] = (U)(e % 2 ? o[e / 2] >> 16 : o[e / 2] & 0xffffu);
+                    if constexpr (LOW) out[v + e - rv.head] = (U)(e % 2 ? o[e / 2] >> 16 : o[e / 2] & 0xffffu);
                     else out[v + e - rv.head] = o[e];
                 }
         }
@@ -750,11 +753,12 @@ template <typename T>
 int launch_grad_t(const TokenGradArgs& a, cudaStream_t st) {
     const Rows& in = a.logits;
     constexpr uint64_t esz = sizeof(typename Bits<T>::U);
-    const uint32_t dtype = std::is_same<T, float>::value ? FB_F32 : std::is_same<T, __half>::value ? FB_F16 : FB_BF16;
+    const uint64_t osz = a.out.dtype == FB_F32 ? 4 : esz, step = 16 / osz;  // step: output elements of 16 bytes
     const uintptr_t x0 = reinterpret_cast<uintptr_t>(in.data) + in.offset * esz;
-    const uintptr_t o0 = reinterpret_cast<uintptr_t>(a.out.data) + a.out.offset * esz;
-    if (in.contiguous_rows && a.out.contiguous_rows && a.out.dtype == dtype && (x0 - o0) % 16 == 0 &&
-        (in.row_stride - a.out.row_stride) * esz % 16 == 0) {
+    const uintptr_t o0 = reinterpret_cast<uintptr_t>(a.out.data) + a.out.offset * osz;
+    // Output elements sit in their 16 bytes as the logits do in theirs.
+    if (in.contiguous_rows && a.out.contiguous_rows && (x0 / esz - o0 / osz) % step == 0 &&
+        (in.row_stride - a.out.row_stride) % step == 0) {
         const uint64_t vectors = (in.cols + 2 * Words<T>::E - 2) / Words<T>::E, chunks = (vectors + 4 * BLOCK - 1) / (4 * BLOCK);
         GradArgs k{};
         const bool strided = row_vec(const_cast<uint32_t*>(a.targets), a.target_offset, a.target_nest, &k.targets) &&
@@ -764,7 +768,8 @@ int launch_grad_t(const TokenGradArgs& a, cudaStream_t st) {
             k.x = reinterpret_cast<const void*>(x0), k.out = reinterpret_cast<void*>(o0);
             k.cols = in.cols, k.x_stride = in.row_stride, k.out_stride = a.out.row_stride;
             k.chunks = (uint32_t)chunks;
-            token_grad_stream_kernel<T><<<(unsigned)(in.rows * chunks), BLOCK, 0, st>>>(k);
+            if (osz == esz) token_grad_stream_kernel<T, typename Bits<T>::U><<<(unsigned)(in.rows * chunks), BLOCK, 0, st>>>(k);
+            else token_grad_stream_kernel<T, uint32_t><<<(unsigned)(in.rows * chunks), BLOCK, 0, st>>>(k);
             count_launch("token_grad_stream_kernel");
             return launch_status("kernel launch");
         }

@@ -342,3 +342,22 @@ def test_logits_past_32_bit_offsets(cuda):
     assert api.device_status() == 0
     del x
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(3, 7), (5, 4099), (60, 9001), (2, 32000)])
+def test_grad_in_f32(cuda, dtype, rows, cols):
+    """f32 gradients of 16-bit logits: odd columns move the rows' alignment, an
+    offset that keeps it and one that does not."""
+    x = rnd((rows, cols), dtype, 85)
+    t = targets_for(x, 86)
+    gl, gh = rnd((rows,), torch.float32, 87), rnd((rows,), torch.float32, 88)
+    check_grad(x, t, gl, gh, torch.empty((rows, cols), device=cuda))
+    assert api.last_route() == ["token_grad_stream_kernel"]
+    n = rows * cols
+    check_grad(x, t, gl, None, torch.empty(n + 4, device=cuda)[4:].view(rows, cols))
+    assert api.last_route() == ["token_grad_stream_kernel"]
+    got = torch.full((n + 3,), 7.0, device=cuda)
+    check_grad(x, t, gl, None, got[1:1 + n].view(rows, cols))
+    assert api.last_route() == ["token_grad_rows_kernel"]
+    assert got[0] == 7 and (got[1 + n:] == 7).all()
