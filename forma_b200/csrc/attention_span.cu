@@ -69,14 +69,15 @@ __device__ __forceinline__ Reach reach(const SpanBase& s, int32_t la, int32_t lb
 // whatever Q's strides are.  A work item is two tiles and the key tiles that
 // either sees; a tile of rows takes part only in the key tiles that it sees.
 // CTAs are persistent, one per SM: the next item's loads start while this
-// one's last products and epilogue run (an item's own start and end cost
-// 12 us when each was a CTA, eight key tiles' time).
+// one's last products and epilogue run.  An item costs 5.8k cycles besides its
+// key tiles (the epilogue 3k, the last product 0.9k, masks 1k per edge; 22k
+// when each item was a CTA), a key tile 3.4k.
 //   warp 0      TMA: both Q tiles, then K and V tiles of 128 keys through
 //               rings of 2 (D = 128) or 4 (D = 64) slots
 //   warp 2      the items' plans
 //   warp 1      TMEM and MMA issue: S_t = Q_t K^T, O_t += P_t V, the two
 //               tiles in turn so that one's products run during the other's
-//               softmax; value rows past the filled keys are zeroed in shared
+//               softmax; value rows that no query sees are zeroed in shared
 //               memory first (a weight of 0 does not hide a NaN there)
 //   warps 4-11  softmax, one query row per thread: lazy running maximum
 //               (raised, and O rescaled, only past 2^8), P over S in TMEM; at
@@ -85,6 +86,11 @@ __device__ __forceinline__ Reach reach(const SpanBase& s, int32_t la, int32_t lb
 // P is handed over in two halves, so that the products of its first 64 keys run
 // while the others' exponentials are taken (with the sums below, 164 -> 149 us
 // for 8192 queries, window 1024, 32/8 heads, D = 128).
+// Bound: the chain of one tile's softmax (1850 cycles), the second half of its
+// P V and its next S (800) and their hand-overs; the tensor pipe is busy 2100
+// of a key tile's 3400 cycles.  8192 queries, 32/8 heads, D = 128, calls back to
+// back: window 1024 147 us (870 TFLOP/s over the visible pairs), 4096 353 us
+// (1170), no window 450 us (1220).
 // Otherwise this is attn_fwd_kernel's pipeline; see there for the orderings, the
 // 2^-shift pre-scale of BF16 weights and the bounded waits.
 struct SpanTileParams {
@@ -846,6 +852,9 @@ struct SpanMergeParams {
     uint64_t o_sb, o_sh, o_sl;
 };
 
+// A row of records per warp.  Bound: L2, each record read once; 16 x 33 queries
+// of 32 heads, D = 128, three records each (26 MB): 10 us by itself, of which the
+// launch before hides the start.
 template <int D>
 __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the records are written
@@ -882,7 +891,12 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // the launch overlaps that kernel (programmatic dependent launch) on the SMs it
 // leaves free; its records are joined at the same place where all CTAs fit
 // there, else by a launch of their own (waiting CTAs would keep others out).
-// Bound: HBM, the visible keys and values once.
+// Bound: HBM, the visible keys and values once: 16 sequences, 32/8 heads, D =
+// 128, window 16384: 178 us, 6.0 TB/s; window 4096 55 us, 4.9 TB/s.  Single users
+// are bound by latency, and by the 50 GB/s that one SM draws: 260 keys 9.4 us.
+// (Clusters of CTAs per short unit, joined through distributed shared memory,
+// took 504 keys from 12.4 to 10.0 us but 260 keys from 9.4 to 9.7 and long streams 1%
+// up; three stages in flight instead of two made long streams 2% slower.)
 constexpr int DTILE = 64;  // keys
 
 struct SpanDecodeParams {
@@ -1363,11 +1377,11 @@ struct TileGrid {
 // NB sequences that make the fewest tiles (33 queries of 16 sequences, groups
 // of 4: 2 x 16, 17 tiles; 32 x 1 would make 32, half of them nearly empty).
 // Key ranges when the pairs of tiles alone do not fill the GPU: about one CTA
-// per SM, at least two key tiles each.  (A key tile takes a CTA 1.5 us with two
-// tiles of rows and 1.7 us with one, so rows are always paired.)
+// per SM, at least two key tiles each.  (A key tile takes a CTA 1.8 us with two
+// tiles of rows and hardly less with one, so rows are always paired.)
 // Where span_decode_kernel streams the own keys meanwhile (`streamed` bytes of
 // them) on the SMs that the tiles leave free, the number of ranges that ends
-// both soonest: a key tile takes 2.2 us (5 us more for a CTA's start and end),
+// both soonest: a key tile next to that stream takes 2.2 us (5 us more for a CTA's start and end),
 // the stream 5.8 TB/s, which 70% of the SMs keep up, a record a write and a read
 // (64 sequences x 8192 shared keys + 512 own: 8 ranges, 64 CTAs, not 16).
 TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared, double streamed = 0.0) {

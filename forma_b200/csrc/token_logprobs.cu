@@ -59,7 +59,8 @@ __device__ __forceinline__ float target_logprob(const T* x, const Nest& inner, u
 
 // Any layout: one block per row, the row read once for its maximum, once for
 // the sums (f64) and once per alternative (the largest (value, lowest index)
-// below the previous one).
+// below the previous one).  Bound: L2 and latency, 2 + k passes; 256 x 50021
+// f32 with a class stride of 256: 197 us, with 5 alternatives 537 us.
 template <typename T>
 __global__ void __launch_bounds__(BLOCK) token_rows_kernel(TokenArgs a) {
     __shared__ uint64_t keys[BLOCK / 32];
@@ -123,6 +124,8 @@ __device__ __forceinline__ float logit_grad(float x, float lse, float h, float g
     return d;
 }
 
+// Any layout: chunks of rows over the blocks.  Bound: the loads' latency; 256 x
+// 50021 f32 with a class stride of 256: 131 us, 0.8 TB/s.
 template <typename T, typename O>
 __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a) {
     const Rows& in = a.logits;
@@ -170,7 +173,14 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
 // read 64 bytes again instead of a segment, measured slower up to 5
 // alternatives and no faster at 20 for rows under 50k classes.)
 //
-// Bound: HBM (the ex2 unit is 3/4 busy at the full rate with 16-bit logits).
+// Bound: HBM (the ex2 unit is 3/4 busy at the full rate with 16-bit logits),
+// and the few microseconds per row in which its CTA puts the alternatives in
+// order and loads nothing.  8200 x 131072 BF16: 375 us, 5.7 TB/s; with 5
+// alternatives 415 us, 5.2 TB/s; 2048 rows 104 and 120 us; f32 1024 x 131072
+// 86 and 96 us, 6.2 and 5.6 TB/s.  64 x 32000 with 8: 11 us, 1 x 50021 with 20:
+// 12 us, latency.  (Measured and not kept: one persistent CTA per slot over
+// several rows; a second launch that splits the rows of a partial last wave, 6%
+// at 740 rows and nothing at 2048.)
 // Few rows are split over the CTAs of a cluster, each with its own sums and
 // alternatives, joined through distributed shared memory.
 constexpr int SM_WARPS = 32;   // resident warps per SM (64 registers a thread)
@@ -682,6 +692,7 @@ int launch_t(const TokenArgs& a, cudaStream_t st) {
 // 0 or infinity.
 // Bound: HBM, one read and one write.  Loads are issued before the row's
 // scalars arrive; each block does one chunk of 4 vectors per thread.
+// 2048 x 131072 BF16: 169 us back to back, 6.4 TB/s; into f32 270 us, 6.0 TB/s.
 template <typename T, typename U>  // U: patterns of the output, T's own or f32's
 __global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(GradArgs a) {
     using W = Words<T>;
