@@ -5,7 +5,7 @@ Tolerance.  f32 operands: 1e-5 of max(|e|, 1), the package's f32 bound.
 16-bit operands, u the unit roundoff of the type (2^-9 BF16, 2^-12 F16, both
 as half an ulp relative to the leading digit's binade): the weights are
 rounded to the operands' type before they multiply V, and the row sum adds
-the rounded weights, so numerator and denominator are each off by at most u
+them before or after that, so numerator and denominator are each off by at most u
 relative to sum p |v| <= max|v|; exponentials and f32 scores add less than
 2^-12 of the same; a 16-bit result is rounded once more:
 |error| <= (2u + 2^-12) max|v| + u |e|."""
