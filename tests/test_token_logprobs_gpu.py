@@ -361,3 +361,15 @@ def test_grad_in_f32(cuda, dtype, rows, cols):
     check_grad(x, t, gl, None, got[1:1 + n].view(rows, cols))
     assert api.last_route() == ["token_grad_rows_kernel"]
     assert got[0] == 7 and (got[1 + n:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,cols", [(torch.bfloat16, 16500), (torch.float16, 25000), (torch.float32, 8300), (torch.float32, 16700)])
+@pytest.mark.parametrize("top", [17, 20, 21, 50, 64])
+def test_forward_parts_with_few_values(cuda, dtype, cols, top):
+    """Rows cut into parts whose last one is short: fewer groups of lanes with
+    values than alternatives."""
+    x = rnd((9, cols), dtype, 89)
+    x[2, 40:] = -torch.inf
+    t = targets_for(x, 90)
+    t[2] = 7
+    check_forward(x, t, top)
