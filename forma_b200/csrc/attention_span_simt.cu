@@ -105,15 +105,20 @@ __global__ void __launch_bounds__(32 * WARPS) span_simt_kernel(SpanArgs s) {
                     for (uint64_t d = 0; d < a.depth; ++d) dot += (double)qrow[d] * (double)Elem<T>::load(kp + d * k_d);
                     score = dot * (double)a.scale;
                 }
-                double tile_max = score;
+                // One maximum for the whole warp, so that all lanes go on or
+                // none does: a NaN compares false either way and would leave its
+                // own lane with another maximum than the rest.  It takes part
+                // through its weight, which makes the row NaN.
+                const bool nan = __any_sync(0xffffffffu, score != score);
+                double tile_max = score == score ? score : excluded;
 #pragma unroll
                 for (int x = 16; x; x >>= 1) {
                     const double o = __shfl_xor_sync(0xffffffffu, tile_max, x);
                     tile_max = o > tile_max ? o : tile_max;
                 }
                 // Every visible score -inf (infinite operands): no weight, as
-                // the general kernel has it; a NaN score falls through below.
-                if (tile_max == excluded && !__any_sync(0xffffffffu, score != score)) continue;
+                // the general kernel has it.
+                if (tile_max == excluded && !nan) continue;
                 const double next = maximum > tile_max ? maximum : tile_max;
                 const double alpha = denominator == 0.0 ? 0.0 : exp(maximum - next);
                 maximum = next;
