@@ -74,13 +74,18 @@ __device__ RowState attend_range(const AttnArgs& a, const RowBases& b, uint64_t 
             for (uint64_t d = 0; d < a.depth; ++d) dot += (double)qrow[d] * (double)Elem<T>::load(kp + d * a.k_stride_d);
             score = dot * (double)a.scale + bias;
         }
-        double tile_max = score;
+        // One maximum for the whole warp, so that all lanes go on or none does:
+        // a NaN compares false either way and would leave its own lane with
+        // another maximum than the rest.  It takes part through its weight,
+        // which makes the row NaN.
+        const bool nan = __any_sync(0xffffffffu, score != score);
+        double tile_max = score == score ? score : excluded;
 #pragma unroll
         for (int s = 16; s; s >>= 1) {
             const double o = __shfl_xor_sync(0xffffffffu, tile_max, s);
             tile_max = o > tile_max ? o : tile_max;
         }
-        if (tile_max == excluded) continue;  // nothing visible in this tile
+        if (tile_max == excluded && !nan) continue;  // nothing visible in this tile
         const double next = maximum > tile_max ? maximum : tile_max;
         // An all-excluded prefix must not evaluate -inf - (-inf).
         const double alpha = denominator == 0.0 ? 0.0 : exp(maximum - next);

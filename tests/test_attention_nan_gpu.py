@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from forma_b200 import api
-from forma_b200.api import AttentionOptions
+from forma_b200.api import AttentionOptions, Mask
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,33 @@ def test_prefix_generic_nan(cuda, dtype, d, pre, keys):
         poisoned, bad = none.clone(), k.clone()
         poisoned[2, :2, lq - 1], bad[2, 0, keys - 1, 0] = True, torch.nan  # the newest key: the last query alone
         rows_are(api.attention_prefix(q, pk, pv, bad, v), want, poisoned)
+
+
+@pytest.mark.parametrize("dtype,d", GENERIC)
+@pytest.mark.parametrize("keys", [1, 31, 33, 65, 700])
+@pytest.mark.parametrize("kind", ["plain", "causal", "keep", "additive"])
+def test_dense_generic_nan(cuda, dtype, d, keys, kind):
+    """The same for the general dense kernel and its split over long key ranges."""
+    lq = 5
+    q, k, v = rnd((2, 4, lq, d), dtype, 15), rnd((2, 2, keys, d), dtype, 16), rnd((2, 2, keys, d), dtype, 17)
+    sees = torch.ones((lq, keys), dtype=torch.bool, device=cuda)
+    mask, options = None, AttentionOptions()
+    if kind == "causal":
+        options = AttentionOptions(causal=keys - 3)
+        sees = torch.arange(keys, device=cuda)[None] <= torch.arange(lq, device=cuda)[:, None] + keys - 3
+    elif kind != "plain":
+        sees[1, keys // 2:] = False
+        sees[3] = False
+        mask = Mask("keep", sees.int()) if kind == "keep" else Mask("additive", torch.where(sees, 0.25, -torch.inf))
+    run = (lambda q, k: api.attention(q, k, v, mask, options)) if dtype == torch.float32 else \
+          (lambda q, k: api.attention_low_f32(q, k, v, mask, options))
+    want = run(q, k)
+    assert all("simt" in r or "attention_part" in r or "attention_merge" in r for r in api.last_route()), api.last_route()
+    poisoned, bad = torch.zeros((2, 4, lq), dtype=torch.bool, device=cuda), q.clone()
+    poisoned[1, 3] = sees.any(1)
+    bad[1, 3, :, 2] = torch.nan
+    rows_are(run(bad, k), want, poisoned)
+    for j in sorted({0, keys // 2, keys - 1}):
+        poisoned, bad = torch.zeros((2, 4, lq), dtype=torch.bool, device=cuda), k.clone()
+        poisoned[0, 2:], bad[0, 1, j, 0] = sees[:, j], torch.nan
+        rows_are(run(q, bad), want, poisoned)
