@@ -36,10 +36,17 @@ __device__ __forceinline__ float ex2(float x) {
 // Inputs are clamped to -127 first; at n = -127 a polynomial value below 1
 // carries its exponent field below zero, which the final max with 0 turns
 // into exactly 0, so -inf (a masked score) gives 0 and a fully masked row
-// keeps a zero sum.  The f32x2 forms process both values in one instruction.
+// keeps a zero sum.  A NaN passes the clamp and comes back with 0 x at the end
+// (the integer steps lose it; a finite x adds nothing there).  The f32x2 forms
+// process both values in one instruction.
+__device__ __forceinline__ float max2_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
     const float2 M = make_float2(12582912.0f, 12582912.0f);
-    const float2 xc = make_float2(fmaxf(x.x, -127.0f), fmaxf(x.y, -127.0f));
+    const float2 xc = make_float2(max2_nan(x.x, -127.0f), max2_nan(x.y, -127.0f));
     const float2 t = __fadd2_rn(xc, M);
     const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
     const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), xc);  // exact: xc - n
@@ -49,7 +56,7 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
     q = __ffma2_rn(q, f, make_float2(0.9999280571937561f, 0.9999280571937561f));
     const int bx = (int)(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23));
     const int by = (int)(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23));
-    return make_float2(__int_as_float(max(bx, 0)), __int_as_float(max(by, 0)));
+    return __ffma2_rn(xc, make_float2(0.0f, 0.0f), make_float2(__int_as_float(max(bx, 0)), __int_as_float(max(by, 0))));
 }
 
 // Three-input extremes.  A NaN score is skipped by the row maximum but its

@@ -129,3 +129,56 @@ def test_dense_generic_nan(cuda, dtype, d, keys, kind):
         poisoned, bad = torch.zeros((2, 4, lq), dtype=torch.bool, device=cuda), k.clone()
         poisoned[0, 2:], bad[0, 1, j, 0] = sees[:, j], torch.nan
         rows_are(run(q, bad), want, poisoned)
+
+
+# Tensor-core kernels: part of the exponentials are polynomials, chosen by the
+# key's place in its tile, so every place is tried.
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,kernel", [(40, "span_tile_kernel"), (2, "span_decode_kernel")])
+def test_window_tensor_core_nan_and_infinity(cuda, dtype, d, lq, kernel):
+    keys, window, sinks = 200, 90, 3
+    q, k, v = rnd((1, 4, lq, d), dtype, 20), rnd((1, 2, keys, d), dtype, 21), rnd((1, 2, keys, d), dtype, 22)
+    want = api.attention_window(q, k, v, window, sinks)
+    assert all(r.startswith(kernel) for r in api.last_route()), api.last_route()
+    p = torch.arange(keys - lq, keys, device=cuda)
+    for j in [0, 1, 2, keys - 1] + list(range(130, 162)):
+        sees = (j <= p) & ((j > p - window) | (j < sinks))
+        poisoned, bad = torch.zeros((1, 4, lq), dtype=torch.bool, device=cuda), k.clone()
+        poisoned[0, 2:], bad[0, 1, j, 3] = sees, torch.nan
+        rows_are(api.attention_window(q, bad, v, window, sinks), want, poisoned)
+        # an infinite score: NaN where it is +inf, no weight where it is -inf
+        bad = k.clone()
+        bad[0, 1, j, 3] = torch.inf
+        got = api.attention_window(q, bad, v, window, sinks)
+        up = torch.zeros((1, 4, lq), dtype=torch.bool, device=cuda)
+        up[0, 2:] = sees & (q[0, 2:, :, 3] > 0)
+        assert torch.equal(torch.isnan(got).any(-1), up) and torch.equal(torch.isnan(got).all(-1), up)
+
+
+@pytest.mark.parametrize("lq,d", [(1, 128), (30, 64)])
+def test_prefix_tensor_core_nan(cuda, lq, d):
+    """A NaN in the shared prefix passes the records and their join."""
+    dt, b, pre, keys = torch.bfloat16, 3, 300, 40
+    q, pk, pv = rnd((b, 8, lq, d), dt, 23), rnd((2, pre, d), dt, 24), rnd((2, pre, d), dt, 25)
+    k, v = rnd((b, 2, keys, d), dt, 26), rnd((b, 2, keys, d), dt, 27)
+    want = api.attention_prefix(q, pk, pv, k, v)
+    assert api.last_route()[0].startswith("span_tile_kernel"), api.last_route()
+    for j in list(range(16)) + [142, 143, 298, 299]:
+        poisoned, bad = torch.zeros((b, 8, lq), dtype=torch.bool, device=cuda), pk.clone()
+        poisoned[:, :4], bad[0, j, 0] = True, torch.nan
+        rows_are(api.attention_prefix(q, bad, pv, k, v), want, poisoned)
+
+
+@pytest.mark.parametrize("lq,keys,d,kernel", [(300, 300, 128, "attn_fwd_kernel"), (190, 190, 64, "attn_short_kernel"),
+                                              (120, 120, 64, "attn_short_kernel")])
+def test_dense_tensor_core_nan(cuda, lq, keys, d, kernel):
+    dt = torch.bfloat16
+    q, k, v = rnd((1, 2, lq, d), dt, 28), rnd((1, 2, keys, d), dt, 29), rnd((1, 2, keys, d), dt, 30)
+    want = api.attention_low_f32(q, k, v)
+    assert any(r.startswith(kernel) for r in api.last_route()), api.last_route()
+    for j in list(range(32)) + [keys - 1]:
+        poisoned, bad = torch.zeros((1, 2, lq), dtype=torch.bool, device=cuda), k.clone()
+        poisoned[0, 1], bad[0, 1, j, 0] = True, torch.nan
+        rows_are(api.attention_low_f32(q, bad, v), want, poisoned)
