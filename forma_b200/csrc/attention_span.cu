@@ -29,6 +29,7 @@ __device__ uint32_t g_span_status;
 struct SpanKeys {
     int32_t pos0, low0;     // without lengths: query 0's position, its window's first key (may be negative)
     int32_t window, sinks;  // at most 2^30
+    int32_t after;          // with lengths: queries of the call behind this launch's last
     const uint32_t* lengths;
     uint64_t length_stride;
 };
@@ -39,7 +40,7 @@ __device__ __forceinline__ SpanBase span_base(const SpanKeys& k, uint32_t b, uin
     SpanBase s{(int32_t)Lk, k.pos0, k.low0};
     if (k.lengths) {
         s.filled = (int32_t)min(Lk, k.lengths[b * k.length_stride]);
-        s.pos0 = s.filled - (int32_t)L;
+        s.pos0 = s.filled - (int32_t)L - k.after;
         s.low0 = s.pos0 - k.window + 1;
     }
     return s;
@@ -1424,6 +1425,7 @@ SpanKeys span_keys(const SpanArgs& s) {
     SpanKeys k{};
     k.pos0 = (int32_t)std::clamp(pos0, -big, big), k.low0 = (int32_t)std::clamp(low0, -big, big);
     k.window = (int32_t)std::min<uint64_t>(s.window, 1u << 30), k.sinks = (int32_t)std::min<uint64_t>(s.sinks, 1u << 30);
+    k.after = (int32_t)s.after;
     k.lengths = s.lengths, k.length_stride = s.length_stride;
     return k;
 }
@@ -1601,36 +1603,52 @@ int launch_decode(const SpanArgs& s, const SpanOperands& a, const DecodeGrid& g,
 
 template <int D>
 int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
-    const bool prefix = s.prefix_keys > 0, own = a.Lk > 0;
+    const bool prefix = s.prefix_keys > 0, own = a.Lk > 0, few = a.G * a.L <= 16;
     const float shift = weight_shift(a.fmt, a.Lk + s.prefix_keys);
-    const double streamed = a.G * a.L <= 16 ? (double)(a.B * a.Hkv * a.Lk) * a.D * 4 : 0.0;
+    const double streamed = few ? (double)(a.B * a.Hkv * a.Lk) * a.D * 4 : 0.0;
     const TileGrid pg = prefix ? tile_grid(s, a, true, streamed) : TileGrid{};
-    const uint64_t ps = pg.splits;
-    const uint64_t rows = a.B * a.H * a.L;
+    const TileGrid og = own && !few ? tile_grid(s, a, false) : TileGrid{};
+    const uint64_t ps = pg.splits, rows = a.B * a.H * a.L;
+    // Records per row: the prefix's ranges and the own keys', none where the
+    // tiles write the output themselves.
+    const uint64_t count = few ? prefix ? ps + 1 : 0 : ps + og.splits > 1 ? ps + og.splits : 0;
     Records rec;
-    // Records of a prefix and of own keys, for as many sequences at a time as
-    // keep them within RECORD_BYTES: a launch fills the GPU long before that.
-    if (prefix && a.B > 1 && rows * (ps + 1) * (D * sizeof(float) + sizeof(float2)) > RECORD_BYTES) {
-        const uint64_t bytes = a.H * a.L * (ps + 1) * (D * sizeof(float) + sizeof(float2));
-        const uint64_t step = std::min(a.B - 1, std::max<uint64_t>(1, RECORD_BYTES / bytes));
-        for (uint64_t b = 0; b < a.B; b += step) {
+    // For as many sequences at a time, or queries of one, as keep the records
+    // within RECORD_BYTES: a launch fills the GPU long before that.
+    const uint64_t row_bytes = count * (D * sizeof(float) + sizeof(float2));
+    if (rows * row_bytes > RECORD_BYTES && (a.B > 1 || a.L > 1)) {
+        const bool batch = a.B > 1;
+        const uint64_t n = batch ? a.B : a.L, bytes = a.H * (batch ? a.L : 1) * row_bytes;
+        uint64_t step = std::min(n - 1, std::max<uint64_t>(1, RECORD_BYTES / bytes));
+        if (!batch && step > TQ) step = step / TQ * TQ;
+        for (uint64_t at = 0; at < n; at += step) {
             SpanArgs sb = s;
             SpanOperands ab = a;
-            ab.B = std::min(step, a.B - b);
-            auto part = [&](RowsLayout& l) {
-                if (!l.batch_bcast) l.batch = ab.B;
-                return l.batch_bcast ? 0 : b * l.s_batch;
-            };
-            ab.qp = static_cast<const uint16_t*>(a.qp) + part(ab.q);
-            ab.kp = static_cast<const uint16_t*>(a.kp) + part(ab.k);
-            ab.vp = static_cast<const uint16_t*>(a.vp) + part(ab.v);
-            ab.op = static_cast<char*>(a.op) + part(ab.o) * (s.base.out_low ? 2 : 4);
-            if (s.lengths) sb.lengths = s.lengths + b * s.length_stride;
+            const uint64_t m = std::min(step, n - at);
+            const uint64_t out_bytes = s.base.out_low ? 2 : 4;
+            if (batch) {
+                ab.B = m;
+                auto part = [&](RowsLayout& l) {
+                    if (!l.batch_bcast) l.batch = m;
+                    return l.batch_bcast ? 0 : at * l.s_batch;
+                };
+                ab.qp = static_cast<const uint16_t*>(a.qp) + part(ab.q);
+                ab.kp = static_cast<const uint16_t*>(a.kp) + part(ab.k);
+                ab.vp = static_cast<const uint16_t*>(a.vp) + part(ab.v);
+                ab.op = static_cast<char*>(a.op) + part(ab.o) * out_bytes;
+                if (s.lengths) sb.lengths = s.lengths + at * s.length_stride;
+            } else {
+                ab.L = ab.q.rows = ab.o.rows = m;
+                ab.qp = static_cast<const uint16_t*>(a.qp) + at * a.q.s_row;
+                ab.op = static_cast<char*>(a.op) + at * a.o.s_row * out_bytes;
+                sb.offset += (int64_t)at;
+                sb.after += n - at - m;
+            }
             if (int r = launch_span<D>(sb, ab, st); r != FB_OK) return r;
         }
         return FB_OK;
     }
-    if (a.G * a.L <= 16) {  // few rows: the own keys streamed, the prefix's records joined there
+    if (few) {  // the own keys streamed, the prefix's records joined there
         DecodeGrid dg;
         if (!decode_grid(s, a, &dg)) return FB_ERR_UNSUPPORTED;
         if (!prefix) return launch_decode<D>(s, a, dg, rec, false, shift, st);
@@ -1642,9 +1660,7 @@ int launch_span(const SpanArgs& s, const SpanOperands& a, cudaStream_t st) {
         if (int r = launch_decode<D>(s, a, dg, rec, join, shift, st); r != FB_OK) return r;
         return join ? FB_OK : launch_merge<D>(s, a, rec, st);
     }
-    const TileGrid og = own ? tile_grid(s, a, false) : TileGrid{};
-    const uint64_t count = ps + og.splits;
-    if (count <= 1) return launch_tiles<D>(s, a, prefix, rec, 0, prefix ? pg : og, shift, false, st);
+    if (!count) return launch_tiles<D>(s, a, prefix, rec, 0, prefix ? pg : og, shift, false, st);
     if (!get_records<D>(st, a, count, SCRATCH_SPAN, rows, &rec)) return FB_ERR_DRIVER;
     if (prefix)
         if (int r = launch_tiles<D>(s, a, true, rec, 0, pg, shift, false, st); r != FB_OK) return r;

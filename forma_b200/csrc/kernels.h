@@ -234,7 +234,7 @@ int launch_attention_tc(const AttnArgs& a, void* stream);
 // fb_attention_window and fb_attention_prefix.  `base` holds the query, the
 // sequences' own keys and values and the output (mask and causal fields
 // unused; out_low as there).  The query of index i in batch b stands at
-// position n_b - L + i (n_b = min(lengths[b], keys)) or, without lengths,
+// position n_b - after - L + i (n_b = min(lengths[b], keys)) or, without lengths,
 // at offset + i over all keys; own key j is visible to a query at position p
 // iff j < n_b, j <= p and (j > p - window or j < sinks).  prefix_keys > 0:
 // every query sees all the keys of [Hkv, prefix_keys, D] too.
@@ -243,6 +243,7 @@ struct SpanArgs {
     const uint32_t* lengths = nullptr;  // one per batch index (row-major over the batch axes), or null
     uint64_t length_stride = 0;
     int64_t offset = 0;
+    uint64_t after = 0;                 // with lengths: queries of the call behind the last one of `base`
     uint64_t window = 0, sinks = 0;
     const void* pk = nullptr;
     const void* pv = nullptr;

@@ -479,3 +479,32 @@ def test_prefix_more_records_than_are_kept_at_once(cuda, lq, b, low):
     got = out[some]
     check(got, exp, torch.bfloat16, top)
     assert api.device_status() == 0
+
+
+@pytest.mark.parametrize("lengths,causal", [([39990], None), (None, None), (None, 100)])
+def test_prefix_one_sequence_past_the_record_bound(cuda, lengths, causal):
+    """One sequence whose intermediate results exceed the scratch bound runs in
+    parts of its queries: rows around the parts' borders against the plain
+    form, and no more scratch than the bound on a stream of its own."""
+    h, hk, d, lq, pre, keys = 32, 4, 128, 40000, 300, 40000
+    q, pk, pv = rnd((1, h, lq, d), torch.bfloat16, 100), rnd((hk, pre, d), torch.bfloat16, 101), rnd((hk, pre, d), torch.bfloat16, 102)
+    k, v = rnd((1, hk, keys, d), torch.bfloat16, 103), rnd((1, hk, keys, d), torch.bfloat16, 104)
+    ln = torch.tensor(lengths, dtype=torch.int32, device=cuda) if lengths else None
+    got = torch.full_like(q, torch.nan)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    free = torch.cuda.mem_get_info()[0]
+    with torch.cuda.stream(s):
+        api.attention_prefix(q, pk, pv, k, v, ln, AttentionOptions(causal=causal), out=got)
+    s.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] <= (1 << 30) + (64 << 20)
+    assert len(api.last_route()) > 3
+    assert torch.isfinite(got).all()
+    rows = [0, 1, 9, 10, 11, 127, 128, 20000, 32127, 32128, 32255, 32256, 32257, 39871, 39999]
+    n = (lengths or [keys])[0]
+    p = torch.tensor(rows, device=cuda) + (n - lq if causal is None else causal)
+    j = torch.arange(keys, device=cuda)
+    seen = ((j[None] <= p[:, None]) & (j[None] < n))[None]
+    exp = attend64(q[:, :, rows], [(pk[None], pv[None], None), (k, v, seen)], d**-0.5)
+    check(got[:, :, rows], exp, torch.bfloat16, max(float(v.double().abs().max()), float(pv.double().abs().max())))
+    assert api.device_status() == 0
