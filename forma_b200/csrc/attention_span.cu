@@ -92,8 +92,8 @@ __device__ __forceinline__ Reach reach(const SpanBase& s, int32_t la, int32_t lb
 // of a key tile's 3400 cycles.  8192 queries, 32/8 heads, D = 128, calls back to
 // back: window 1024 147 us (870 TFLOP/s over the visible pairs), 4096 353 us
 // (1170), no window 450 us (1220).
-// Otherwise this is attn_fwd_kernel's pipeline; see there for the orderings, the
-// 2^-shift pre-scale of BF16 weights and the bounded waits.
+// Otherwise this is attn_fwd_kernel's pipeline; see there for the orderings and
+// the bounded waits, and weight_shift for the scale of the weights.
 struct SpanTileParams {
     uint32_t B, H, L, Lk;          // sequences, query heads, queries, keys per head
     uint32_t group;                // query heads per key/value head
@@ -1356,9 +1356,22 @@ struct SpanOperands {
     void* op;
 };
 
-float weight_shift(uint32_t fmt, uint64_t keys) {  // see attn_fwd_kernel: BF16 weights pre-scaled by 2^-shift
-    return fmt ? 9.0f + std::ceil(std::log2((float)std::max<uint64_t>(keys, 1))) : 0.0f;
+// Weights are 2^(logit - reference - shift).  BF16: see attn_fwd_kernel.  F16
+// holds nothing below 2^-25, and many keys that far below one add up (131072
+// keys 18 nats below it are 0.2% of the row): a shift of -7 puts the largest
+// weight, 2^8 past the reference at most, at 2^15, and keeps all keys down to
+// 2^-32 of the row's largest.
+float weight_shift(uint32_t fmt, uint64_t keys) {
+    return fmt ? 9.0f + std::ceil(std::log2((float)std::max<uint64_t>(keys, 1))) : -7.0f;
 }
+
+// Most keys that one accumulator takes.  The matrix units align products to
+// the accumulator and cut them off at 2^-25 of it, so n keys can leave up to
+// n 2^-25 of a row out of O (measured with 16384 keys of weight 2^-18 to 2^-27
+// beside one of 1: 2^-25.1 a key at most; below 2^-25 nothing of them arrives).
+// At u 2^26 keys, u the type's unit roundoff, that is 2 u, what the weights' own
+// rounding may cost; longer ranges are divided and joined in f32.
+uint64_t range_keys(uint32_t fmt) { return fmt ? 131072 : 16384; }
 
 uint64_t largest_divisor(uint64_t n, uint64_t most) {
     uint64_t d = std::min(n, most);
@@ -1404,16 +1417,17 @@ TileGrid tile_grid(const SpanArgs& s, const SpanOperands& a, bool shared, double
         keys = std::min(keys, (std::min(s.sinks, a.Lk) + std::min(s.window, a.Lk) + 2 * g.LB + 16 + TK - 1) / TK);
     const uint64_t sms = (uint64_t)sm_count();
     const uint64_t ctas = g.units * ((g.tiles + 1) / 2);
-    g.splits = 1;
+    const uint64_t most = range_keys(a.fmt) / TK, least = std::max<uint64_t>(1, (keys + most - 1) / most);
+    g.splits = least;
     if (ctas < sms && keys >= 4) {
         const double stream = streamed / 5.8e6, record = (double)(a.B * a.H * a.L) * a.D * 8 / 5.0e6;
-        double least = INFINITY;
-        for (uint64_t want = 1; want <= std::min<uint64_t>(sms / ctas, keys / 2); ++want) {
+        double lowest = INFINITY;
+        for (uint64_t want = least; want <= std::max(least, std::min<uint64_t>(sms / ctas, keys / 2)); ++want) {
             const uint64_t per = (keys + want - 1) / want, n = (keys + per - 1) / per;
             const double tiles = (double)per * 2.2 + 5.0, done = (double)(sms - std::min(sms, ctas * n)) * tiles;
             const double left = std::max(0.0, (stream * 0.7 * (double)sms - done) / (double)sms);
             const double cost = std::max(stream, tiles + left) + record * (double)n;
-            if (cost < least) least = cost, g.splits = n;
+            if (cost < lowest) lowest = cost, g.splits = n;
         }
     }
     return g;
@@ -1546,7 +1560,7 @@ int launch_merge(const SpanArgs& s, const SpanOperands& a, const Records& rec, c
 // warps stream it in the time that joining two CTAs' records takes), of two
 // warps when there are more units than CTAs of four fit the GPU at once; longer
 // ones are dealt out to two CTAs per SM, at least two tiles each once every SM
-// has one.
+// has one, and to more where a warp would take more than range_keys.
 struct DecodeGrid {
     uint64_t ctas = 0;
     bool whole = false;
@@ -1561,6 +1575,8 @@ bool decode_grid(const SpanArgs& s, const SpanOperands& a, DecodeGrid* g) {
     g->whole = seen <= 8 * DTILE;
     g->warps = g->whole && units > 2 * sms ? 2 : 4;
     g->ctas = g->whole ? units : tiles <= sms ? tiles : std::min<uint64_t>(2 * sms, std::max(sms, tiles / 2));
+    const uint64_t most = 4 * range_keys(a.fmt) / DTILE;  // tiles of a CTA of four warps
+    if (!g->whole) g->ctas = std::max(g->ctas, (tiles + most - 1) / most);
     return true;
 }
 
