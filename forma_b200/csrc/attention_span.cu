@@ -85,8 +85,8 @@ __device__ __forceinline__ Reach reach(const SpanBase& s, int32_t la, int32_t lb
 //               an item's end O / l, or a record, through shared memory and
 //               TMA stores of 128 bytes per row
 // P is handed over in two halves, so that the products of its first 64 keys run
-// while the others' exponentials are taken (with the sums below, 164 -> 149 us
-// for 8192 queries, window 1024, 32/8 heads, D = 128).
+// while the others' exponentials are taken (164 -> 149 us for 8192 queries,
+// window 1024, 32/8 heads, D = 128).
 // Bound: the chain of one tile's softmax (1850 cycles), the second half of its
 // P V and its next S (800) and their hand-overs; the tensor pipe is busy 2100
 // of a key tile's 3400 cycles.  8192 queries, 32/8 heads, D = 128, calls back to
@@ -261,6 +261,20 @@ __device__ __forceinline__ void tma_store_5d(const CUtensorMap* map, int32_t x, 
                      reinterpret_cast<uint64_t>(map)),
                  "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(src))
                  : "memory");
+}
+
+// acc + the two 16-bit weights of a packed word, each sum in f32.
+template <int FMT>
+__device__ __forceinline__ float2 add_weights(float2 acc, uint32_t w) {
+    if constexpr (FMT == 1)
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.bf16 %0, l, %0;\n\tadd.rn.f32.bf16 %1, h, %1;\n\t}"
+            : "+f"(acc.x), "+f"(acc.y)
+            : "r"(w));
+    else
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tadd.rn.f32.f16 %0, l, %0;\n\tadd.rn.f32.f16 %1, h, %1;\n\t}"
+            : "+f"(acc.x), "+f"(acc.y)
+            : "r"(w));
+    return acc;
 }
 
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
@@ -657,10 +671,10 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 float2 lsa[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 // Packed pairs overwrite the scores they came from, so P needs no
                 // registers of its own; one pair in eight takes the polynomial.
-                // The row sum adds the weights before they are rounded: summing
-                // the rounded ones after the hand-over took two more instructions
-                // per pair and 6% of the kernel; the roundings are unbiased, and
-                // both sums are within the weights' unit roundoff of each other.
+                // The row sum adds the weights as they were rounded, so that the
+                // rounding of a dominant one cancels, after the hand-over and with
+                // adds that widen their 16-bit operand (unpacking them first: 149
+                // -> 165 us for 8192 queries, window 1024).
                 uint32_t* xb = reinterpret_cast<uint32_t*>(x);
                 const float2 sl2 = make_float2(mul, mul), nb2 = make_float2(-ref, -ref);
 #pragma unroll
@@ -669,7 +683,6 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                     for (int e = 0; e < 16; ++e) {
                         const float2 z = __ffma2_rn(make_float2(x[c * 32 + 2 * e], x[c * 32 + 2 * e + 1]), sl2, nb2);
                         const float2 w = (e & 7) == 7 ? ex2_poly2(z) : make_float2(ex2(z.x), ex2(z.y));
-                        lsa[e & 3] = __fadd2_rn(lsa[e & 3], w);
                         xb[c * 32 + e] = pack2(w.x, w.y, FMT);
                     }
                     tmem_st16(tm_s + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&xb[c * 32]));
@@ -684,6 +697,8 @@ __global__ void __launch_bounds__(TCfg<D>::THREADS, 1) span_tile_kernel(const __
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
+#pragma unroll
+                for (int e = 0; e < TK / 2; ++e) lsa[e & 3] = add_weights<FMT>(lsa[e & 3], xb[(e / 16) * 32 + e % 16]);
                 const float2 l2 = __fadd2_rn(__fadd2_rn(lsa[0], lsa[1]), __fadd2_rn(lsa[2], lsa[3]));
                 lsum = lsum * alpha + (l2.x + l2.y);
             }

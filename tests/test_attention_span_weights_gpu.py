@@ -40,3 +40,49 @@ def test_many_keys_far_below_one(cuda, dtype, b, lq, place):
         exp = (v0 + rest) / (1 + rest)
         assert (got - exp).abs().max() <= 2 * u + 2.0**-12 + u * abs(exp)
     assert api.device_status() == 0
+
+
+def ones_case(dtype, b, h, hk, d, lq, keys, window, sinks, pre, spread):
+    """Values of one: whatever the weights, P V and their sum are the same sum.
+    f32 output; both are f32 sums of at most `keys` terms: 2^-24 of the whole each."""
+    q, k = rnd((b, h, lq, d), dtype, 1), rnd((b, hk, keys, d), dtype, 2) * spread
+    v = torch.ones((b, hk, keys, d), dtype=dtype, device="cuda")
+    out = torch.empty((b, h, lq, d), device="cuda")
+    if pre:
+        pk = rnd((hk, pre, d), dtype, 3) * spread
+        api.attention_prefix(q, pk, torch.ones_like(pk), k, v, out=out)
+    else:
+        api.attention_window(q, k, v, window, sinks, out=out)
+    assert (out.double() - 1).abs().max() <= (keys + pre) * 2.0**-24
+    assert api.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq", [1, 60])
+@pytest.mark.parametrize("spread", [0.1, 1.0, 3.0])
+def test_sums_are_of_the_weights_that_multiply(cuda, dtype, d, lq, spread):
+    for keys, window, sinks in ((90, 1000, 0), (700, 300, 4), (1500, 5000, 0)):
+        ones_case(dtype, 2, 4, 2, d, lq, keys, window, sinks, 0, spread)
+    ones_case(dtype, 3, 4, 2, d, lq, 80, 0, 0, 900, spread)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lq", [1, 40])
+@pytest.mark.parametrize("logit", [1.3, 3.7, 5.0, 5.45, 11.0])
+def test_dominant_key_in_a_late_tile(cuda, dtype, lq, logit):
+    """A key that outweighs the rest, with and without passing the 2^8 below
+    which the running maximum stays: its weight's rounding cancels.  The other
+    key's share s of the row is off by its own and the dominant one's rounding,
+    2u s; f32 output."""
+    keys, d = 300, 64
+    q, k, v = (torch.zeros((1, 2, n, d), dtype=dtype, device=cuda) for n in (lq, keys, keys))
+    q[..., 0], k[..., 0] = 1.0, -200.0
+    k[:, :, 0, 0], k[:, :, 200, 0] = 0.0, logit
+    v[:, :, 0], v[:, :, 200] = -1.0, 1.0
+    out = torch.empty((1, 2, lq, d), device=cuda)
+    api.attention_window(q, k, v, 1000, 0, options=AttentionOptions(scale=1.0, causal=keys), out=out)
+    share = 1.0 / (1.0 + math.exp(float(k[0, 0, 200, 0])))
+    exp = 1.0 - 2.0 * share
+    # exponentials: 7.5e-5 of a weight where the polynomial takes it, 2^-22 otherwise
+    assert (out.double() - exp).abs().max() <= 2 * share * (2 * UNIT[dtype] + 1e-4) + 2.0**-22
