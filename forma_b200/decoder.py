@@ -76,12 +76,43 @@ class Prompt:
 @dataclass
 class Continuations:
     """Caches of `sequences` continuations of one prompt.  ``lengths`` (int32
-    [G]) counts each one's own tokens."""
+    [G]) counts each one's own tokens; it may be set back, or replaced."""
 
     prompt: Prompt
     caches: List[Tuple[torch.Tensor, torch.Tensor]]  # [G, Hkv, rows, D]
     kept: List[int]                                  # prompt rows at the front of each cache
     lengths: torch.Tensor
+    _known: Optional[tuple] = None                   # lengths that the host knows: (tensor, its version, their maximum)
+
+    @property
+    def room(self) -> int:
+        """Own tokens that every layer's cache holds."""
+        return min(c[0].shape[2] - n for c, n in zip(self.caches, self.kept))
+
+    def require(self, sequences: int, tokens: int, positions: int) -> int:
+        """The longest continuation's tokens, if ``tokens`` more fit each one's
+        cache and the model's ``positions``; ValueError otherwise.  Past the
+        room a cache would be indexed out of range on the device, which ends the
+        process's context.  The device is read only where `lengths` were set
+        from outside."""
+        G = self.lengths.shape[0]
+        if sequences != G:
+            raise ValueError(f"tokens of {sequences} continuations for caches of {G}")
+        if self._known is None or self._known[0] is not self.lengths or self._known[1] != self.lengths._version:
+            low, high = (int(x) for x in self.lengths.aminmax()) if G else (0, 0)
+            if low < 0 or high > self.room:
+                raise ValueError(f"lengths {low} to {high} for caches of {self.room} tokens")
+            self._known = (self.lengths, self.lengths._version, high)
+        longest = self._known[2]
+        if longest + tokens > self.room:
+            raise ValueError(f"{tokens} tokens behind {longest} exceed the caches' room of {self.room}")
+        if self.prompt.length + longest + tokens > positions:
+            raise ValueError(f"position {self.prompt.length + longest + tokens - 1} exceeds the model's {positions}")
+        return longest
+
+    def advance(self, tokens: int, longest: int) -> None:
+        self.lengths = self.lengths + tokens
+        self._known = (self.lengths, self.lengths._version, longest + tokens)
 
 
 class Decoder:
@@ -138,6 +169,8 @@ class Decoder:
     def read(self, tokens: torch.Tensor) -> Prompt:
         """Reads one prompt (int32 [P]) and keeps what its continuations need of it."""
         cfg, P = self.cfg, tokens.shape[0]
+        if P > cfg.positions:
+            raise ValueError(f"a prompt of {P} tokens exceeds the model's {cfg.positions} positions")
         kept: List[Tuple[torch.Tensor, torch.Tensor]] = []
 
         def attend(layer, q, k, v, out):
@@ -169,11 +202,13 @@ class Decoder:
 
     def extend(self, state: Continuations, tokens: torch.Tensor) -> torch.Tensor:
         """Appends tokens (int32 [G, L]) to every continuation and returns their
-        normed hidden rows [G, L, E] in the low dtype."""
+        normed hidden rows [G, L, E] in the low dtype.  ValueError, with nothing
+        changed, where they do not fit."""
         cfg = self.cfg
         G, L = tokens.shape
+        longest = state.require(G, L, cfg.positions)
         at = state.lengths[:, None].long() + torch.arange(L, device=self.device)  # place among the own tokens
-        state.lengths = state.lengths + L
+        state.advance(L, longest)
         seq = torch.arange(G, device=self.device)[:, None]
 
         def attend(layer, q, k, v, out):
@@ -214,7 +249,9 @@ class Decoder:
     def generate(self, state: Continuations, tokens: torch.Tensor, steps: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """Extends every continuation by ``steps`` tokens, each the likeliest
         one after the last ([G] int32 starts); returns the tokens and their log
-        probabilities, [G, steps] each."""
+        probabilities, [G, steps] each.  ValueError before the first where not
+        all of them fit."""
+        state.require(tokens.shape[0], steps, self.cfg.positions)
         chosen, scores = [], []
         for _ in range(steps):
             best = api.token_logprobs(self.logits(self.extend(state, tokens[:, None]))[:, 0], top=1)
