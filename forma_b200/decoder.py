@@ -258,4 +258,6 @@ class Decoder:
             tokens = best.top_index[:, 0]
             chosen.append(tokens)
             scores.append(best.top_logprob[:, 0])
+        if not chosen:
+            return tokens.new_empty(tokens.shape[0], 0), torch.empty(tokens.shape[0], 0, device=tokens.device)
         return torch.stack(chosen, 1), torch.stack(scores, 1)

@@ -78,3 +78,11 @@ def test_positions_and_batch(dec):
     with pytest.raises(ValueError):
         dec.read(torch.zeros(41, dtype=torch.int32))
     accepted(lambda: dec.read(torch.zeros(40, dtype=torch.int32)))
+
+
+def test_no_steps(dec):
+    state = started(dec, 5, 3, 10)
+    chosen, scores = dec.generate(state, tokens(3, 1)[:, 0], 0)
+    assert chosen.shape == scores.shape == (3, 0)
+    assert chosen.dtype == torch.int32 and scores.dtype == torch.float32
+    assert state.lengths.tolist() == [0, 0, 0]
