@@ -89,13 +89,18 @@ def build(force: bool = False, jobs: int | None = None) -> Path:
 
 
 def build_bind(force: bool = False) -> Path:
-    """The torch binding of the serving operators, linked to the library beside it."""
+    """The torch binding of the serving operators, linked to the library beside
+    it.  Built for one torch and one Python: rebuilt when either changes."""
+    import platform
     import sysconfig
 
     import torch
 
     src = PKG / "bind" / "torch_bind.cpp"
-    if force or _stale(BIND, [src, ROOT / "include" / "forma_b200.h"]):
+    made_for = f"torch {torch.__version__}, python {platform.python_version()}\n"
+    stamp = OBJ / "torch_bind.for"
+    known = stamp.read_text() if stamp.exists() else ""
+    if force or known != made_for or _stale(BIND, [src, ROOT / "include" / "forma_b200.h"]):
         root = Path(torch.__file__).resolve().parent
         cuda = Path(NVCC).resolve().parent.parent
         tmp = BIND.with_suffix(".so.tmp")
@@ -109,6 +114,8 @@ def build_bind(force: bool = False) -> Path:
             check=True,
         )
         os.replace(tmp, BIND)
+        OBJ.mkdir(exist_ok=True)
+        stamp.write_text(made_for)
     return BIND
 
 
