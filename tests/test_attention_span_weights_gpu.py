@@ -86,3 +86,57 @@ def test_dominant_key_in_a_late_tile(cuda, dtype, lq, logit):
     exp = 1.0 - 2.0 * share
     # exponentials: 7.5e-5 of a weight where the polynomial takes it, 2^-22 otherwise
     assert (out.double() - exp).abs().max() <= 2 * share * (2 * UNIT[dtype] + 1e-4) + 2.0**-22
+
+
+def definition(q, k, v, seen, scale):
+    g = q.shape[1] // k.shape[1]
+    s = q.double() @ k.double().repeat_interleave(g, 1).transpose(-1, -2) * scale
+    return torch.softmax(s.masked_fill(~seen, -torch.inf), -1) @ v.double().repeat_interleave(g, 1)
+
+
+def window_seen(lq, keys, window, sinks):
+    p = torch.arange(keys - lq, keys, device="cuda")[:, None]
+    j = torch.arange(keys, device="cuda")[None]
+    return (j <= p) & ((j > p - window) | (j < sinks))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lq", [1, 200])
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_scores_move_by_their_own_error_only(cuda, dtype, lq, d):
+    """Scores in the hundreds.  Each is off by at most e = D 2^-24 sum |q k|
+    scale (f32 sums of D products), which moves the weights of a row by at most
+    exp(2e) - 1 in all; the rest as for small scores."""
+    keys, scale = 300, d**-0.5
+    q, k, v = rnd((1, 4, lq, d), dtype, 1) * 20, rnd((1, 2, keys, d), dtype, 2) * 20, rnd((1, 2, keys, d), dtype, 3)
+    got = api.attention_window(q, k, v, 150, 2).double()
+    exp = definition(q, k, v, window_seen(lq, keys, 150, 2), scale)
+    e = d * 2.0**-24 * scale * (q.double().abs() @ k.double().abs().repeat_interleave(2, 1).transpose(-1, -2)).amax(-1, keepdim=True)
+    u, top = UNIT[dtype], float(v.double().abs().max())
+    bound = (torch.expm1(2 * e) + 2 * u + 2.0**-12) * top + u * exp.abs()
+    assert bound.max() < 0.1 * top
+    assert ((got - exp).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lq", [1, 40])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("step", [0.125, 0.03125, 0.0078125, -0.125, -0.03125])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+def test_maximum_rises_from_tile_to_tile(cuda, dtype, lq, d, step, scale):
+    """Logits that rise (or fall) along the keys, by more and by less than 2^8
+    a tile, so that the running maximum and O are rescaled often or seldom."""
+    keys, pre = 600, 400
+    q, k, v = rnd((1, 4, lq, d), dtype, 1) * 0.05, rnd((1, 2, keys, d), dtype, 2), rnd((1, 2, keys, d), dtype, 3)
+    q[..., 0] = 1.0
+    k[..., 0] = (torch.arange(keys, device=cuda) * (step * scale)).to(dtype)
+    options = AttentionOptions(scale=scale)
+    u, top = UNIT[dtype], float(v.double().abs().max())
+    for window, sinks in ((1000, 0), (300, 4)):
+        got = api.attention_window(q, k, v, window, sinks, options=options).double()
+        exp = definition(q, k, v, window_seen(lq, keys, window, sinks), scale)
+        assert ((got - exp).abs() <= (2 * u + 2.0**-12) * top + u * exp.abs()).all()
+    got = api.attention_prefix(q, k[0, :, :pre], v[0, :, :pre], k[:, :, pre:], v[:, :, pre:], options=options).double()
+    exp = definition(q, k, v, window_seen(lq, keys, 1000, 0), scale)
+    assert ((got - exp).abs() <= (2 * u + 2.0**-12) * top + u * exp.abs()).all()
+    assert api.device_status() == 0
