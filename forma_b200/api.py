@@ -419,7 +419,7 @@ def attention_window(query, key, value, window: int, sinks: int = 0, lengths: Op
 def attention_prefix(query, prefix_key, prefix_value, key, value, lengths: Optional[torch.Tensor] = None,
                      options: AttentionOptions = AttentionOptions(), out: Optional[torch.Tensor] = None):
     """Attention of a batch [B, H, L, D] that continues one shared prefix
-    [Hkv, P, D], read once for the whole batch, over each sequence's own keys
+    [Hkv, P, D], read once for many rows of the batch, over each sequence's own keys
     [B, Hkv, S, D] (causal, ``lengths`` of them filled, as in
     :func:`attention_window`)."""
     return bind().attention_prefix(query, prefix_key, prefix_value, key, value, lengths, options.scale, options.causal, out)

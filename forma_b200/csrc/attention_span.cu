@@ -87,11 +87,15 @@ __device__ __forceinline__ Reach reach(const SpanBase& s, int32_t la, int32_t lb
 // P is handed over in two halves, so that the products of its first 64 keys run
 // while the others' exponentials are taken (164 -> 149 us for 8192 queries,
 // window 1024, 32/8 heads, D = 128).
+// P is rounded to the operands' type, the only one the matrix unit takes beside
+// V's.  With the output's own rounding it is the result's error: 0.0022 (BF16)
+// and 2.9e-4 (F16) of the outputs' norm, 0.0016 and 2.1e-4 by the output alone.
 // Bound: the chain of one tile's softmax (1850 cycles), the second half of its
 // P V and its next S (800) and their hand-overs; the tensor pipe is busy 2100
-// of a key tile's 3400 cycles.  8192 queries, 32/8 heads, D = 128, calls back to
-// back: window 1024 147 us (870 TFLOP/s over the visible pairs), 4096 353 us
-// (1170), no window 450 us (1220).
+// of a key tile's 3400 cycles.  8192 queries, 32/8 heads, D = 128, short runs of
+// calls back to back: window 1024 149 us (860 TFLOP/s over the visible pairs),
+// 4096 355 us (1170), no window 455 us (1210); in longer runs, under the power
+// cap, window 1024 takes 166 to 170 us.
 // Otherwise this is attn_fwd_kernel's pipeline; see there for the orderings and
 // the bounded waits, and weight_shift for the scale of the weights.
 struct SpanTileParams {
@@ -892,7 +896,8 @@ __global__ void __launch_bounds__(256) span_merge_kernel(SpanMergeParams p) {
 // warp-level MMAs (m16n8k16) per (sequence, key/value head), as in
 // attn_decode16_kernel (see there for the depth permutation and the combine),
 // over exactly the keys that the rows see: virtual key v of a sequence is key
-// v < s ? v : v + lo - s, with s first keys and the window [lo, hi].
+// v < s ? v : v + lo - s, with s first keys and the window [lo, hi].  Weights are
+// rounded and summed as span_tile_kernel's.
 //
 // Work split: the visible keys of all (sequence, key/value head) units, in
 // 64-key tiles, are dealt out evenly: CTA c takes the tiles [c q, (c + 1) q)
@@ -969,8 +974,8 @@ __global__ void __launch_bounds__(32 * NW) span_decode_kernel(SpanDecodeParams p
     constexpr int QW = D / 8, KS = D / 16, NJ = D / 8, CPR = C::CPR, STAGE = C::STAGE;
     extern __shared__ uint4 dsm[];
     __shared__ uint32_t scan[NW], found[2], last;
-    __shared__ float2 heads[16];             // the CTA's combined records: heads, and rows in
-    __shared__ float wts[16][NW];    // the upper part of warp 0's ring
+    __shared__ float2 heads[16];     // the CTA's combined records: heads; rows in `cmb`, the upper part of warp 0's ring
+    __shared__ float wts[16][NW];    // the warps' weights in them
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     uint4* ring = dsm + (size_t)warp * C::RING;
@@ -1384,8 +1389,10 @@ float weight_shift(uint32_t fmt, uint64_t keys) {
 // the accumulator and cut them off at 2^-25 of it, so n keys can leave up to
 // n 2^-25 of a row out of O (measured with 16384 keys of weight 2^-18 to 2^-27
 // beside one of 1: 2^-25.1 a key at most; below 2^-25 nothing of them arrives).
-// At u 2^26 keys, u the type's unit roundoff, that is 2 u, what the weights' own
-// rounding may cost; longer ranges are divided and joined in f32.
+// At u 2^25 keys, u the type's unit roundoff (2^-8, 2^-11), that is u, no more than
+// a weight's own rounding; longer ranges are divided and joined in f32.  (32/8 heads,
+// D = 128, F16: a prompt of 32768 without a window 8.4 -> 9.1 ms, single tokens
+// of 16 sequences of 65536 keys 681 -> 689 us.)
 uint64_t range_keys(uint32_t fmt) { return fmt ? 131072 : 16384; }
 
 uint64_t largest_divisor(uint64_t n, uint64_t most) {

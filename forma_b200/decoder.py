@@ -17,7 +17,7 @@ with attention over everything and the others with a window::
     logits = LN(x) W_head                    low dtype; token_logprobs, token_logprobs_grad
 
 Caches.  A full layer's prompt keys are stored once, whatever the number of
-continuations, and read once per call (attention_prefix).  A windowed layer
+continuations, and shared by their rows in every call (attention_prefix).  A windowed layer
 sees only its first `sinks` and last `window` positions, so each continuation
 starts from a copy of the prompt's first `sinks` and last `window - 1` rows:
 dropping the rows between shifts the positions of what follows by one amount

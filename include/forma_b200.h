@@ -240,7 +240,11 @@ int fb_attention_low(const fb_tensor* query, const fb_tensor* key,
  * or BF16 of one dtype; `output` is f32, or the operands' 16-bit dtype
  * (rounded once, nearest even).  With 16-bit operands, D = value depth in
  * {64, 128}, contiguous depth and 16-byte aligned rows the tensor cores serve
- * the call; other geometries run CUDA-core kernels in f64.
+ * the call: the softmax weights are rounded to the operands' type (unit
+ * roundoff u: 2^-8 BF16, 2^-11 F16) and up to u of a row's smallest weights may
+ * drop out, so that a result is within (3u + 2^-12) max|v| of the softmax of
+ * the f32 scores before its own rounding.  Other geometries run CUDA-core
+ * kernels in f64.  A row that sees a NaN, or a score of +inf, is NaN.
  *
  * `lengths` (NULL, or u32 of the batch dims, one stride) says how many of
  * each sequence's key rows are filled: n_b = min(lengths[b], Lk); the rest of
@@ -260,7 +264,8 @@ int fb_attention_window(const fb_tensor* query, const fb_tensor* key, const fb_t
 
 /* fb_attention_prefix: a batch of sequences that continue one shared prefix.
  * query [B, H, L, D]; prefix_key [Hkv, P, D] and prefix_value [Hkv, P, Dv]
- * are visible to every query and read once for the whole batch; key
+ * are visible to every query, and on the tensor cores read once for up to 256
+ * query rows of the batch (the CUDA-core kernels read them per query row); key
  * [B, Hkv, S, D] and value [B, Hkv, S, Dv] are each sequence's own keys, key
  * j visible iff j < n_b and j <= p (positions and n_b as above, counted
  * within the sequence's own keys).  P or S may be 0. */

@@ -1,8 +1,8 @@
 """What the 16-bit weights of the span attentions keep of a softmax.
 
-Tolerance, as in the other span tests: u the unit roundoff of the type (2^-9
-BF16, 2^-12 F16), |error| <= (2u + 2^-12) max|v| + u |e|, unless a test says
-less."""
+Tolerance, as in the other span tests: |error| <= (2u + 2^-12) max|v| + u |e|
+with u = 2^-9 (BF16) and 2^-12 (F16), half the type's unit roundoff, unless a
+test says less."""
 
 import math
 
