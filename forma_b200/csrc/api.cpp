@@ -741,8 +741,13 @@ int token_logprobs_grad_impl(const fb_tensor* logits, const fb_tensor* targets, 
         FB_TRY(row_f32(entropy, "entropy", lead, false, &a.entropy));
     }
     const bool low_out = grad && is_low(grad->dtype) && grad->dtype == in.dtype;
-    FB_TRY(check_output(grad, "grad_logits", in.dims, low_out ? in.dtype : (uint32_t)FB_F32, &out));
+    // (not check_output: logits are often rows of something wider, and an
+    // update in place has their layout)
+    FB_TRY(view_of(grad, "grad_logits", &out));
+    if (out.dtype != (low_out ? in.dtype : (uint32_t)FB_F32)) return fail(FB_ERR_DTYPE, "grad_logits: output dtype mismatch");
+    if (out.dims != in.dims) return fail(FB_ERR_INVALID_INPUT, "grad_logits needs the logits' dims");
     if (out.count == 0) return FB_OK;
+    if (!distinct_addresses(out)) return fail(FB_ERR_INVALID_INPUT, "grad_logits layout must address each element once");
     // An update in place reads each logit before it writes it: only the
     // identical view may share memory.
     auto span = [](const View& v) {
@@ -1281,20 +1286,7 @@ int fb_add(const fb_tensor* a, const fb_tensor* b, fb_tensor* output, void* stre
     if (x.dtype != FB_F32 || y.dtype != FB_F32 || out.dtype != FB_F32) return fail(FB_ERR_DTYPE, "add needs f32 operands");
     if (x.dims != out.dims || y.dims != out.dims) return fail(FB_ERR_INVALID_INPUT, "add operand dims differ from output");
     if (out.count == 0) return FB_OK;
-    // The output may be any layout that gives every element its own address:
-    // non-unit axes sorted by stride, each stride at least the extent of the
-    // axes inside it.
-    {
-        std::vector<std::pair<uint64_t, uint64_t>> ax;
-        for (size_t i = 0; i < out.dims.size(); ++i)
-            if (out.dims[i] > 1) ax.push_back({out.strides[i], out.dims[i]});
-        std::sort(ax.begin(), ax.end());
-        uint64_t extent = 1;
-        for (auto& e : ax) {
-            if (e.first < extent) return fail(FB_ERR_INVALID_INPUT, "add output layout must address each element once");
-            extent = e.first * e.second;
-        }
-    }
+    if (!distinct_addresses(out)) return fail(FB_ERR_INVALID_INPUT, "add output layout must address each element once");
     // An operand may share memory with the output only as the identical view.
     auto same_view = [&](const View& v) {
         return v.data == out.data && v.offset == out.offset && v.strides == out.strides;

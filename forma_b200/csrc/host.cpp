@@ -175,6 +175,19 @@ Error check_output(const fb_tensor* t, const char* name, const Dims& dims, uint3
     return {};
 }
 
+bool distinct_addresses(const View& v) {
+    std::vector<std::pair<uint64_t, uint64_t>> axes;
+    for (size_t i = 0; i < v.dims.size(); ++i)
+        if (v.dims[i] > 1) axes.push_back({v.strides[i], v.dims[i]});
+    std::sort(axes.begin(), axes.end());
+    uint64_t extent = 1;
+    for (auto& a : axes) {
+        if (a.first < extent) return false;
+        extent = a.first * a.second;
+    }
+    return true;
+}
+
 // ------------------------------------------------------------------ conv
 
 Error conv_plan(const Dims& input, const Dims& weight, const fb_conv_options* o, ConvPlan* plan) {

@@ -62,6 +62,10 @@ bool is_contiguous(const View& v);
 // block is allowed, so a channels-last conv output can be a permuted view).
 Error check_output(const fb_tensor* t, const char* name, const Dims& dims, uint32_t dtype, View* out);
 
+// Whether every element has its own address, gaps allowed: non-unit axes
+// sorted by stride, each stride at least the extent of the axes inside it.
+bool distinct_addresses(const View& v);
+
 uint64_t dtype_size(uint32_t dtype);
 bool is_low(uint32_t dtype);
 

@@ -139,3 +139,16 @@ def test_token_gradient_arguments():
     raises(bwd(g=desc([5, 100], _lib.F32, ptr=0x10000)), "InvalidInput")             # in place needs the logits' type
     e = desc([0], _lib.F32)
     assert bwd(x=desc([0, 9]), t=desc([0], _lib.U32), lse=e, gl=e, g=desc([0, 9])) == 0
+
+
+def test_token_gradient_layouts():
+    """Rows with gaps are an output (the launch then needs a GPU); rows on one another are not."""
+    lib = api.lib()
+    x, t, f = desc([5, 100]), desc([5], _lib.U32), desc([5], _lib.F32)
+
+    def bwd(g):
+        return lib.fb_token_logprobs_grad(ref(x), ref(t), ref(f), ref(f), None, None, ref(g), None)
+
+    raises(bwd(desc([5, 100], strides=[99, 1], storage=600, ptr=0x900000)), "InvalidInput")
+    raises(bwd(desc([5, 100], strides=[0, 1], ptr=0x900000)), "InvalidInput")
+    raises(bwd(desc([5, 100], strides=[1, 4], storage=600, ptr=0x900000)), "InvalidInput")

@@ -373,3 +373,27 @@ def test_forward_parts_with_few_values(cuda, dtype, cols, top):
     t = targets_for(x, 90)
     t[2] = 7
     check_forward(x, t, top)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,view", [((50, 5000), lambda w: w[:, :4990]), ((50, 5000), lambda w: w[:, 3:4001]),
+                                        ((20, 7, 1000), lambda w: w[:, -1]), ((9, 6, 515), lambda w: w[:, ::2, 1:514]),
+                                        ((30, 2000), lambda w: w[:, ::2]), ((1, 70000), lambda w: w[:, 8:69999])])
+def test_grad_into_rows_of_something_wider(cuda, dtype, shape, view):
+    """In place on a part of a padded buffer, and into a part of another: what
+    lies between the rows keeps its bits."""
+    wide = rnd(shape, dtype, 11)
+    x = view(wide)
+    t = targets_for(x, 1)
+    gl, gh = rnd(t.shape, torch.float32, 2), rnd(t.shape, torch.float32, 3)
+    st = api.token_logprobs(x, t)
+    untouched = torch.ones(shape, dtype=torch.bool, device=cuda)
+    view(untouched).fill_(False)
+    for out_dtype in (torch.float32, dtype):
+        other = torch.full(shape, 7.0, dtype=out_dtype, device=cuda)
+        got = check_grad(x, t, gl, gh, view(other))
+        assert (other[untouched] == 7.0).all()
+    before = wide.clone()
+    again = api.token_logprobs_grad(x, t, st.logsumexp, gl, st.entropy, gh, out=x)
+    assert again is x and torch.equal(x, got) and torch.equal(wide[untouched], before[untouched])
+    assert api.device_status() == 0
