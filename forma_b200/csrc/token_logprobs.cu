@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(BLOCK) token_grad_rows_kernel(TokenGradArgs a)
 // Bound: HBM (the ex2 unit is 3/4 busy at the full rate with 16-bit logits),
 // and the few microseconds per row in which its CTA puts the alternatives in
 // order and loads nothing.  8200 x 131072 BF16: 375 us, 5.7 TB/s; with 5
-// alternatives 415 us, 5.2 TB/s; 2048 rows 104 and 121 to 127 us; f32 1024 x 131072
+// alternatives 415 us, 5.2 TB/s; 2048 rows 104 and 121 to 128 us; f32 1024 x 131072
 // 86 and 96 us, 6.2 and 5.6 TB/s.  64 x 32000 with 8: 11 us, 1 x 50021 with 20:
 // 12 us, latency.  (Measured and not kept: one persistent CTA per slot over
 // several rows; a second launch that splits the rows of a partial last wave, 6%
@@ -699,7 +699,7 @@ int launch_t(const TokenArgs& a, cudaStream_t st) {
 // 0 or infinity.
 // Bound: HBM, one read and one write.  Loads are issued before the row's
 // scalars arrive; each block does one chunk of 4 vectors per thread.
-// 2048 x 131072 BF16: 170 to 183 us back to back (6.3 to 5.9 TB/s), 191 us (5.6
+// 2048 x 131072 BF16: 170 to 183 us back to back (6.3 to 5.9 TB/s), 191 to 193 us (5.6
 // TB/s) with other logits and another output every call; into f32 270 us, 6.0 TB/s.
 template <typename T, typename U>  // U: patterns of the output, T's own or f32's
 __global__ void __launch_bounds__(BLOCK) token_grad_stream_kernel(GradArgs a) {
